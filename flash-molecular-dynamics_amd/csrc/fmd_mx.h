@@ -1,0 +1,135 @@
+// Block-scaled numbers (32 columns of a row share a power of two) and the bf16 planes the products are made of.
+//
+//   4 bits   value = e2m1 * 2^(byte-127)            e2m1 in {0,.5,1,1.5,2,3,4,6}, two to a byte, even column low
+//   8 bits   value = int8 / 64 * 2^(byte-127)       int8 in [-127,127]
+//
+// byte = max(floor(log2 amax) - (4 bits: 2, 8 bits: 0), -127) + 127; a block that holds an Inf or a NaN gets byte 255
+// and stands for NaN.  Scaling by a power of two is exact, so the codes are a function of the input's bits alone.
+//
+// Planes: an fp32 value is the exact sum of three bf16 (truncation keeps 8 significant bits at a time), an fp16 value of
+// two, a bf16 value and every 4- or 8-bit block value is one.  A product of plane sums keeps the plane pairs (i, j) with
+// i + j < max(planes): what is dropped is below the last kept plane's last bit.  bf16 has fp32's range, so no operand
+// needs a scale of its own.
+#pragma once
+#include "fmd_common.h"
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+
+struct mx_bf16 { uint16_t u; };  // bf16 in memory
+
+template <class T> struct MxType;
+template <> struct MxType<float> {
+  static constexpr int planes = 3;
+  static __device__ __forceinline__ float to(float v) { return v; }
+  static __device__ __forceinline__ float from(float v) { return v; }
+};
+template <> struct MxType<_Float16> {
+  static constexpr int planes = 2;
+  static __device__ __forceinline__ float to(_Float16 v) { return (float)v; }
+  static __device__ __forceinline__ _Float16 from(float v) { return (_Float16)v; }
+};
+template <> struct MxType<mx_bf16> {
+  static constexpr int planes = 1;
+  static __device__ __forceinline__ float to(mx_bf16 v) { return __builtin_bit_cast(float, (uint32_t)v.u << 16); }
+  static __device__ __forceinline__ mx_bf16 from(float v) {  // nearest even
+    const __bf16 b = (__bf16)v;
+    return mx_bf16{__builtin_bit_cast(uint16_t, b)};
+  }
+};
+
+static inline int64_t mx_blocks(int64_t k) { return (k + 31) / 32; }
+static inline int64_t mx_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
+
+// pairs (i, j) of planes whose product is kept, the smallest first
+struct MxPairs { int n; int8_t a[6], b[6]; };
+static inline MxPairs mx_pairs(int pa, int pb) {
+  MxPairs p{};
+  const int top = pa > pb ? pa : pb;
+  for (int s = top - 1; s >= 0; --s)
+    for (int i = 0; i < pa; ++i) {
+      const int j = s - i;
+      if (j >= 0 && j < pb) { p.a[p.n] = (int8_t)i; p.b[p.n] = (int8_t)j; ++p.n; }
+    }
+  return p;
+}
+
+// ---- scales ---------------------------------------------------------------------------------------------------------
+// scale byte of a block from the largest bit pattern of |x| (an unsigned maximum: a NaN's pattern is above Inf's)
+template <int BITS>
+__device__ __forceinline__ uint32_t mx_scale_byte(uint32_t top) {
+  if (top >= 0x7f800000u) return 255u;
+  // floor(log2) of a subnormal is below every exponent the byte can hold
+  const int e = (int)(top >> 23) - (BITS == 4 ? 2 : 0);  // biased by 127 already
+  return e > 0 ? (uint32_t)e : 0u;
+}
+// 2^(byte-127) as fp32 (byte 0: the subnormal 2^-127; byte 255: NaN)
+__device__ __forceinline__ float mx_scale_value(uint32_t byte) {
+  return __builtin_bit_cast(float, byte == 0 ? 0x00400000u : byte == 255u ? 0x7fc00000u : byte << 23);
+}
+
+// 8-bit code of x in a block of the given scale byte
+__device__ __forceinline__ int mx_code8(float x, uint32_t byte) {
+  const float q = __builtin_rintf(__builtin_ldexpf(x, 133 - (int)byte));  // 64 x / 2^E; v_ldexp_f32 rounds once
+  const int i = (int)fminf(fmaxf(q, -127.f), 127.f);
+  return byte == 255u ? 0 : i;
+}
+__device__ __forceinline__ float mx_value8(int code, uint32_t byte) {
+  return byte == 255u ? __builtin_nanf("") : __builtin_ldexpf((float)code, (int)byte - 133);
+}
+// eight 4-bit codes (columns 0..7 from the low bits up) of a block of the given scale value
+__device__ __forceinline__ uint32_t mx_codes4(const float (&v)[8], float scale) {
+  uint32_t o = 0;
+  o = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(o, v[0], v[1], scale, 0);
+  o = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(o, v[2], v[3], scale, 1);
+  o = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(o, v[4], v[5], scale, 2);
+  o = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(o, v[6], v[7], scale, 3);
+  return o;
+}
+// eight 4-bit codes as bf16 (exact: e2m1 has two significant bits)
+__device__ __forceinline__ u32x4 mx_bf16_from4(uint32_t codes, float scale) {
+  u32x4 r;
+  r[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 0));
+  r[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 1));
+  r[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 2));
+  r[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 3));
+  return r;
+}
+
+// ---- planes -----------------------------------------------------------------------------------------------------------
+// two fp32 values -> one dword of bf16 pairs per plane.  Cutting off the low half keeps 8 significant bits and cannot
+// overflow; the remainder is exact.  x == hi for an Inf, whose remainder is then 0 and not Inf - Inf; a NaN whose low
+// half alone is set leaves a NaN remainder, so no NaN is lost.
+template <int P>
+__device__ __forceinline__ void mx_split2(float x, float y, uint32_t (&out)[P]) {
+  if constexpr (P == 1) {  // one plane: rounded to nearest even
+    bf16x2 b;
+    b[0] = (__bf16)x;
+    b[1] = (__bf16)y;
+    out[0] = __builtin_bit_cast(uint32_t, b);
+  } else {
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      const uint32_t ux = __builtin_bit_cast(uint32_t, x), uy = __builtin_bit_cast(uint32_t, y);
+      out[p] = __builtin_amdgcn_perm(uy, ux, 0x07060302u);
+      if (p + 1 < P) {
+        const float hx = __builtin_bit_cast(float, ux & 0xffff0000u), hy = __builtin_bit_cast(float, uy & 0xffff0000u);
+        x = x == hx ? 0.f : x - hx;
+        y = y == hy ? 0.f : y - hy;
+      }
+    }
+  }
+}
+template <int P>
+__device__ __forceinline__ void mx_split8(const float (&v)[8], u32x4 (&out)[P]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    uint32_t o[P];
+    mx_split2<P>(v[2 * i], v[2 * i + 1], o);
+#pragma unroll
+    for (int p = 0; p < P; ++p) out[p][i] = o[p];
+  }
+}

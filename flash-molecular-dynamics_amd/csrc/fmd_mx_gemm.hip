@@ -1,0 +1,543 @@
+// The general product of block-scaled layers: any sizes, any type.
+//
+//   1. lay the operands out as K-contiguous rows of 128-byte tiles: bf16 planes (fmd_mx.h) for 32- and 16-bit operands and
+//      for 8-bit checkpoints, the 4-bit codes themselves where both operands are in 4 bits
+//   2. C = A B^T on the matrix cores, tile by tile
+//   3. where the rows of C are too few to fill the chip, the contraction is split and the parts are summed in a fixed order
+//
+// The transforms (tanh, the gradient's tanh', dequantisation) happen in step 1, once per element, or in the epilogue.
+#include <type_traits>
+
+#include "fmd_mx_host.h"
+
+namespace {
+
+// =====================================================================================================================
+// operand sources: eight neighbouring columns of one row as fp32
+// =====================================================================================================================
+template <class T, bool TANH>
+struct SrcDense {
+  const T* p;
+  int64_t cols;
+  bool vec;
+  __device__ __forceinline__ void load(int64_t row, int64_t c0, float (&v)[8]) const {
+    const T* r = p + row * cols;
+    if (vec && c0 + 8 <= cols) {
+      T t[8];
+#pragma unroll
+      for (int i = 0; i < (int)sizeof(T) / 2; ++i) ((u32x4*)t)[i] = *(const u32x4*)(r + c0 + i * (16 / sizeof(T)));
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = MxType<T>::to(t[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = c0 + i < cols ? MxType<T>::to(r[c0 + i]) : 0.f;
+    }
+    if constexpr (TANH)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = fmd_tanh(v[i]);  // tanh(0) = 0: padding stays zero
+  }
+};
+// a gradient times the derivative of the activation behind it.  AUX 1: aux = y in fp32, factor 1 - y^2; 2: aux = the factor in fp16
+template <class T, int AUX>
+struct SrcGrad {
+  const T* p;
+  const void* aux;
+  int64_t cols;
+  bool vec;
+  __device__ __forceinline__ void load(int64_t row, int64_t c0, float (&v)[8]) const {
+    SrcDense<T, false>{p, cols, vec}.load(row, c0, v);
+    if constexpr (AUX == 1) {
+      float y[8];
+      SrcDense<float, false>{(const float*)aux, cols, vec}.load(row, c0, y);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] *= 1.f - y[i] * y[i];
+    } else if constexpr (AUX == 2) {
+      float d[8];
+      SrcDense<_Float16, false>{(const _Float16*)aux, cols, vec}.load(row, c0, d);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] *= d[i];
+    }
+  }
+};
+// 8-bit checkpoint; codes [row][32 nb] are padded with zeros
+template <bool TANH>
+struct SrcI8 {
+  const uint8_t* codes;
+  const uint8_t* scales;
+  int64_t cols, nb;
+  __device__ __forceinline__ void load(int64_t row, int64_t c0, float (&v)[8]) const {
+    if (c0 >= cols) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = 0.f;
+      return;
+    }
+    const u32x2 c = *(const u32x2*)(codes + (row * nb) * 32 + c0);
+    const uint32_t byte = scales[row * nb + (c0 >> 5)];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float x = mx_value8((int)(int8_t)(c[i >> 2] >> (8 * (i & 3))), byte);
+      v[i] = c0 + i < cols ? (TANH ? fmd_tanh(x) : x) : 0.f;
+    }
+  }
+};
+struct SrcFp4 {
+  const uint8_t* codes;
+  const uint8_t* scales;
+  int64_t cols, nb;
+  __device__ __forceinline__ void load(int64_t row, int64_t c0, float (&v)[8]) const {
+    if (c0 >= cols) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = 0.f;
+      return;
+    }
+    const uint32_t c = *(const uint32_t*)(codes + (row * nb) * 16 + (c0 >> 1));
+    const u32x4 b = mx_bf16_from4(c, mx_scale_value(scales[row * nb + (c0 >> 5)]));
+#pragma unroll
+    for (int i = 0; i < 8; ++i)  // columns behind the last one hold whatever the caller's codes hold there
+      v[i] = c0 + i < cols ? __builtin_bit_cast(float, i & 1 ? b[i >> 1] & 0xffff0000u : b[i >> 1] << 16) : 0.f;
+  }
+};
+
+// rows x cols -> planes [P][rows][pad] (pad = cols rounded up to 64, zeros behind cols)
+template <class S, int P>
+__global__ __launch_bounds__(256) void planes_kernel(S src, int64_t rows, int64_t pad, uint16_t* __restrict__ out) {
+  const int64_t per = pad >> 3, total = rows * per;
+  for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < total; t += (int64_t)gridDim.x * 256) {
+    const int64_t row = t / per, c0 = (t - row * per) * 8;
+    float v[8];
+    src.load(row, c0, v);
+    u32x4 o[P];
+    mx_split8<P>(v, o);
+#pragma unroll
+    for (int p = 0; p < P; ++p) *(u32x4*)(out + (int64_t)p * rows * pad + row * pad + c0) = o[p];
+  }
+}
+
+// rows x cols -> planes [P][cols][pad] of the transposed matrix (pad = rows rounded up to 64, zeros behind rows); 64 x 64 tiles
+// through LDS, rows 66 halves apart so that neither side meets a bank twice more than it has to
+template <class S, int P>
+__global__ __launch_bounds__(256) void planes_t_kernel(S src, int64_t rows, int64_t cols, int64_t pad, uint16_t* __restrict__ out) {
+  __shared__ uint32_t tile[P][64][33];
+  const int64_t r0 = (int64_t)blockIdx.x * 64, c0 = (int64_t)blockIdx.y * 64;
+  const int t = threadIdx.x;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int r = (t >> 3) + 32 * i, c = (t & 7) * 8;
+    float v[8];
+    if (r0 + r < rows) {
+      src.load(r0 + r, c0 + c, v);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = 0.f;
+    }
+    u32x4 o[P];
+    mx_split8<P>(v, o);
+#pragma unroll
+    for (int p = 0; p < P; ++p)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) tile[p][r][(c >> 1) + j] = o[p][j];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int c = (t >> 3) + 32 * i, r = (t & 7) * 8;
+    if (c0 + c >= cols) continue;
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      u32x4 o;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t lo = tile[p][r + 2 * j][c >> 1], hi = tile[p][r + 2 * j + 1][c >> 1];
+        o[j] = c & 1 ? __builtin_amdgcn_perm(hi, lo, 0x07060302u) : __builtin_amdgcn_perm(hi, lo, 0x05040100u);
+      }
+      *(u32x4*)(out + ((int64_t)p * cols + c0 + c) * pad + r0 + r) = o;
+    }
+  }
+}
+
+// scales [rows][nb] -> [tile of 8 blocks][rows][8], zeros behind nb
+__global__ __launch_bounds__(256) void scale_tiles_kernel(const uint8_t* __restrict__ s, int64_t rows, int64_t nb, int64_t kt,
+                                                          uint64_t* __restrict__ out) {
+  for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < rows * kt; t += (int64_t)gridDim.x * 256) {
+    const int64_t q = t / rows, row = t - q * rows;
+    uint64_t v = 0;
+    for (int i = 0; i < 8; ++i)
+      if (q * 8 + i < nb) v |= (uint64_t)s[row * nb + q * 8 + i] << (8 * i);
+    out[t] = v;
+  }
+}
+
+// =====================================================================================================================
+// C[m,n] = epi(A B^T + bias): BM x BN tiles, TM x TN matrix tiles of 32 x 32 per wave, K tiles of 128 bytes a row
+// (64 bf16 or 256 4-bit elements), two LDS buffers filled by direct loads one tile ahead.
+//
+// LDS: slot (row, p) of 16 bytes holds granule p ^ ((row / T) & 7) of the row's tile, T the matrix tiles per wave in that
+// direction: the 32 lanes of a fragment read rows T*lane + t, so eight neighbouring lanes meet eight different positions.
+// That row order also gives a lane T neighbouring columns of C.
+// =====================================================================================================================
+__device__ u32x4 mx_zero_granule;
+
+struct GemmArgs {
+  const char *a, *b;
+  int64_t a_plane, b_plane, a_pitch, b_pitch;  // bytes
+  const uint64_t *sa, *sb;                     // 4-bit operands: scales [tile][row][8]
+  int m, n, kt, granules, tiles_m, tiles_n, splits, npairs;
+  uint32_t pa, pb;                             // planes of pair i: bits 2i, 2i+1
+  MxEpilogue e;
+  float* partial;  // [splits][m][n], or null: the epilogue writes C
+};
+
+template <class T>
+__device__ __forceinline__ void finish_one(const MxEpilogue& e, int64_t row, int64_t col, int64_t ld, float v) {
+  if (e.bias) v += MxType<T>::to(((const T*)e.bias)[col]);
+  if (e.tanh) v = fmd_tanh(v);
+  if (e.dact) ((_Float16*)e.dact)[row * ld + col] = (_Float16)(1.f - v * v);
+  if (e.codes8) {
+    const float t = fmd_tanh(mx_value8((int)(int8_t)e.codes8[row * e.nb8 * 32 + col], e.scales8[row * e.nb8 + (col >> 5)]));
+    v *= 1.f - t * t;
+  }
+  ((T*)e.out)[row * ld + col] = MxType<T>::from(v);
+}
+
+template <class T, bool FP4, int WM, int WN, int TM, int TN>
+__global__ __launch_bounds__(64 * WM * WN) void gemm_kernel(const GemmArgs g) {
+  constexpr int BM = 32 * WM * TM, BN = 32 * WN * TN, NW = WM * WN, SLOTS = (BM + BN) * 8, LOADS = SLOTS / (64 * NW);
+  __shared__ __attribute__((aligned(16))) char lds[2 * (BM + BN) * 128];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, j = lane & 31, h = lane >> 5;
+  const int wm = wave / WN, wn = wave % WN;
+  // one XCD gets a run of neighbouring tiles (workgroups are dealt to the eight XCDs in turn), eight tile rows at a time
+  int bid = blockIdx.x;
+  const int tiles = g.tiles_m * g.tiles_n;
+  if ((tiles & 7) == 0) bid = (bid & 7) * (tiles >> 3) + (bid >> 3);
+  const int group = 8 * g.tiles_n, first = bid / group * 8, high = min(8, g.tiles_m - first);
+  const int m0 = (first + bid % group % high) * BM, n0 = bid % group / high * BN;
+  const int split = blockIdx.y;
+  const int all = g.npairs * g.kt, begin = (int)((int64_t)all * split / g.splits), end = (int)((int64_t)all * (split + 1) / g.splits);
+
+  // this wave's direct loads: byte offset of (row, granule) and the granule's number
+  int64_t off[LOADS];
+  int gran[LOADS];
+#pragma unroll
+  for (int i = 0; i < LOADS; ++i) {
+    const int slot = (i * NW + wave) * 64 + lane, r = slot >> 3, p = slot & 7;
+    const bool is_a = (i * NW + wave) * 64 < BM * 8;  // uniform: BM * 8 is a multiple of 64
+    const int rr = is_a ? r : r - BM;
+    gran[i] = p ^ ((is_a ? rr / TM : rr / TN) & 7);
+    const int row = is_a ? min(m0 + rr, g.m - 1) : min(n0 + rr, g.n - 1);
+    off[i] = (int64_t)row * (is_a ? g.a_pitch : g.b_pitch) + gran[i] * 16;
+  }
+  auto issue = [&](int pair, int t, char* buf) {
+    const char* pa = g.a + (g.pa >> 2 * pair & 3) * g.a_plane + (int64_t)t * 128;
+    const char* pb = g.b + (g.pb >> 2 * pair & 3) * g.b_plane + (int64_t)t * 128;
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const bool is_a = (i * NW + wave) * 64 < BM * 8;
+      const char* src = (is_a ? pa : pb) + off[i];
+      if (FP4 && t * 8 + gran[i] >= g.granules) src = (const char*)&mx_zero_granule;
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
+                                       (__attribute__((address_space(3))) void*)(buf + (i * NW + wave) * 1024), 16, 0, 0);
+    }
+  };
+  f32x16 acc[TM][TN];
+#pragma unroll
+  for (int a = 0; a < TM; ++a)
+#pragma unroll
+    for (int b = 0; b < TN; ++b)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[a][b][r] = 0.f;
+
+  uint64_t sa_next[TM], sb_next[TN];
+  auto load_scales = [&](int t) {
+    if constexpr (FP4) {
+#pragma unroll
+      for (int a = 0; a < TM; ++a) sa_next[a] = g.sa[(int64_t)t * g.m + min(m0 + (wm * 32 + j) * TM + a, g.m - 1)];
+#pragma unroll
+      for (int b = 0; b < TN; ++b) sb_next[b] = g.sb[(int64_t)t * g.n + min(n0 + (wn * 32 + j) * TN + b, g.n - 1)];
+    }
+  };
+  uint32_t sa[TM], sb[TN];
+  auto take_scales = [&]() {
+    if constexpr (FP4) {  // bytes h, h+2, h+4, h+6: the scales of this half wave's block in each of the four steps
+      const uint32_t pick = h ? 0x07050301u : 0x06040200u;
+#pragma unroll
+      for (int a = 0; a < TM; ++a) sa[a] = __builtin_amdgcn_perm((uint32_t)(sa_next[a] >> 32), (uint32_t)sa_next[a], pick);
+#pragma unroll
+      for (int b = 0; b < TN; ++b) sb[b] = __builtin_amdgcn_perm((uint32_t)(sb_next[b] >> 32), (uint32_t)sb_next[b], pick);
+    }
+  };
+  auto compute = [&](const char* buf) {
+    const char* la = buf + (wm * 32 + j) * TM * 128;
+    const char* lb = buf + BM * 128 + (wn * 32 + j) * TN * 128;
+#define MX_STEP(s)                                                                                                          \
+  {                                                                                                                         \
+    const int at = (((s) * 2 + h) ^ (j & 7)) * 16;                                                                          \
+    u32x4 fa[TM], fb[TN];                                                                                                   \
+    _Pragma("unroll") for (int a = 0; a < TM; ++a) fa[a] = *(const u32x4*)(la + a * 128 + at);                              \
+    _Pragma("unroll") for (int b = 0; b < TN; ++b) fb[b] = *(const u32x4*)(lb + b * 128 + at);                              \
+    _Pragma("unroll") for (int a = 0; a < TM; ++a) _Pragma("unroll") for (int b = 0; b < TN; ++b) {                         \
+      if constexpr (FP4) {                                                                                                  \
+        const i32x8 xa = {(int)fa[a][0], (int)fa[a][1], (int)fa[a][2], (int)fa[a][3], 0, 0, 0, 0};                          \
+        const i32x8 xb = {(int)fb[b][0], (int)fb[b][1], (int)fb[b][2], (int)fb[b][3], 0, 0, 0, 0};                          \
+        acc[a][b] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(xa, xb, acc[a][b], 4, 4, (s), (int)sa[a], (s), (int)sb[b]); \
+      } else {                                                                                                              \
+        acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, fa[a]), __builtin_bit_cast(bf16x8, fb[b]), \
+                                                            acc[a][b], 0, 0, 0);                                            \
+      }                                                                                                                     \
+    }                                                                                                                       \
+  }
+    MX_STEP(0) MX_STEP(1) MX_STEP(2) MX_STEP(3)
+#undef MX_STEP
+  };
+
+  int pair = begin / g.kt, t = begin - pair * g.kt, half = 0;
+  if (begin < end) {
+    issue(pair, t, lds);
+    load_scales(t);
+  }
+  for (int it = begin; it < end; ++it) {
+    // this tile has landed for every wave, and every wave is done with the other buffer
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    take_scales();
+    if (++t == g.kt) t = 0, ++pair;
+    if (it + 1 < end) {
+      issue(pair, t, lds + ((BM + BN) * 128 - half));
+      load_scales(t);
+    }
+    compute(lds + half);
+    half = (BM + BN) * 128 - half;
+  }
+
+  // a lane's TN columns are neighbours: stored together where every row starts on a multiple of them
+  const int64_t ld = g.n, col = n0 + (wn * 32 + j) * TN;
+  const bool whole = TN == 2 && (g.n & 1) == 0 && col < g.n;
+  auto store = [&](auto finish) {
+#pragma unroll
+    for (int a = 0; a < TM; ++a)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int64_t row = m0 + (wm * 32 + (r & 3) + 8 * (r >> 2) + 4 * h) * TM + a;
+        if (row >= g.m) continue;
+        finish(row, &acc[a], r);
+      }
+  };
+  auto write = [&](auto* p, const float (&v)[TN]) {  // p: (row, col) of the output
+    using U = typename std::remove_reference<decltype(*p)>::type;
+    if (whole) {
+      struct alignas(sizeof(U) * TN) Vec { U e[TN]; } o;
+#pragma unroll
+      for (int b = 0; b < TN; ++b) o.e[b] = MxType<U>::from(v[b]);
+      *(Vec*)p = o;
+    } else {
+#pragma unroll
+      for (int b = 0; b < TN; ++b)
+        if (col + b < g.n) p[b] = MxType<U>::from(v[b]);
+    }
+  };
+  float v[TN];
+  if (g.partial) {
+    store([&](int64_t row, const f32x16(*c)[TN], int r) {
+#pragma unroll
+      for (int b = 0; b < TN; ++b) v[b] = (*c)[b][r];
+      write(g.partial + ((int64_t)split * g.m + row) * ld + col, v);
+    });
+  } else if (g.e.codes8) {
+    store([&](int64_t row, const f32x16(*c)[TN], int r) {
+      if (col >= g.n) return;
+      const uint32_t byte = g.e.scales8[row * g.e.nb8 + (col >> 5)];
+#pragma unroll
+      for (int b = 0; b < TN; ++b) {  // col is a multiple of TN: one block
+        const float x = fmd_tanh(mx_value8((int)(int8_t)g.e.codes8[row * g.e.nb8 * 32 + col + b], byte));
+        v[b] = (*c)[b][r] * (1.f - x * x);
+      }
+      write((T*)g.e.out + row * ld + col, v);
+    });
+  } else {
+    float bias[TN] = {};
+    if (g.e.bias)
+#pragma unroll
+      for (int b = 0; b < TN; ++b)
+        if (col + b < g.n) bias[b] = MxType<T>::to(((const T*)g.e.bias)[col + b]);
+    if (g.e.tanh) {
+      store([&](int64_t row, const f32x16(*c)[TN], int r) {
+#pragma unroll
+        for (int b = 0; b < TN; ++b) v[b] = fmd_tanh((*c)[b][r] + bias[b]);
+        write((T*)g.e.out + row * ld + col, v);
+        if (g.e.dact) {
+#pragma unroll
+          for (int b = 0; b < TN; ++b) v[b] = 1.f - v[b] * v[b];
+          write((_Float16*)g.e.dact + row * ld + col, v);
+        }
+      });
+    } else {
+      store([&](int64_t row, const f32x16(*c)[TN], int r) {
+#pragma unroll
+        for (int b = 0; b < TN; ++b) v[b] = (*c)[b][r] + bias[b];
+        write((T*)g.e.out + row * ld + col, v);
+      });
+    }
+  }
+}
+
+// out = epi(sum over parts), in the parts' order
+template <class T>
+__global__ __launch_bounds__(256) void sum_parts_kernel(const float* __restrict__ parts, int64_t count, int64_t m, int64_t n,
+                                                        MxEpilogue e) {
+  for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < m * n; t += (int64_t)gridDim.x * 256) {
+    float v = 0.f;
+    for (int64_t s = 0; s < count; ++s) v += parts[s * m * n + t];
+    const int64_t row = t / n;
+    finish_one<T>(e, row, t - row * n, n, v);
+  }
+}
+
+// column sums of a gradient: part [blockIdx.y] of 64 columns
+template <class S>
+__global__ __launch_bounds__(256) void column_sums_kernel(S src, int64_t rows, int64_t cols, int64_t rows_per_part,
+                                                          float* __restrict__ part) {
+  __shared__ float lds[32][64];
+  const int t = threadIdx.x, c = (t & 7) * 8;
+  const int64_t c0 = (int64_t)blockIdx.x * 64, r0 = (int64_t)blockIdx.y * rows_per_part;
+  const int64_t r1 = min(rows, r0 + rows_per_part);
+  float s[8] = {};
+  for (int64_t r = r0 + (t >> 3); r < r1; r += 32) {
+    float v[8];
+    if (c0 + c < cols) {
+      src.load(r, c0 + c, v);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s[i] += v[i];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) lds[t >> 3][c + i] = s[i];
+  __syncthreads();
+  if (t < 64 && c0 + t < cols) {
+    float v = 0.f;
+    for (int i = 0; i < 32; ++i) v += lds[i][t];
+    part[(int64_t)blockIdx.y * cols + c0 + t] = v;
+  }
+}
+
+int grid_for(int64_t threads) {
+  const int64_t g = (threads + 255) / 256;
+  return (int)(g < 1 ? 1 : g < 8192 ? g : 8192);
+}
+
+template <class S, int P>
+void run_planes(S src, int64_t rows, int64_t pad, void* out, hipStream_t s) {
+  planes_kernel<S, P><<<grid_for(rows * (pad >> 3)), 256, 0, s>>>(src, rows, pad, (uint16_t*)out);
+}
+template <class S, int P>
+void run_planes_t(S src, int64_t rows, int64_t cols, int64_t pad, void* out, hipStream_t s) {
+  const dim3 grid((unsigned)(pad / 64), (unsigned)((cols + 63) / 64));
+  planes_t_kernel<S, P><<<grid, 256, 0, s>>>(src, rows, cols, pad, (uint16_t*)out);
+}
+
+bool vec_ok(const void* p, int64_t cols, int size) { return ((uintptr_t)p & 15) == 0 && cols * size % 16 == 0; }
+
+}  // namespace
+
+// ---- host ------------------------------------------------------------------------------------------------------------
+void mx_planes(const MxSource& q, int64_t rows, int64_t cols, bool transposed, void* out, hipStream_t s) {
+  if (rows < 1) return;
+  const int64_t pad = mx_up(transposed ? rows : cols, 64);
+#define MX_RUN(S, P, ...)                                                        \
+  do {                                                                           \
+    if (transposed) run_planes_t<S, P>(S __VA_ARGS__, rows, cols, pad, out, s);  \
+    else run_planes<S, P>(S __VA_ARGS__, rows, pad, out, s);                     \
+  } while (0)
+#define MX_TYPED(T, P)                                                                                                   \
+  do {                                                                                                                   \
+    const bool vec = vec_ok(q.p, cols, sizeof(T));                                                                       \
+    if (q.kind == MX_SRC_DENSE) MX_RUN(MX_ARG(SrcDense<T, false>), P, {(const T*)q.p, cols, vec});                       \
+    else if (q.kind == MX_SRC_TANH) MX_RUN(MX_ARG(SrcDense<T, true>), P, {(const T*)q.p, cols, vec});                    \
+    else if (q.kind == MX_SRC_GRAD_Y)                                                                                    \
+      MX_RUN(MX_ARG(SrcGrad<T, 1>), P, {(const T*)q.p, q.aux, cols, vec && vec_ok(q.aux, cols, 4)});                     \
+    else if (q.kind == MX_SRC_GRAD_D)                                                                                    \
+      MX_RUN(MX_ARG(SrcGrad<T, 2>), P, {(const T*)q.p, q.aux, cols, vec && vec_ok(q.aux, cols, 2)});                     \
+    else if (q.kind == MX_SRC_I8_TANH)                                                                                   \
+      MX_RUN(SrcI8<true>, P, {(const uint8_t*)q.p, (const uint8_t*)q.aux, cols, mx_blocks(cols)});                       \
+  } while (0)
+#define MX_ARG(...) __VA_ARGS__
+  if (q.kind == MX_SRC_I8) MX_RUN(SrcI8<false>, 1, {(const uint8_t*)q.p, (const uint8_t*)q.aux, cols, mx_blocks(cols)});
+  else if (q.kind == MX_SRC_FP4) MX_RUN(SrcFp4, 1, {(const uint8_t*)q.p, (const uint8_t*)q.aux, cols, mx_blocks(cols)});
+  else if (q.dtype == FMD_F32) MX_TYPED(float, 3);
+  else if (q.dtype == FMD_F16) MX_TYPED(_Float16, 2);
+  else MX_TYPED(mx_bf16, 1);
+#undef MX_RUN
+#undef MX_TYPED
+#undef MX_ARG
+}
+
+void mx_scale_tiles(const void* scales, int64_t rows, int64_t nb, void* out, hipStream_t s) {
+  const int64_t kt = (nb + 7) / 8;
+  scale_tiles_kernel<<<grid_for(rows * kt), 256, 0, s>>>((const uint8_t*)scales, rows, nb, kt, (uint64_t*)out);
+}
+
+// rows of a large matrix tile are worth it once they fill the chip; else the small tile, and the contraction in parts
+MxProductPlan mx_product_plan(int64_t m, int64_t n, int64_t kt, int npairs) {
+  MxProductPlan p{};
+  const int64_t big = ((m + 255) / 256) * ((n + 255) / 256), small = ((m + 127) / 128) * ((n + 127) / 128);
+  p.big = big >= 192;
+  p.tiles = p.big ? big : small;
+  const int64_t its = kt * npairs;
+  int64_t s = p.tiles >= 192 ? 1 : 512 / p.tiles;
+  if (s > its / 4) s = its / 4;
+  if (s > 64) s = 64;
+  p.splits = (int)(s < 1 ? 1 : s);
+  return p;
+}
+
+template <class T, bool FP4>
+static void launch_gemm(const GemmArgs& g, bool big, hipStream_t s) {
+  const dim3 grid((unsigned)(g.tiles_m * g.tiles_n), (unsigned)g.splits);
+  if (big) gemm_kernel<T, FP4, 2, 4, 4, 2><<<grid, 512, 0, s>>>(g);
+  else gemm_kernel<T, FP4, 2, 2, 2, 2><<<grid, 256, 0, s>>>(g);
+}
+
+void mx_product(const MxOperand& a, const MxOperand& b, int64_t m, int64_t n, int64_t kt, const MxProductPlan& plan, int dtype,
+                const MxEpilogue& e, float* parts, hipStream_t s) {
+  GemmArgs g{};
+  g.a = (const char*)a.p, g.b = (const char*)b.p;
+  g.a_plane = a.plane, g.b_plane = b.plane, g.a_pitch = a.pitch, g.b_pitch = b.pitch;
+  g.sa = (const uint64_t*)a.scales, g.sb = (const uint64_t*)b.scales;
+  g.m = (int)m, g.n = (int)n, g.kt = (int)kt, g.granules = (int)(a.pitch / 16);
+  const int side = plan.big ? 256 : 128;
+  g.tiles_m = (int)((m + side - 1) / side), g.tiles_n = (int)((n + side - 1) / side), g.splits = plan.splits;
+  const MxPairs pairs = mx_pairs(a.planes, b.planes);
+  g.npairs = pairs.n;
+  for (int i = 0; i < pairs.n; ++i) g.pa |= (uint32_t)pairs.a[i] << 2 * i, g.pb |= (uint32_t)pairs.b[i] << 2 * i;
+  g.e = e;
+  g.partial = parts;
+  const bool fp4 = a.scales != nullptr;
+  if (parts || dtype == FMD_F32) fp4 ? launch_gemm<float, true>(g, plan.big, s) : launch_gemm<float, false>(g, plan.big, s);
+  else if (dtype == FMD_F16) fp4 ? launch_gemm<_Float16, true>(g, plan.big, s) : launch_gemm<_Float16, false>(g, plan.big, s);
+  else fp4 ? launch_gemm<mx_bf16, true>(g, plan.big, s) : launch_gemm<mx_bf16, false>(g, plan.big, s);
+}
+
+void mx_sum_parts(const float* parts, int64_t count, int64_t m, int64_t n, int dtype, const MxEpilogue& e, hipStream_t s) {
+  if (dtype == FMD_F32) sum_parts_kernel<float><<<grid_for(m * n), 256, 0, s>>>(parts, count, m, n, e);
+  else if (dtype == FMD_F16) sum_parts_kernel<_Float16><<<grid_for(m * n), 256, 0, s>>>(parts, count, m, n, e);
+  else sum_parts_kernel<mx_bf16><<<grid_for(m * n), 256, 0, s>>>(parts, count, m, n, e);
+}
+
+void mx_column_sums(const MxSource& q, int64_t rows, int64_t cols, int64_t parts, float* out, hipStream_t s) {
+  const dim3 grid((unsigned)((cols + 63) / 64), (unsigned)parts);
+  const int64_t per = (rows + parts - 1) / parts;
+#define MX_TYPED(T)                                                                                                        \
+  do {                                                                                                                     \
+    const bool vec = vec_ok(q.p, cols, sizeof(T));                                                                         \
+    if (q.kind == MX_SRC_DENSE)                                                                                            \
+      column_sums_kernel<<<grid, 256, 0, s>>>(SrcDense<T, false>{(const T*)q.p, cols, vec}, rows, cols, per, out);         \
+    else if (q.kind == MX_SRC_GRAD_Y)                                                                                      \
+      column_sums_kernel<<<grid, 256, 0, s>>>(SrcGrad<T, 1>{(const T*)q.p, q.aux, cols, vec && vec_ok(q.aux, cols, 4)},    \
+                                              rows, cols, per, out);                                                       \
+    else                                                                                                                   \
+      column_sums_kernel<<<grid, 256, 0, s>>>(SrcGrad<T, 2>{(const T*)q.p, q.aux, cols, vec && vec_ok(q.aux, cols, 2)},    \
+                                              rows, cols, per, out);                                                       \
+  } while (0)
+  if (q.dtype == FMD_F32) MX_TYPED(float);
+  else if (q.dtype == FMD_F16) MX_TYPED(_Float16);
+  else MX_TYPED(mx_bf16);
+#undef MX_TYPED
+}

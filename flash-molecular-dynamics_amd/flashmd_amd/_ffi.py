@@ -36,6 +36,18 @@ SIGNATURES = {
     "fmd_linear_f16": (I32, [P, P, P, I32, I64, I64, I64, P]),
     "fmd_tanh_bwd_grad_x_f16": (I32, [P, I32, P, P, P, I64, I64, I64, P]),
     "fmd_matmul_f32_f16_to_f16": (I32, [P, P, P, I64, I64, I64, P]),
+    "fmd_mxfp4_quantize": (I32, [P, I32, I64, I64, P, P, P]),
+    "fmd_mxfp4_dequantize": (I32, [P, P, I64, I64, P, I32, P]),
+    "fmd_mxint8_quantize": (I32, [P, I32, I64, I64, P, P, P]),
+    "fmd_mxint8_dequantize": (I32, [P, P, I64, I64, P, I32, P]),
+    "fmd_mxfp4_linear_workspace_bytes": (I64, [I32, I64, I64, I64, I32]),
+    "fmd_mxfp4_linear": (I32, [P, I32, P, P, P, P, P, I64, I64, I64, I32, I32, P, P]),
+    "fmd_mxfp4_linear_bwd_workspace_bytes": (I64, [I32, I64, I64, I64, I32, I32]),
+    "fmd_mxfp4_linear_bwd": (I32, [P, I32, P, I32, P, P, P, P, I64, I64, I64, P, P]),
+    "fmd_linear_ckpt8_workspace_bytes": (I64, [I32, I64, I64, I64]),
+    "fmd_linear_ckpt8": (I32, [P, I32, P, P, P, P, P, I64, I64, I64, I32, P, P]),
+    "fmd_linear_ckpt8_bwd_workspace_bytes": (I64, [I32, I64, I64, I64, I32, I32, I32, I32]),
+    "fmd_linear_ckpt8_bwd": (I32, [P, I32, P, P, P, P, P, P, I64, I64, I64, I32, P, P]),
     "fmd_schnet_pack_bytes": (I64, [P]),
     "fmd_schnet_pack": (I32, [P, P, P, P]),
     "fmd_schnet_workspace_bytes": (I64, [P, I64, I64, I64]),

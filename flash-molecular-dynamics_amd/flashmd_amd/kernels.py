@@ -23,6 +23,8 @@ import torch
 
 from . import _ffi
 from ._ffi import call, ptr, stream
+from .mx import (fused_tanh_linear_ckpt8_autograd, linear_ckpt8_autograd, mxfp4_dequantize, mxfp4_linear,
+                 mxfp4_linear_autograd, mxfp4_quantize, mxint8_dequantize, mxint8_quantize)
 
 __all__ = [
     "radius_graph",
@@ -37,6 +39,9 @@ __all__ = [
     "build_csr_index", "build_src_csr_index", "fused_csr_cfconv", "fused_csr_cfconv_autograd",
     "fused_src_csr_grad_x", "csr_segment_reduce",
     "fused_tanh_backward_grad_x_v2", "matmul_fp32_fp16_to_fp16_v2", "gemm_f32",
+    # block-scaled layers (flashmd_amd.mx; not in the reference's surface)
+    "mxfp4_quantize", "mxfp4_dequantize", "mxint8_quantize", "mxint8_dequantize", "mxfp4_linear", "mxfp4_linear_autograd",
+    "linear_ckpt8_autograd", "fused_tanh_linear_ckpt8_autograd",
 ]
 
 

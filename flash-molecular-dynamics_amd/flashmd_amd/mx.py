@@ -1,0 +1,274 @@
+"""Linear layers on block-scaled numbers: 32 columns of a row share a power of two (formats: include/flashmd_hip.h).
+
+  mxfp4_quantize / mxfp4_dequantize          4-bit blocks (e2m1 elements)
+  mxint8_quantize / mxint8_dequantize        8-bit blocks
+  mxfp4_linear[_autograd]                    y = f(x W^T + b) with W -- and, if asked for, x -- in 4-bit blocks
+  linear_ckpt8_autograd                      y = x W + b          } for training: the backward pass has x in 8-bit blocks
+  fused_tanh_linear_ckpt8_autograd           y = tanh(x) W + b    } instead of the tensor itself
+
+Not part of the reference's surface (its narrowest format is fp16, reference models/gptq.py); conventions are those of
+``flashmd_amd.kernels``: contiguous GPU tensors, HIP kernels on torch's current stream, fresh outputs, no CPU fallback.
+Dense tensors are float32, float16 or bfloat16, one type within a call.  The gradients are not differentiable again.
+"""
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _ffi
+from ._ffi import call, ptr, stream
+
+__all__ = ["mxfp4_quantize", "mxfp4_dequantize", "mxint8_quantize", "mxint8_dequantize", "mxfp4_linear",
+           "mxfp4_linear_autograd", "linear_ckpt8_autograd", "fused_tanh_linear_ckpt8_autograd"]
+
+BLOCK = 32
+DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}   # FMD_F32, FMD_F16, FMD_BF16
+AUX_NONE, AUX_Y, AUX_DACT = 0, 1, 2
+
+
+def blocks(k: int) -> int:
+    return (k + BLOCK - 1) // BLOCK
+
+
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _dense(x: torch.Tensor, what: str = "x") -> int:
+    """Checks a dense matrix; its type's number."""
+    _ffi.require_gpu(x)
+    assert x.dim() == 2, f"{what} must be a matrix, got {x.dim()} dimensions"
+    assert x.dtype in DTYPES, f"{what} must be float32, float16 or bfloat16, got {x.dtype}"
+    assert x.is_contiguous(), f"{what} must be contiguous"
+    return DTYPES[x.dtype]
+
+
+def _blocked(codes: torch.Tensor, scales: torch.Tensor, k: int, per_block: int, dtype: torch.dtype):
+    _ffi.require_gpu(codes, scales)
+    assert codes.dtype == dtype and scales.dtype == torch.uint8, f"codes must be {dtype} and scales uint8"
+    assert codes.dim() == 2 and scales.dim() == 2 and codes.is_contiguous() and scales.is_contiguous()
+    assert k >= 1 and codes.shape == (scales.shape[0], per_block * blocks(k)) and scales.shape[1] == blocks(k), \
+        f"{k} columns take {blocks(k)} blocks a row: codes {tuple(codes.shape)}, scales {tuple(scales.shape)}"
+    assert codes.device == scales.device
+
+
+def _vector(b: Optional[torch.Tensor], n: int, like: torch.Tensor):
+    if b is not None:
+        _ffi.require_gpu(b)
+        assert b.shape == (n,) and b.dtype == like.dtype and b.is_contiguous() and b.device == like.device, \
+            f"bias must be {n} contiguous {like.dtype} on {like.device}"
+
+
+class _on:
+    """Launch on the tensor's device, whichever is current."""
+    __slots__ = ("guard",)
+
+    def __init__(self, t: torch.Tensor):
+        self.guard = None if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+
+def _workspace(nbytes: int, device) -> torch.Tensor:
+    if nbytes < 0:
+        raise RuntimeError(f"flashmd_amd: {_ffi.strerror(nbytes)} (layer sizes)")
+    return torch.empty(max(int(nbytes), 16), dtype=torch.uint8, device=device)
+
+
+def _quantize(name: str, x, per_block: int, dtype) -> tuple:
+    kind = _dense(x)
+    m, k = x.shape
+    assert k >= 1, "no columns to quantise"
+    x = _aligned(x.detach())
+    codes = torch.empty((m, per_block * blocks(k)), dtype=dtype, device=x.device)
+    scales = torch.empty((m, blocks(k)), dtype=torch.uint8, device=x.device)
+    with _on(x):
+        call(name, ptr(x), kind, m, k, ptr(codes), ptr(scales), stream())
+    return codes, scales
+
+
+def _dequantize(name: str, codes, scales, num_columns: int, dtype, per_block: int, code_dtype) -> torch.Tensor:
+    _blocked(codes, scales, num_columns, per_block, code_dtype)
+    assert dtype in DTYPES, f"dtype must be float32, float16 or bfloat16, got {dtype}"
+    codes = _aligned(codes)
+    out = torch.empty((codes.shape[0], num_columns), dtype=dtype, device=codes.device)
+    with _on(codes):
+        call(name, ptr(codes), ptr(scales), codes.shape[0], num_columns, ptr(out), DTYPES[dtype], stream())
+    return out
+
+
+def mxfp4_quantize(x: torch.Tensor) -> tuple:
+    """x [M,K] -> (codes uint8 [M, 16 ceil(K/32)], scales uint8 [M, ceil(K/32)])."""
+    return _quantize("fmd_mxfp4_quantize", x, BLOCK // 2, torch.uint8)
+
+
+def mxfp4_dequantize(codes, scales, num_columns: int, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """The values of 4-bit blocks (exact in float32 and bfloat16; float16 rounds what is beyond its range)."""
+    return _dequantize("fmd_mxfp4_dequantize", codes, scales, num_columns, dtype, BLOCK // 2, torch.uint8)
+
+
+def mxint8_quantize(x: torch.Tensor) -> tuple:
+    """x [M,K] -> (codes int8 [M, 32 ceil(K/32)], scales uint8 [M, ceil(K/32)])."""
+    return _quantize("fmd_mxint8_quantize", x, BLOCK, torch.int8)
+
+
+def mxint8_dequantize(codes, scales, num_columns: int, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """The values of 8-bit blocks (exact in float32 and bfloat16; float16 rounds what is beyond its range)."""
+    return _dequantize("fmd_mxint8_dequantize", codes, scales, num_columns, dtype, BLOCK, torch.int8)
+
+
+# ==================================================================================================
+# y = f(x W^T + b), W in 4-bit blocks
+# ==================================================================================================
+
+
+def _check_linear(x, codes, scales, bias, activation) -> int:
+    kind = _dense(x)
+    assert activation in (None, "tanh"), f"activation must be None or 'tanh', got {activation!r}"
+    _blocked(codes, scales, x.shape[1], BLOCK // 2, torch.uint8)
+    assert codes.device == x.device and codes.shape[0] >= 1
+    _vector(bias, codes.shape[0], x)
+    return kind
+
+
+def _linear(x, codes, scales, bias, kind: int, tanh: bool, quantize_input: bool, want_dact: bool) -> tuple:
+    m, k = x.shape
+    n = codes.shape[0]
+    x, codes = _aligned(x), _aligned(codes)
+    y = torch.empty((m, n), dtype=x.dtype, device=x.device)
+    dact = torch.empty((m, n), dtype=torch.float16, device=x.device) if want_dact else None
+    if m:
+        with _on(x):
+            ws = _workspace(_ffi.lib().fmd_mxfp4_linear_workspace_bytes(kind, m, n, k, int(quantize_input)), x.device)
+            call("fmd_mxfp4_linear", ptr(x), kind, ptr(codes), ptr(scales), ptr(bias), ptr(y), ptr(dact), m, n, k, int(tanh),
+                 int(quantize_input), ptr(ws), stream())
+    return y, dact
+
+
+def mxfp4_linear(x, codes, scales, bias=None, activation: Optional[str] = None, quantize_input: bool = False) -> torch.Tensor:
+    """y [M,N] = f(x W^T + b) for x [M,K] and W [N,K] (nn.Linear's layout) as ``mxfp4_quantize`` returns it; f is tanh or
+    nothing.  ``quantize_input``: x, too, is taken in its 4-bit blocks (both operands on the 4-bit matrix instruction);
+    without it x is exact and only the weights are narrow."""
+    kind = _check_linear(x, codes, scales, bias, activation)
+    return _linear(x, codes, scales, bias, kind, activation == "tanh", quantize_input, False)[0]
+
+
+class MXFP4LinearFunction(torch.autograd.Function):
+    """gx = (g f') W, gb = sum g f'.  The codes have no gradient; with ``quantize_input`` the quantisation of x passes the
+    gradient on as if it were the identity.  f' = 1 - y^2 comes from y in float32 and, in 16 bits, where 1 - y^2 of the
+    rounded y would lose its leading digits near saturation, from a float16 copy made before y is rounded."""
+
+    @staticmethod
+    def forward(ctx, x, codes, scales, bias, tanh, quantize_input):
+        need = ctx.needs_input_grad[0] or ctx.needs_input_grad[3]
+        wide = x.dtype == torch.float32
+        y, dact = _linear(x, codes, scales, bias, DTYPES[x.dtype], tanh, quantize_input, tanh and need and not wide)
+        ctx.aux_kind = AUX_NONE if not tanh else AUX_Y if wide else AUX_DACT
+        ctx.k = x.shape[1]
+        ctx.save_for_backward(codes, scales, y if ctx.aux_kind == AUX_Y else dact)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_output):
+        codes, scales, aux = ctx.saved_tensors
+        want_x, want_b = ctx.needs_input_grad[0], ctx.needs_input_grad[3]
+        g = _aligned(grad_output.contiguous())
+        m, n = g.shape
+        kind = DTYPES[g.dtype]
+        gx = torch.empty((m, ctx.k), dtype=g.dtype, device=g.device) if want_x else None
+        gb = torch.empty(n, dtype=g.dtype, device=g.device) if want_b else None
+        codes = _aligned(codes)
+        if m or want_b:
+            with _on(g):
+                ws = _workspace(_ffi.lib().fmd_mxfp4_linear_bwd_workspace_bytes(kind, m, n, ctx.k, int(want_x), int(want_b)), g.device)
+                call("fmd_mxfp4_linear_bwd", ptr(g), kind, ptr(aux), ctx.aux_kind, ptr(codes), ptr(scales), ptr(gx), ptr(gb), m, n,
+                     ctx.k, ptr(ws), stream())
+        return gx, None, None, gb, None, None
+
+
+def mxfp4_linear_autograd(x, codes, scales, bias=None, activation: Optional[str] = None,
+                          quantize_input: bool = False) -> torch.Tensor:
+    """``mxfp4_linear`` with gradients of x and bias.  Without ``quantize_input`` the gradient of x is the derivative of what
+    was computed, so forces taken through such layers are those of their energy."""
+    _check_linear(x, codes, scales, bias, activation)
+    return MXFP4LinearFunction.apply(x, codes, scales, bias, activation == "tanh", bool(quantize_input))
+
+
+# ==================================================================================================
+# y = p(x) W + b for training, x kept in 8-bit blocks
+# ==================================================================================================
+
+
+class LinearCkpt8Function(torch.autograd.Function):
+    """gx = (g W^T) p'(x8), gw = p(x8)^T g, gb = sum g, x8 the 8-bit blocks of x: 33 bytes for 32 columns are all that is kept
+    of x.  The blocks are those of the layer's INPUT, so what the backward pass sees is a function of x's bits and not of the
+    last digit of a computed tanh."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, tanh):
+        m, k = x.shape
+        n = weight.shape[1]
+        kind = DTYPES[x.dtype]
+        x, w = _aligned(x), _aligned(weight)
+        y = torch.empty((m, n), dtype=x.dtype, device=x.device)
+        keep = ctx.needs_input_grad[1] or (tanh and ctx.needs_input_grad[0])
+        codes = torch.empty((m, BLOCK * blocks(k)), dtype=torch.int8, device=x.device) if keep else None
+        scales = torch.empty((m, blocks(k)), dtype=torch.uint8, device=x.device) if keep else None
+        if m:
+            with _on(x):
+                ws = _workspace(_ffi.lib().fmd_linear_ckpt8_workspace_bytes(kind, m, n, k), x.device)
+                call("fmd_linear_ckpt8", ptr(x), kind, ptr(w), ptr(bias), ptr(y), ptr(codes), ptr(scales), m, n, k, int(tanh),
+                     ptr(ws), stream())
+        ctx.save_for_backward(codes, scales, weight)
+        ctx.tanh = tanh
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_output):
+        codes, scales, weight = ctx.saved_tensors
+        want_x, want_w, want_b = ctx.needs_input_grad[:3]
+        g = _aligned(grad_output.contiguous())
+        (m, n), k = g.shape, weight.shape[0]
+        new = torch.empty if m else torch.zeros
+        gx = new((m, k), dtype=g.dtype, device=g.device) if want_x else None
+        gw = new((k, n), dtype=g.dtype, device=g.device) if want_w else None
+        gb = new(n, dtype=g.dtype, device=g.device) if want_b else None
+        if m:
+            kind, w = DTYPES[g.dtype], _aligned(weight)
+            with _on(g):
+                ws = _workspace(_ffi.lib().fmd_linear_ckpt8_bwd_workspace_bytes(kind, m, n, k, int(ctx.tanh), int(want_x), int(want_w),
+                                                                                int(want_b)), g.device)
+                call("fmd_linear_ckpt8_bwd", ptr(g), kind, ptr(codes), ptr(scales), ptr(w), ptr(gx), ptr(gw), ptr(gb), m, n, k,
+                     int(ctx.tanh), ptr(ws), stream())
+        return gx, gw, gb, None
+
+
+def _ckpt8(x, weight, bias, tanh: bool) -> torch.Tensor:
+    _dense(x)
+    _dense(weight, "weight")
+    assert x.dtype == weight.dtype and x.device == weight.device, "x and weight must have one type and one device"
+    assert x.shape[1] == weight.shape[0], f"Dimension mismatch: x has {x.shape[1]} columns but weight has {weight.shape[0]} rows"
+    assert weight.shape[0] >= 1 and weight.shape[1] >= 1, "an empty weight"
+    _vector(bias, weight.shape[1], x)
+    return LinearCkpt8Function.apply(x, weight, bias, tanh)
+
+
+def linear_ckpt8_autograd(x, weight, bias=None) -> torch.Tensor:
+    """y = x W + b, W [K,N]; the backward pass computes the weight's gradient from x's 8-bit blocks (gx and gb are exact)."""
+    return _ckpt8(x, weight, bias, False)
+
+
+def fused_tanh_linear_ckpt8_autograd(x, weight, bias=None) -> torch.Tensor:
+    """y = tanh(x) W + b, W [K,N], as ``fused_tanh_linear_autograd``; the backward pass computes tanh and its derivative from
+    x's 8-bit blocks."""
+    return _ckpt8(x, weight, bias, True)

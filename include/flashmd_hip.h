@@ -168,6 +168,56 @@ int fmd_matmul_f32_f16_to_f16(const float* a, const void* b, void* c, int64_t m,
                               void* stream);
 
 /* ---------------------------------------------------------------------------------------------
+ * Linear layers on block-scaled numbers (no counterpart in the reference).  32 columns of a row share a power of two;
+ * nb = ceil(k / 32) blocks a row, the last one may be shorter and its codes behind column k are zero.
+ *   4 bits: codes [m][16 nb] bytes, two e2m1 {0,.5,1,1.5,2,3,4,6} to a byte (even column in the low half, bit 3 the sign),
+ *           scales [m][nb]: byte = max(floor(log2 amax) - 2, -127) + 127, value = e2m1 * 2^(byte-127);
+ *           nearest even, above 6 becomes 6
+ *   8 bits: codes [m][32 nb] int8 in [-127,127], byte = max(floor(log2 amax), -127) + 127, value = code / 64 * 2^(byte-127);
+ *           nearest even
+ *   A block that holds an Inf or a NaN has byte 255, codes 0 and stands for NaN.
+ * dtype: FMD_F32 | FMD_F16 | FMD_BF16 of every dense tensor of a call.  Device pointers of dense tensors, codes and
+ * workspaces are 16-byte aligned, else FMD_EINVAL; m = 0 is a call that does nothing.  Sums are held in fp32.  Results do
+ * not depend on timing (no atomics).  A value that is not finite makes what is computed from it not finite (Inf may
+ * become NaN).
+ *
+ *   fmd_mxfp4_quantize / _dequantize, fmd_mxint8_quantize / _dequantize: x [m,k] <-> codes, scales
+ *   fmd_mxfp4_linear      y[m,n] = f(x^ W^T + bias): W [n,k] as codes, scales; f the identity or (tanh != 0) tanh;
+ *        x^ = x, or with quantize_input x's own 4-bit blocks.  dact (fp16 [m,n], or NULL): 1 - y^2 before y is rounded, for the
+ *        backward pass of a 16-bit layer
+ *   fmd_mxfp4_linear_bwd  gx = (g f') W^, gbias = sum over rows of g f'; f' from aux: FMD_AUX_NONE (f' = 1), FMD_AUX_Y (fp32
+ *        only: aux = y, f' = 1 - y^2), FMD_AUX_DACT (16 bits only: aux = dact).  gx / gbias may be NULL.  With quantize_input
+ *        this is the gradient that passes the quantisation unchanged
+ *   fmd_linear_ckpt8      y = p(x) W + bias, W [k,n], p the identity or tanh; codes, scales (both or neither NULL): x in
+ *        8-bit blocks
+ *   fmd_linear_ckpt8_bwd  from those: gx = (g W^T) p'(x8), gw[k,n] = p(x8)^T g, gbias = sum g; each may be NULL; m >= 1
+ *   *_workspace_bytes     negative: FMD_EINVAL
+ * ------------------------------------------------------------------------------------------- */
+#define FMD_F32 0
+#define FMD_F16 1
+#define FMD_BF16 2
+#define FMD_AUX_NONE 0
+#define FMD_AUX_Y 1
+#define FMD_AUX_DACT 2
+int fmd_mxfp4_quantize(const void* x, int dtype, int64_t m, int64_t k, void* codes, void* scales, void* stream);
+int fmd_mxfp4_dequantize(const void* codes, const void* scales, int64_t m, int64_t k, void* out, int dtype, void* stream);
+int fmd_mxint8_quantize(const void* x, int dtype, int64_t m, int64_t k, void* codes, void* scales, void* stream);
+int fmd_mxint8_dequantize(const void* codes, const void* scales, int64_t m, int64_t k, void* out, int dtype, void* stream);
+int64_t fmd_mxfp4_linear_workspace_bytes(int dtype, int64_t m, int64_t n, int64_t k, int quantize_input);
+int fmd_mxfp4_linear(const void* x, int dtype, const void* codes, const void* scales, const void* bias, void* y, void* dact,
+                     int64_t m, int64_t n, int64_t k, int tanh, int quantize_input, void* workspace, void* stream);
+int64_t fmd_mxfp4_linear_bwd_workspace_bytes(int dtype, int64_t m, int64_t n, int64_t k, int want_gx, int want_gbias);
+int fmd_mxfp4_linear_bwd(const void* g, int dtype, const void* aux, int aux_kind, const void* codes, const void* scales, void* gx,
+                         void* gbias, int64_t m, int64_t n, int64_t k, void* workspace, void* stream);
+int64_t fmd_linear_ckpt8_workspace_bytes(int dtype, int64_t m, int64_t n, int64_t k);
+int fmd_linear_ckpt8(const void* x, int dtype, const void* w, const void* bias, void* y, void* codes, void* scales, int64_t m,
+                     int64_t n, int64_t k, int tanh, void* workspace, void* stream);
+int64_t fmd_linear_ckpt8_bwd_workspace_bytes(int dtype, int64_t m, int64_t n, int64_t k, int tanh, int want_gx, int want_gw,
+                                             int want_gbias);
+int fmd_linear_ckpt8_bwd(const void* g, int dtype, const void* codes, const void* scales, const void* w, void* gx, void* gw,
+                         void* gbias, int64_t m, int64_t n, int64_t k, int tanh, void* workspace, void* stream);
+
+/* ---------------------------------------------------------------------------------------------
  * Whole-path engine: energy[B] and forces[N,3] of a batch in one call, no [E,F] tensor in HBM.
  * Replaces SchNet.forward (models/schnet.py:178-369) + GradientsOut.forward
  * (models/gradients.py:226-290) for StandardSchNet models (Gaussian basis, cosine cutoff with
