@@ -99,6 +99,22 @@ __device__ __forceinline__ u32x4 mx_bf16_from4(uint32_t codes, float scale) {
   return r;
 }
 
+// tanh without a branch: 1 - 2 / (e^{2|x|} + 1) from |x| = 1/4 up (absolute error 8e-8), the odd Taylor polynomial to x^9 below
+// (the next term is 2e-9 of it there), so that small values keep their relative accuracy
+__device__ __forceinline__ float mx_tanh(float x) {
+  const float a = fabsf(x), x2 = x * x;
+  const float p = x * (1.0f + x2 * (-0.33333334f + x2 * (0.13333334f + x2 * (-0.053968254f + x2 * 0.021869488f))));
+  const float t = copysignf(1.0f - 2.0f * __builtin_amdgcn_rcpf(__expf(2.0f * a) + 1.0f), x);
+  return a < 0.25f ? p : t;  // a NaN takes the second and stays one
+}
+
+// a wave-uniform value that the compiler takes for a new one: what is computed from it stays where it is used, in scalar
+// registers, instead of becoming dozens of loop-invariant vector registers
+__device__ __forceinline__ int mx_here(int v) {
+  asm volatile("" : "+s"(v));
+  return v;
+}
+
 // ---- planes -----------------------------------------------------------------------------------------------------------
 // two fp32 values -> one dword of bf16 pairs per plane.  Cutting off the low half keeps 8 significant bits and cannot
 // overflow; the remainder is exact.  x == hi for an Inf, whose remainder is then 0 and not Inf - Inf; a NaN whose low

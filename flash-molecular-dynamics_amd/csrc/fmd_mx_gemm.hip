@@ -34,7 +34,7 @@ struct SrcDense {
     }
     if constexpr (TANH)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = fmd_tanh(v[i]);  // tanh(0) = 0: padding stays zero
+      for (int i = 0; i < 8; ++i) v[i] = mx_tanh(v[i]);  // tanh(0) = 0: padding stays zero
   }
 };
 // a gradient times the derivative of the activation behind it.  AUX 1: aux = y in fp32, factor 1 - y^2; 2: aux = the factor in fp16
@@ -76,7 +76,7 @@ struct SrcI8 {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const float x = mx_value8((int)(int8_t)(c[i >> 2] >> (8 * (i & 3))), byte);
-      v[i] = c0 + i < cols ? (TANH ? fmd_tanh(x) : x) : 0.f;
+      v[i] = c0 + i < cols ? (TANH ? mx_tanh(x) : x) : 0.f;
     }
   }
 };
@@ -190,10 +190,10 @@ struct GemmArgs {
 template <class T>
 __device__ __forceinline__ void finish_one(const MxEpilogue& e, int64_t row, int64_t col, int64_t ld, float v) {
   if (e.bias) v += MxType<T>::to(((const T*)e.bias)[col]);
-  if (e.tanh) v = fmd_tanh(v);
+  if (e.tanh) v = mx_tanh(v);
   if (e.dact) ((_Float16*)e.dact)[row * ld + col] = (_Float16)(1.f - v * v);
   if (e.codes8) {
-    const float t = fmd_tanh(mx_value8((int)(int8_t)e.codes8[row * e.nb8 * 32 + col], e.scales8[row * e.nb8 + (col >> 5)]));
+    const float t = mx_tanh(mx_value8((int)(int8_t)e.codes8[row * e.nb8 * 32 + col], e.scales8[row * e.nb8 + (col >> 5)]));
     v *= 1.f - t * t;
   }
   ((T*)e.out)[row * ld + col] = MxType<T>::from(v);
@@ -347,7 +347,7 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_kernel(const GemmArgs g) {
       const uint32_t byte = g.e.scales8[row * g.e.nb8 + (col >> 5)];
 #pragma unroll
       for (int b = 0; b < TN; ++b) {  // col is a multiple of TN: one block
-        const float x = fmd_tanh(mx_value8((int)(int8_t)g.e.codes8[row * g.e.nb8 * 32 + col + b], byte));
+        const float x = mx_tanh(mx_value8((int)(int8_t)g.e.codes8[row * g.e.nb8 * 32 + col + b], byte));
         v[b] = (*c)[b][r] * (1.f - x * x);
       }
       write((T*)g.e.out + row * ld + col, v);
@@ -361,7 +361,7 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_kernel(const GemmArgs g) {
     if (g.e.tanh) {
       store([&](int64_t row, const f32x16(*c)[TN], int r) {
 #pragma unroll
-        for (int b = 0; b < TN; ++b) v[b] = fmd_tanh((*c)[b][r] + bias[b]);
+        for (int b = 0; b < TN; ++b) v[b] = mx_tanh((*c)[b][r] + bias[b]);
         write((T*)g.e.out + row * ld + col, v);
         if (g.e.dact) {
 #pragma unroll

@@ -1,0 +1,253 @@
+// Weight and bias gradients of a narrow layer over many rows: gw[k,n] = sum over rows p(x8)[.,k] g[.,n], gb[n] = sum g[.,n],
+// k and n at most 128, x8 in 8-bit blocks.
+//
+// The contraction runs over the rows, so a matrix fragment wants 8 rows of one column in a lane.  Lane i of a half wave takes
+// columns NT*i .. NT*i+NT-1 of g (one 16-byte load a row) and KT*i .. of the checkpoint; over 8 rows that is one fragment for each
+// of its columns, with no transposition through LDS: which matrix column a lane stands for is free, and the result is stored
+// back in the same order.  A wave holds all of gw in its accumulators (up to 128 x 128: 256 of a lane's 512 registers, one wave a
+// SIMD) and takes 16 rows a step, the next step's rows already on their way.  The waves of a workgroup add up in LDS, the
+// workgroups in a second kernel, in a fixed order.  Bound by reading g and the checkpoint once.
+#include <type_traits>
+
+#include "fmd_mx_host.h"
+
+namespace {
+
+constexpr int WAVES = 4;
+constexpr uint32_t NOWHERE = 0x40000000u;
+typedef __amdgpu_buffer_rsrc_t Rows;
+
+struct GradArgs {
+  const void* g;
+  const uint8_t *codes, *scales;
+  float* part;  // [slice][32 KT + 1][32 NT]; the last row: bias
+  int64_t m;
+  int k, n, nb, vec;
+};
+
+__device__ __forceinline__ Rows rows_of(const void* p, int64_t row0, int64_t m, int row_bytes) {
+  const int64_t left = m - row0;
+  const int n = left < 16 ? (left > 0 ? (int)left : 0) : 16;
+  return __builtin_amdgcn_make_buffer_rsrc((char*)p + row0 * row_bytes, 0, n * row_bytes, 0x00020000);
+}
+
+// workgroups a CU: two where half the registers are enough
+template <class T, int KT> constexpr int PER_CU = sizeof(T) == 2 && KT == 2 ? 2 : 1;
+
+template <class T, bool TANH, int KT, int NT>
+__global__ __launch_bounds__(64 * WAVES, (PER_CU<T, KT>)) void gradient_kernel(const GradArgs a) {
+  constexpr int PA = TANH ? MxType<T>::planes : 1, PB = MxType<T>::planes, TOP = PA > PB ? PA : PB, S = sizeof(T);
+  constexpr int W = NT * S / 4;                    // dwords of a lane's columns in a row of g
+  extern __shared__ __attribute__((aligned(16))) float lds[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), j = lane & 31, h = lane >> 5;
+  const int k0 = KT * j, n0 = NT * j;
+  const int steps = (int)((a.m + 15) >> 4), stride = gridDim.x * WAVES;  // m is at most 2^34
+
+  uint32_t g_raw[8][W], s_raw[8];
+  uint32_t c_raw[8];
+  const bool kept = a.codes && k0 < a.nb * 32;  // the bias's gradient alone needs no checkpoint
+  const uint32_t c_off = kept ? (uint32_t)(8 * h * a.nb * 32 + k0) : NOWHERE;
+  const uint32_t s_off = kept ? (uint32_t)(8 * h * a.nb + (k0 >> 5)) : NOWHERE;
+  auto fetch = [&](int step) {
+    const int64_t row0 = (int64_t)step * 16;
+    const Rows g = rows_of(a.g, row0, a.m, a.n * S), c = rows_of(a.codes, row0, a.m, a.nb * 32), s = rows_of(a.scales, row0, a.m, a.nb);
+    const int gs = mx_here(a.n * S), nbs = mx_here(a.nb);
+    const uint32_t at = (uint32_t)(8 * h * a.n + n0) * S;
+    if (a.vec) {
+      const uint32_t off = n0 < a.n ? at : NOWHERE;
+#pragma unroll
+      for (int r = 0; r < 8; ++r) {
+        if constexpr (W == 4) *(u32x4*)g_raw[r] = __builtin_amdgcn_raw_buffer_load_b128(g, off, r * gs, 0);
+        else if constexpr (W == 2) *(u32x2*)g_raw[r] = __builtin_amdgcn_raw_buffer_load_b64(g, off, r * gs, 0);
+        else g_raw[r][0] = __builtin_amdgcn_raw_buffer_load_b32(g, off, r * gs, 0);
+      }
+    } else {
+#pragma unroll
+      for (int r = 0; r < 8; ++r)
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+          if constexpr (S == 4) {
+            g_raw[r][w] = __builtin_amdgcn_raw_buffer_load_b32(g, n0 + w < a.n ? at + 4 * w : NOWHERE, r * gs, 0);
+          } else {
+            const uint32_t lo = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(g, n0 + 2 * w < a.n ? at + 4 * w : NOWHERE, r * gs, 0);
+            const uint32_t hi = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(g, n0 + 2 * w + 1 < a.n ? at + 4 * w + 2 : NOWHERE, r * gs, 0);
+            g_raw[r][w] = lo | hi << 16;
+          }
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+      if constexpr (KT == 4) c_raw[r] = __builtin_amdgcn_raw_buffer_load_b32(c, c_off, r * 32 * nbs, 0);
+      else c_raw[r] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(c, c_off, r * 32 * nbs, 0);
+      s_raw[r] = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(s, s_off, r * nbs, 0);
+    }
+  };
+  auto g_value = [&](int r, int t) {
+    if constexpr (S == 4) return __builtin_bit_cast(float, g_raw[r][t]);
+    else if constexpr (std::is_same<T, mx_bf16>::value)
+      return __builtin_bit_cast(float, t & 1 ? g_raw[r][t >> 1] & 0xffff0000u : g_raw[r][t >> 1] << 16);
+    else return (float)__builtin_bit_cast(_Float16, (uint16_t)(g_raw[r][t >> 1] >> 16 * (t & 1)));
+  };
+
+  f32x16 acc[KT][NT];
+  float bias[NT] = {};
+#pragma unroll
+  for (int i = 0; i < KT; ++i)
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[i][t][r] = 0.f;
+
+  int step = wave * gridDim.x + blockIdx.x;
+  if (step < steps) fetch(step);
+  for (; step < steps; step += stride) {
+    u32x4 fa[KT][PA], fb[NT][PB];
+#pragma unroll
+    for (int i = 0; i < KT; ++i) {
+      float v[8];
+#pragma unroll
+      for (int r = 0; r < 8; ++r) {
+        const float x = mx_value8((int)(int8_t)(c_raw[r] >> 8 * i), s_raw[r]);
+        v[r] = TANH ? mx_tanh(x) : x;
+      }
+      mx_split8<PA>(v, fa[i]);
+    }
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      float v[8];
+#pragma unroll
+      for (int r = 0; r < 8; ++r) v[r] = g_value(r, t);
+      mx_split8<PB>(v, fb[t]);
+      bias[t] += ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+    }
+    if (step + stride < steps) fetch(step + stride);
+#pragma unroll
+    for (int sum = TOP - 1; sum >= 0; --sum)
+#pragma unroll
+      for (int p = 0; p < PA; ++p)
+        if (sum - p >= 0 && sum - p < PB)
+#pragma unroll
+          for (int i = 0; i < KT; ++i)
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+              acc[i][t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, fa[i][p]),
+                                                                  __builtin_bit_cast(bf16x8, fb[t][sum - p]), acc[i][t], 0, 0, 0);
+  }
+
+  // the waves add up in LDS, one after the other: [register][lane], then the bias
+  constexpr int REGS = KT * NT * 16;
+  for (int w = 0; w < WAVES; ++w) {
+    if (wave == w) {
+      float* mine = lds + lane;
+#pragma unroll
+      for (int i = 0; i < KT; ++i)
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          // keeps the 256 sums of a full tile where they are: the compiler would copy all of them out before the loop
+          // (the nops: a matrix result is read at the earliest 18 states after its instruction)
+          if constexpr (KT * NT == 16) asm volatile("s_nop 15\n\ts_nop 15" : "+a"(acc[i][t]));
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            float* to = mine + ((i * NT + t) * 16 + r) * 64;
+            *to = w ? *to + acc[i][t][r] : acc[i][t][r];
+          }
+          __builtin_amdgcn_sched_barrier(0);  // a tile at a time, or the compiler holds all of them twice
+        }
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        const float v = fmd_xor32_sum(bias[t]);
+        float* to = lds + REGS * 64 + n0 + t;
+        if (h == 0) *to = w ? *to + v : v;
+      }
+    }
+    __syncthreads();
+  }
+  float* part = a.part + (int64_t)blockIdx.x * (32 * KT + 1) * (32 * NT);
+  for (int at = threadIdx.x; at < 32 * KT * 32 * NT; at += 64 * WAVES) {
+    const int k = at / (32 * NT), n = at % (32 * NT), i = k % KT, row = k / KT, t = n % NT;
+    part[at] = lds[((i * NT + t) * 16 + (row & 3) + 4 * (row >> 3)) * 64 + 32 * (row >> 2 & 1) + n / NT];
+  }
+  if (threadIdx.x < 32 * NT) part[32 * KT * 32 * NT + threadIdx.x] = lds[REGS * 64 + threadIdx.x];
+}
+
+// gw and gb from the slices: 64 outputs a workgroup, four groups of slices each, added in a fixed order
+template <class T>
+__global__ __launch_bounds__(256) void gradient_sum_kernel(const float* __restrict__ part, int slices, int rows, int pitch, int k, int n,
+                                                           T* __restrict__ gw, T* __restrict__ gb) {
+  __shared__ float lds[4][64];
+  const int at = blockIdx.x * 64 + (threadIdx.x & 63), q = threadIdx.x >> 6;
+  const int row = at / n, col = at - row * n;  // row k: the bias
+  const bool want = row < k ? gw != nullptr : row == k && gb != nullptr;
+  float v = 0.f;
+  if (want) {
+    const float* p = part + (int64_t)(row < k ? row : rows) * pitch + col;
+    const int64_t slice = (int64_t)(rows + 1) * pitch;
+    const int s0 = slices * q / 4, s1 = slices * (q + 1) / 4;
+    for (int s = s0; s < s1; ++s) v += p[s * slice];
+  }
+  lds[q][threadIdx.x & 63] = v;
+  __syncthreads();
+  if (q == 0 && want) {
+    v = (lds[0][threadIdx.x] + lds[1][threadIdx.x]) + (lds[2][threadIdx.x] + lds[3][threadIdx.x]);
+    if (row < k) gw[(int64_t)row * n + col] = MxType<T>::from(v);
+    else gb[col] = MxType<T>::from(v);
+  }
+}
+
+template <class K>
+hipError_t allow_lds(K kernel, int bytes) {
+  static bool done[64] = {};
+  int dev = 0;
+  hipError_t e = hipGetDevice(&dev);
+  if (e != hipSuccess) return e;
+  if (dev >= 0 && dev < 64 && done[dev]) return hipSuccess;
+  e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == hipSuccess && dev >= 0 && dev < 64) done[dev] = true;
+  return e;
+}
+
+template <class T, bool TANH, int KT, int NT>
+int launch(const GradArgs& a, int slices, hipStream_t s) {
+  constexpr int bytes = (KT * NT * 16 * 64 + 32 * NT) * 4;
+  static_assert(bytes * PER_CU<T, KT> <= 160 * 1024, "LDS of a CU");
+  if (allow_lds(&gradient_kernel<T, TANH, KT, NT>, bytes) != hipSuccess) return FMD_ELAUNCH;
+  gradient_kernel<T, TANH, KT, NT><<<slices, 64 * WAVES, bytes, s>>>(a);
+  return hipGetLastError() == hipSuccess ? FMD_OK : FMD_ELAUNCH;
+}
+
+template <class T, bool TANH>
+int by_width(const GradArgs& a, int slices, hipStream_t s) {
+  if (a.k <= 64) return a.n <= 64 ? launch<T, TANH, 2, 2>(a, slices, s) : launch<T, TANH, 2, 4>(a, slices, s);
+  return a.n <= 64 ? launch<T, TANH, 4, 2>(a, slices, s) : launch<T, TANH, 4, 4>(a, slices, s);
+}
+
+template <class T>
+int run(GradArgs a, bool tanh, int slices, void* gw, void* gb, hipStream_t s) {
+  const int nt = a.n <= 64 ? 2 : 4, rows = a.k <= 64 ? 64 : 128;
+  a.vec = ((uintptr_t)a.g & 15) == 0 && a.n % nt == 0;
+  const int rc = tanh ? by_width<T, true>(a, slices, s) : by_width<T, false>(a, slices, s);
+  if (rc != FMD_OK) return rc;
+  gradient_sum_kernel<T><<<((a.k + 1) * a.n + 63) / 64, 256, 0, s>>>(a.part, slices, rows, 32 * nt, a.k, a.n, (T*)gw, (T*)gb);
+  return hipGetLastError() == hipSuccess ? FMD_OK : FMD_ELAUNCH;
+}
+
+// workgroups along the rows: one step of 16 rows for each wave at least, what fits the chip at once at most
+int slices_for(int dtype, int64_t m, int64_t k) {
+  const int64_t s = (m + 16 * WAVES - 1) / (16 * WAVES), most = k <= 64 && dtype != FMD_F32 ? 512 : 256;
+  return (int)(s < most ? s : most);
+}
+
+}  // namespace
+
+int64_t mx_gradient_bytes(int dtype, int64_t m, int64_t n, int64_t k) {
+  return (int64_t)slices_for(dtype, m, k) * ((k <= 64 ? 64 : 128) + 1) * (n <= 64 ? 64 : 128) * 4;
+}
+
+int mx_gradient(const void* g, const uint8_t* codes, const uint8_t* scales, bool tanh, int dtype, int64_t m, int64_t n, int64_t k,
+                void* gw, void* gb, void* workspace, hipStream_t s) {
+  const GradArgs a{g, codes, scales, (float*)workspace, m, (int)k, (int)n, (int)mx_blocks(k), 0};
+  const int slices = slices_for(dtype, m, k);
+  if (dtype == FMD_F32) return run<float>(a, tanh, slices, gw, gb, s);
+  if (dtype == FMD_F16) return run<_Float16>(a, tanh, slices, gw, gb, s);
+  return run<mx_bf16>(a, tanh, slices, gw, gb, s);
+}

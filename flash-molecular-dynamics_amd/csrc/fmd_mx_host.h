@@ -40,6 +40,34 @@ void mx_product(const MxOperand& a, const MxOperand& b, int64_t m, int64_t n, in
 void mx_sum_parts(const float* parts, int64_t count, int64_t m, int64_t n, int dtype, const MxEpilogue& e, hipStream_t s);
 void mx_column_sums(const MxSource& q, int64_t rows, int64_t cols, int64_t parts, float* out, hipStream_t s);
 
+// a layer of at most 128 x 128 in one pass over the rows (fmd_mx_layer.hip)
+enum { MX_WEIGHT_DENSE, MX_WEIGHT_FP4, MX_WEIGHT_FP4_BOTH, MX_WEIGHT_FP4_ACROSS };
+struct MxLayer {
+  const void *in, *aux;
+  int pro;                     // MX_SRC_DENSE, _TANH, _GRAD_Y, _GRAD_D
+  const void *w, *wscales;
+  int weight;
+  int64_t sk, sn;              // dense weight: strides of the contraction and of the outputs
+  uint8_t *codes8, *scales8;   // written (null: not kept), or read for dtanh
+  bool dtanh;
+  MxEpilogue e;                // bias, out, dact, tanh
+  float* sums;                 // MX_WEIGHT_FP4_ACROSS: workspace of mx_layer_sums_bytes for the input's column totals, or null
+  void* totals;
+};
+int64_t mx_layer_sums_bytes(int64_t m, int64_t c);
+bool mx_layer_fits(int64_t c, int64_t o);
+int mx_layer(const MxLayer& l, int dtype, int64_t m, int64_t c, int64_t o, hipStream_t s);
+
+// gw [k,n] and gb [n] (either may be null) of a layer of at most 128 x 128, one pass over the rows (fmd_mx_gradient.hip)
+int64_t mx_gradient_bytes(int dtype, int64_t m, int64_t n, int64_t k);
+int mx_gradient(const void* g, const uint8_t* codes, const uint8_t* scales, bool tanh, int dtype, int64_t m, int64_t n, int64_t k,
+                void* gw, void* gb, void* workspace, hipStream_t s);
+
+// at most 64 rows through a layer with 4-bit weights of any width (fmd_mx_rows.hip)
+bool mx_rows_fits(int64_t m);
+int mx_rows(const void* x, int dtype, const void* codes, const void* scales, bool both, int64_t m, int64_t n, int64_t k,
+            const MxEpilogue& e, hipStream_t s);
+
 static inline int mx_dtype_size(int dtype) { return dtype == FMD_F32 ? 4 : 2; }
 static inline int mx_dtype_planes(int dtype) { return dtype == FMD_F32 ? 3 : dtype == FMD_F16 ? 2 : 1; }
 

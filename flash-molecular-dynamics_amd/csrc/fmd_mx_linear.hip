@@ -93,6 +93,16 @@ struct Fp4Linear {
 
 int64_t fp4_forward(const Fp4Linear& c, void* base, bool run, hipStream_t s) {
   MxArena ar{(char*)base, 0};
+  if (mx_layer_fits(c.k, c.n)) {
+    if (run)
+      mx_layer({c.x, nullptr, MX_SRC_DENSE, c.codes, c.scales, c.both ? MX_WEIGHT_FP4_BOTH : MX_WEIGHT_FP4, 0, 0, nullptr, nullptr, false, c.e, nullptr, nullptr},
+               c.dtype, c.m, c.k, c.n, s);
+    return 0;
+  }
+  if (mx_rows_fits(c.m)) {
+    if (run) mx_rows(c.x, c.dtype, c.codes, c.scales, c.both, c.m, c.n, c.k, c.e, s);
+    return 0;
+  }
   const int64_t nb = mx_blocks(c.k);
   if (c.both) {
     const int64_t kt = (nb + 7) / 8;
@@ -127,12 +137,18 @@ struct Fp4Backward {
 int64_t fp4_backward(const Fp4Backward& c, void* base, bool run, bool want_gx, bool want_gb, hipStream_t s) {
   MxArena ar{(char*)base, 0};
   const MxSource g{c.kind, c.dtype, c.g, c.aux};
-  if (want_gx) {
+  const MxEpilogue to_gx{nullptr, c.gx, nullptr, nullptr, nullptr, 0, 0};
+  if (want_gx && mx_layer_fits(c.n, c.k)) {
+    float* sums = want_gb ? (float*)ar.take(mx_layer_sums_bytes(c.m, c.n)) : nullptr;
+    if (run)
+      mx_layer({c.g, c.aux, c.kind, c.codes, c.scales, MX_WEIGHT_FP4_ACROSS, 0, 0, nullptr, nullptr, false, to_gx, sums, c.gb}, c.dtype, c.m,
+               c.n, c.k, s);
+    return ar.used;
+  } else if (want_gx) {
     const int64_t pad = mx_up(c.n, 64);
     void* w = ar.take(c.k * pad * 2);
     if (run) mx_planes({MX_SRC_FP4, FMD_BF16, c.codes, c.scales}, c.n, c.k, true, w, s);
-    product_of_rows(ar, run, g, c.m, c.n, {w, c.k * pad * 2, pad * 2, 1, nullptr}, c.k, c.dtype,
-                    MxEpilogue{nullptr, c.gx, nullptr, nullptr, nullptr, 0, 0}, s);
+    product_of_rows(ar, run, g, c.m, c.n, {w, c.k * pad * 2, pad * 2, 1, nullptr}, c.k, c.dtype, to_gx, s);
   }
   if (want_gb) sum_over_rows(ar, run, g, c.m, c.n, c.dtype, c.gb, s);
   return ar.used;
@@ -151,6 +167,12 @@ struct Kept {
 
 int64_t kept_forward(const Kept& c, void* base, bool run, hipStream_t s) {
   MxArena ar{(char*)base, 0};
+  if (mx_layer_fits(c.k, c.n)) {
+    if (run)
+      mx_layer({c.x, nullptr, c.tanh ? MX_SRC_TANH : MX_SRC_DENSE, c.w, nullptr, MX_WEIGHT_DENSE, c.n, 1, c.codes, c.scales, false, c.e, nullptr, nullptr},
+               c.dtype, c.m, c.k, c.n, s);
+    return 0;
+  }
   const int p = mx_dtype_planes(c.dtype);
   const int64_t pad = mx_up(c.k, 64);
   void* w = ar.take(p * c.n * pad * 2);
@@ -167,13 +189,23 @@ int64_t kept_backward(const Kept& c, void* base, bool run, bool want_gx, bool wa
   MxArena ar{(char*)base, 0};
   const int p = mx_dtype_planes(c.dtype);
   const MxSource g{MX_SRC_DENSE, c.dtype, c.g, nullptr};
-  if (want_gx) {
+  const bool narrow = mx_layer_fits(c.n, c.k);
+  if (want_gx && narrow) {
+    if (run)
+      mx_layer({c.g, nullptr, MX_SRC_DENSE, c.w, nullptr, MX_WEIGHT_DENSE, 1, c.n, c.tanh ? c.codes : nullptr, c.tanh ? c.scales : nullptr, c.tanh,
+                {nullptr, c.gx, nullptr, nullptr, nullptr, 0, 0}, nullptr, nullptr}, c.dtype, c.m, c.n, c.k, s);
+  } else if (want_gx) {
     const int64_t pad = mx_up(c.n, 64);
     void* w = ar.take(p * c.k * pad * 2);
     if (run) mx_planes({MX_SRC_DENSE, c.dtype, c.w, nullptr}, c.k, c.n, false, w, s);
     MxEpilogue e{nullptr, c.gx, nullptr, nullptr, nullptr, 0, 0};
     if (c.tanh) e.codes8 = c.codes, e.scales8 = c.scales, e.nb8 = mx_blocks(c.k);
     product_of_rows(ar, run, g, c.m, c.n, {w, c.k * pad * 2, pad * 2, p, nullptr}, c.k, c.dtype, e, s);
+  }
+  if ((want_gw || want_gb) && narrow) {  // the bias's sums come along
+    void* part = ar.take(mx_gradient_bytes(c.dtype, c.m, c.n, c.k));
+    if (run) mx_gradient(c.g, c.codes, c.scales, c.tanh, c.dtype, c.m, c.n, c.k, c.gw, c.gb, part, s);
+    return ar.used;
   }
   if (want_gw)
     product_over_rows(ar, run, {c.tanh ? MX_SRC_I8_TANH : MX_SRC_I8, c.dtype, c.codes, c.scales}, c.tanh ? p : 1, c.k, g, c.n, c.m,
@@ -184,7 +216,7 @@ int64_t kept_backward(const Kept& c, void* base, bool run, bool want_gx, bool wa
 
 bool bad_sizes(int dtype, int64_t m, int64_t n, int64_t k) {
   // rows of a product are counted in 32 bits within a chunk, and a weight in all
-  return dtype < 0 || dtype > 2 || m < 0 || n < 1 || k < 1 || m > (int64_t)1 << 40 || n > 1 << 24 || k > 1 << 24;
+  return dtype < 0 || dtype > 2 || m < 0 || n < 1 || k < 1 || m > (int64_t)1 << 34 || n > 1 << 24 || k > 1 << 24;
 }
 bool off16(const void* p) { return ((uintptr_t)p & 15) != 0; }
 
@@ -201,9 +233,9 @@ extern "C" int fmd_mxfp4_linear(const void* x, int dtype, const void* codes, con
                                 int64_t m, int64_t n, int64_t k, int tanh, int quantize_input, void* workspace, void* stream) {
   if (bad_sizes(dtype, m, n, k) || (quantize_input && m > INT32_MAX)) return FMD_EINVAL;
   if (m == 0) return FMD_OK;
-  if (!x || !codes || !scales || !y || !workspace || off16(x) || off16(codes) || off16(y) || off16(workspace) || (dact && !tanh))
-    return FMD_EINVAL;
+  if (!x || !codes || !scales || !y || off16(x) || off16(codes) || off16(y) || off16(workspace) || (dact && !tanh)) return FMD_EINVAL;
   const Fp4Linear c{x, codes, scales, dtype, m, n, k, quantize_input != 0, {bias, y, dact, nullptr, nullptr, 0, tanh}};
+  if (!workspace && fp4_forward(c, nullptr, false, nullptr)) return FMD_EINVAL;
   fp4_forward(c, workspace, true, fmd_stream(stream));
   FMD_CHECK_LAUNCH();
   return FMD_OK;
@@ -222,9 +254,10 @@ extern "C" int fmd_mxfp4_linear_bwd(const void* g, int dtype, const void* aux, i
   if (m && (!g || off16(g) || (aux_kind && (!aux || off16(aux))) || (gx && (!codes || !scales || off16(gx) || off16(codes)))))
     return FMD_EINVAL;
   if (!gx && !gbias) return FMD_OK;
-  if ((m || gbias) && (!workspace || off16(workspace))) return FMD_EINVAL;
+  if (off16(workspace)) return FMD_EINVAL;
   const int kind = aux_kind == FMD_AUX_Y ? MX_SRC_GRAD_Y : aux_kind == FMD_AUX_DACT ? MX_SRC_GRAD_D : MX_SRC_DENSE;
   const Fp4Backward c{g, aux, codes, scales, gx, gbias, dtype, kind, m, n, k};
+  if (!workspace && fp4_backward(c, nullptr, false, gx && m, gbias, nullptr)) return FMD_EINVAL;
   fp4_backward(c, workspace, true, gx && m, gbias, fmd_stream(stream));
   FMD_CHECK_LAUNCH();
   return FMD_OK;
@@ -242,10 +275,11 @@ extern "C" int fmd_linear_ckpt8(const void* x, int dtype, const void* w, const v
                                 int64_t n, int64_t k, int tanh, void* workspace, void* stream) {
   if (bad_sizes(dtype, m, n, k) || (codes != nullptr) != (scales != nullptr)) return FMD_EINVAL;
   if (m == 0) return FMD_OK;
-  if (!x || !w || !y || !workspace || off16(x) || off16(w) || off16(y) || off16(codes) || off16(workspace)) return FMD_EINVAL;
+  if (!x || !w || !y || off16(x) || off16(w) || off16(y) || off16(codes) || off16(workspace)) return FMD_EINVAL;
   Kept c{};
   c.x = x, c.w = w, c.codes = (uint8_t*)codes, c.scales = (uint8_t*)scales, c.dtype = dtype, c.m = m, c.n = n, c.k = k, c.tanh = tanh != 0;
   c.e = {bias, y, nullptr, nullptr, nullptr, 0, 0};
+  if (!workspace && kept_forward(c, nullptr, false, nullptr)) return FMD_EINVAL;
   kept_forward(c, workspace, true, fmd_stream(stream));
   FMD_CHECK_LAUNCH();
   return FMD_OK;
@@ -265,11 +299,12 @@ extern "C" int fmd_linear_ckpt8_bwd(const void* g, int dtype, const void* codes,
   if (bad_sizes(dtype, m, n, k) || m == 0) return FMD_EINVAL;
   if (!gx && !gw && !gbias) return FMD_OK;
   const bool kept = gw || (gx && tanh);
-  if (!g || !workspace || off16(g) || off16(workspace) || (gx && (!w || off16(w) || off16(gx))) || (kept && (!codes || !scales || off16(codes))))
+  if (!g || off16(g) || off16(workspace) || (gx && (!w || off16(w) || off16(gx))) || (kept && (!codes || !scales || off16(codes))))
     return FMD_EINVAL;
   Kept c{};
   c.g = g, c.w = w, c.codes = (uint8_t*)codes, c.scales = (uint8_t*)scales, c.gx = gx, c.gw = gw, c.gb = gbias;
   c.dtype = dtype, c.m = m, c.n = n, c.k = k, c.tanh = tanh != 0;
+  if (!workspace && kept_backward(c, nullptr, false, gx, gw, gbias, nullptr)) return FMD_EINVAL;
   kept_backward(c, workspace, true, gx, gw, gbias, fmd_stream(stream));
   FMD_CHECK_LAUNCH();
   return FMD_OK;

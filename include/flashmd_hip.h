@@ -191,7 +191,7 @@ int fmd_matmul_f32_f16_to_f16(const float* a, const void* b, void* c, int64_t m,
  *   fmd_linear_ckpt8      y = p(x) W + bias, W [k,n], p the identity or tanh; codes, scales (both or neither NULL): x in
  *        8-bit blocks
  *   fmd_linear_ckpt8_bwd  from those: gx = (g W^T) p'(x8), gw[k,n] = p(x8)^T g, gbias = sum g; each may be NULL; m >= 1
- *   *_workspace_bytes     negative: FMD_EINVAL
+ *   *_workspace_bytes     0: none is needed and NULL will do; negative: FMD_EINVAL
  * ------------------------------------------------------------------------------------------- */
 #define FMD_F32 0
 #define FMD_F16 1
