@@ -71,11 +71,15 @@ __device__ __forceinline__ float mx_scale_value(uint32_t byte) {
   return __builtin_bit_cast(float, byte == 0 ? 0x00400000u : byte == 255u ? 0x7fc00000u : byte << 23);
 }
 
-// 8-bit code of x in a block of the given scale byte
-__device__ __forceinline__ int mx_code8(float x, uint32_t byte) {
-  const float q = __builtin_rintf(__builtin_ldexpf(x, 133 - (int)byte));  // 64 x / 2^E; v_ldexp_f32 rounds once
-  const int i = (int)fminf(fmaxf(q, -127.f), 127.f);
-  return byte == 255u ? 0 : i;
+// four 8-bit codes of a block, the first in the low byte.  64 x / 2^E is exact; adding 1.5 * 2^23 rounds it to nearest even and
+// leaves the integer in the low bits
+__device__ __forceinline__ uint32_t mx_codes8(float x0, float x1, float x2, float x3, uint32_t byte) {
+  const int e = 133 - (int)byte;
+  auto bits = [e](float x) {
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_fmed3f(__builtin_ldexpf(x, e), -127.f, 127.f) + 12582912.f);
+  };
+  const uint32_t lo = __builtin_amdgcn_perm(bits(x1), bits(x0), 0x0c0c0400u), hi = __builtin_amdgcn_perm(bits(x3), bits(x2), 0x0c0c0400u);
+  return byte == 255u ? 0u : lo | hi << 16;
 }
 __device__ __forceinline__ float mx_value8(int code, uint32_t byte) {
   return byte == 255u ? __builtin_nanf("") : __builtin_ldexpf((float)code, (int)byte - 133);

@@ -171,9 +171,10 @@ __global__ __launch_bounds__(256) void scale_tiles_kernel(const uint8_t* __restr
 // C[m,n] = epi(A B^T + bias): BM x BN tiles, TM x TN matrix tiles of 32 x 32 per wave, K tiles of 128 bytes a row
 // (64 bf16 or 256 4-bit elements), two LDS buffers filled by direct loads one tile ahead.
 //
-// LDS: slot (row, p) of 16 bytes holds granule p ^ ((row / T) & 7) of the row's tile, T the matrix tiles per wave in that
-// direction: the 32 lanes of a fragment read rows T*lane + t, so eight neighbouring lanes meet eight different positions.
-// That row order also gives a lane T neighbouring columns of C.
+// LDS: lines of two rows, 16 slots of 16 bytes (all 64 banks).  Granule q of row r is in slot ((r & 1) * 8 + q) ^ ((r / T) & 15) of
+// line r / 2, T (even) the matrix tiles per wave in that direction: the 32 lanes of a fragment read rows T*lane + t, so 16
+// neighbouring lanes meet 16 different slots.  That row order also gives a lane T neighbouring columns of C.  (With the two rows
+// of a line swizzled apart, half the banks served a read: 4 conflict cycles on 4.)
 // =====================================================================================================================
 __device__ u32x4 mx_zero_granule;
 
@@ -201,6 +202,7 @@ __device__ __forceinline__ void finish_one(const MxEpilogue& e, int64_t row, int
 
 template <class T, bool FP4, int WM, int WN, int TM, int TN>
 __global__ __launch_bounds__(64 * WM * WN) void gemm_kernel(const GemmArgs g) {
+  static_assert(TM % 2 == 0 && TN % 2 == 0, "two rows of a line belong to one lane");
   constexpr int BM = 32 * WM * TM, BN = 32 * WN * TN, NW = WM * WN, SLOTS = (BM + BN) * 8, LOADS = SLOTS / (64 * NW);
   __shared__ __attribute__((aligned(16))) char lds[2 * (BM + BN) * 128];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, j = lane & 31, h = lane >> 5;
@@ -219,10 +221,10 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_kernel(const GemmArgs g) {
   int gran[LOADS];
 #pragma unroll
   for (int i = 0; i < LOADS; ++i) {
-    const int slot = (i * NW + wave) * 64 + lane, r = slot >> 3, p = slot & 7;
     const bool is_a = (i * NW + wave) * 64 < BM * 8;  // uniform: BM * 8 is a multiple of 64
-    const int rr = is_a ? r : r - BM;
-    gran[i] = p ^ ((is_a ? rr / TM : rr / TN) & 7);
+    const int slot = (i * NW + wave) * 64 + lane - (is_a ? 0 : BM * 8), line = slot >> 4;
+    const int id = (slot & 15) ^ ((is_a ? 2 * line / TM : 2 * line / TN) & 15), rr = 2 * line + (id >> 3);
+    gran[i] = id & 7;
     const int row = is_a ? min(m0 + rr, g.m - 1) : min(n0 + rr, g.n - 1);
     off[i] = (int64_t)row * (is_a ? g.a_pitch : g.b_pitch) + gran[i] * 16;
   }
@@ -270,10 +272,10 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_kernel(const GemmArgs g) {
     const char* lb = buf + BM * 128 + (wn * 32 + j) * TN * 128;
 #define MX_STEP(s)                                                                                                          \
   {                                                                                                                         \
-    const int at = (((s) * 2 + h) ^ (j & 7)) * 16;                                                                          \
+    const int q = (s) * 2 + h, at = (q ^ (j & 15)) * 16, odd = ((8 + q) ^ (j & 15)) * 16;                                   \
     u32x4 fa[TM], fb[TN];                                                                                                   \
-    _Pragma("unroll") for (int a = 0; a < TM; ++a) fa[a] = *(const u32x4*)(la + a * 128 + at);                              \
-    _Pragma("unroll") for (int b = 0; b < TN; ++b) fb[b] = *(const u32x4*)(lb + b * 128 + at);                              \
+    _Pragma("unroll") for (int a = 0; a < TM; ++a) fa[a] = *(const u32x4*)(la + (a >> 1) * 256 + (a & 1 ? odd : at));        \
+    _Pragma("unroll") for (int b = 0; b < TN; ++b) fb[b] = *(const u32x4*)(lb + (b >> 1) * 256 + (b & 1 ? odd : at));        \
     _Pragma("unroll") for (int a = 0; a < TM; ++a) _Pragma("unroll") for (int b = 0; b < TN; ++b) {                         \
       if constexpr (FP4) {                                                                                                  \
         const i32x8 xa = {(int)fa[a][0], (int)fa[a][1], (int)fa[a][2], (int)fa[a][3], 0, 0, 0, 0};                          \
@@ -310,16 +312,22 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_kernel(const GemmArgs g) {
 
   // a lane's TN columns are neighbours: stored together where every row starts on a multiple of them
   const int64_t ld = g.n, col = n0 + (wn * 32 + j) * TN;
-  const bool whole = TN == 2 && (g.n & 1) == 0 && col < g.n;
+  const bool whole = g.n % TN == 0 && col < g.n;
   auto store = [&](auto finish) {
 #pragma unroll
-    for (int a = 0; a < TM; ++a)
+    for (int a = 0; a < TM; ++a) {
+      // 256 sums stay where they are until a row of tiles is stored: the compiler would copy all of them first (the nops: a
+      // matrix result is read at the earliest 18 states after its instruction)
+      if constexpr (TM * TN == 16)
+#pragma unroll
+        for (int b = 0; b < TN; ++b) asm volatile("s_nop 15\n\ts_nop 15" : "+a"(acc[a][b]));
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const int64_t row = m0 + (wm * 32 + (r & 3) + 8 * (r >> 2) + 4 * h) * TM + a;
         if (row >= g.m) continue;
         finish(row, &acc[a], r);
       }
+    }
   };
   auto write = [&](auto* p, const float (&v)[TN]) {  // p: (row, col) of the output
     using U = typename std::remove_reference<decltype(*p)>::type;

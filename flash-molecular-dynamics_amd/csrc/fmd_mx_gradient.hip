@@ -1,12 +1,15 @@
-// Weight and bias gradients of a narrow layer over many rows: gw[k,n] = sum over rows p(x8)[.,k] g[.,n], gb[n] = sum g[.,n],
-// k and n at most 128, x8 in 8-bit blocks.
+// Weight and bias gradients: gw[k,n] = sum over rows p(x8)[.,k] g[.,n], gb[n] = sum g[.,n], x8 in 8-bit blocks.
 //
-// The contraction runs over the rows, so a matrix fragment wants 8 rows of one column in a lane.  Lane i of a half wave takes
+// gradient_kernel, for narrow layers (k and n at most 128) over many rows.  The contraction runs over the rows, so a matrix fragment wants 8 rows of one column in a lane.  Lane i of a half wave takes
 // columns NT*i .. NT*i+NT-1 of g (one 16-byte load a row) and KT*i .. of the checkpoint; over 8 rows that is one fragment for each
 // of its columns, with no transposition through LDS: which matrix column a lane stands for is free, and the result is stored
 // back in the same order.  A wave holds all of gw in its accumulators (up to 128 x 128: 256 of a lane's 512 registers, one wave a
 // SIMD) and takes 16 rows a step, the next step's rows already on their way.  The waves of a workgroup add up in LDS, the
 // workgroups in a second kernel, in a fixed order.  Bound by reading g and the checkpoint once.
+//
+// gradient_tile_kernel, for few rows and any width.  A workgroup makes one 32 x 32 tile of gw from a slice of the rows; its eight
+// waves take 16 rows each in turn.  g and the checkpoint are read once for every tile beside or below, from the caches, but a
+// few rows spread over many workgroups, and a workgroup has 16 sums a lane to bring together instead of 256.
 #include <type_traits>
 
 #include "fmd_mx_host.h"
@@ -14,7 +17,7 @@
 namespace {
 
 constexpr int WAVES = 4;
-constexpr uint32_t NOWHERE = 0x40000000u;
+constexpr uint32_t NOWHERE = 0x40000000u;  // behind the end of every descriptor: 16 rows of at most 2^24 fp32
 typedef __amdgpu_buffer_rsrc_t Rows;
 
 struct GradArgs {
@@ -57,9 +60,9 @@ __global__ __launch_bounds__(64 * WAVES, (PER_CU<T, KT>)) void gradient_kernel(c
       const uint32_t off = n0 < a.n ? at : NOWHERE;
 #pragma unroll
       for (int r = 0; r < 8; ++r) {
-        if constexpr (W == 4) *(u32x4*)g_raw[r] = __builtin_amdgcn_raw_buffer_load_b128(g, off, r * gs, 0);
-        else if constexpr (W == 2) *(u32x2*)g_raw[r] = __builtin_amdgcn_raw_buffer_load_b64(g, off, r * gs, 0);
-        else g_raw[r][0] = __builtin_amdgcn_raw_buffer_load_b32(g, off, r * gs, 0);
+        if constexpr (W == 4) *(u32x4*)g_raw[r] = __builtin_amdgcn_raw_buffer_load_b128(g, off + r * gs, 0, 0);
+        else if constexpr (W == 2) *(u32x2*)g_raw[r] = __builtin_amdgcn_raw_buffer_load_b64(g, off + r * gs, 0, 0);
+        else g_raw[r][0] = __builtin_amdgcn_raw_buffer_load_b32(g, off + r * gs, 0, 0);
       }
     } else {
 #pragma unroll
@@ -67,19 +70,19 @@ __global__ __launch_bounds__(64 * WAVES, (PER_CU<T, KT>)) void gradient_kernel(c
 #pragma unroll
         for (int w = 0; w < W; ++w) {
           if constexpr (S == 4) {
-            g_raw[r][w] = __builtin_amdgcn_raw_buffer_load_b32(g, n0 + w < a.n ? at + 4 * w : NOWHERE, r * gs, 0);
+            g_raw[r][w] = __builtin_amdgcn_raw_buffer_load_b32(g, n0 + w < a.n ? at + 4 * w + r * gs : NOWHERE, 0, 0);
           } else {
-            const uint32_t lo = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(g, n0 + 2 * w < a.n ? at + 4 * w : NOWHERE, r * gs, 0);
-            const uint32_t hi = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(g, n0 + 2 * w + 1 < a.n ? at + 4 * w + 2 : NOWHERE, r * gs, 0);
+            const uint32_t lo = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(g, n0 + 2 * w < a.n ? at + 4 * w + r * gs : NOWHERE, 0, 0);
+            const uint32_t hi = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(g, n0 + 2 * w + 1 < a.n ? at + 4 * w + 2 + r * gs : NOWHERE, 0, 0);
             g_raw[r][w] = lo | hi << 16;
           }
         }
     }
 #pragma unroll
     for (int r = 0; r < 8; ++r) {
-      if constexpr (KT == 4) c_raw[r] = __builtin_amdgcn_raw_buffer_load_b32(c, c_off, r * 32 * nbs, 0);
-      else c_raw[r] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(c, c_off, r * 32 * nbs, 0);
-      s_raw[r] = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(s, s_off, r * nbs, 0);
+      if constexpr (KT == 4) c_raw[r] = __builtin_amdgcn_raw_buffer_load_b32(c, c_off + r * 32 * nbs, 0, 0);
+      else c_raw[r] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(c, c_off + r * 32 * nbs, 0, 0);
+      s_raw[r] = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(s, s_off + r * nbs, 0, 0);
     }
   };
   auto g_value = [&](int r, int t) {
@@ -170,25 +173,109 @@ __global__ __launch_bounds__(64 * WAVES, (PER_CU<T, KT>)) void gradient_kernel(c
   if (threadIdx.x < 32 * NT) part[32 * KT * 32 * NT + threadIdx.x] = lds[REGS * 64 + threadIdx.x];
 }
 
-// gw and gb from the slices: 64 outputs a workgroup, four groups of slices each, added in a fixed order
+constexpr int TILE_WAVES = 8;
+
+template <class T, bool TANH>
+__global__ __launch_bounds__(64 * TILE_WAVES) void gradient_tile_kernel(const GradArgs a, T* __restrict__ gw, T* __restrict__ gb) {
+  constexpr int PA = TANH ? MxType<T>::planes : 1, PB = MxType<T>::planes, TOP = PA > PB ? PA : PB, S = sizeof(T);
+  __shared__ float lds[TILE_WAVES][17][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), j = lane & 31, h = lane >> 5;
+  const int block = blockIdx.x, k = block * 32 + j, n = blockIdx.y * 32 + j;  // 32 columns of the checkpoint: one block
+  const int steps = (int)((a.m + 15) >> 4), stride = gridDim.z * TILE_WAVES;
+
+  uint32_t g_raw[8], c_raw[8], s_raw[8];
+  const uint32_t g_off = n < a.n ? (uint32_t)(8 * h * a.n + n) * S : NOWHERE;
+  const uint32_t c_off = a.codes ? (uint32_t)(8 * h * a.nb * 32 + k) : NOWHERE, s_off = a.codes ? (uint32_t)(8 * h * a.nb + block) : NOWHERE;
+  auto fetch = [&](int step) {
+    const int64_t row0 = (int64_t)step * 16;
+    const Rows g = rows_of(a.g, row0, a.m, a.n * S), c = rows_of(a.codes, row0, a.m, a.nb * 32), s = rows_of(a.scales, row0, a.m, a.nb);
+    const int gs = mx_here(a.n * S), nbs = mx_here(a.nb);
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+      if constexpr (S == 4) g_raw[r] = __builtin_amdgcn_raw_buffer_load_b32(g, g_off + r * gs, 0, 0);
+      else g_raw[r] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(g, g_off + r * gs, 0, 0);
+      c_raw[r] = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(c, c_off + r * 32 * nbs, 0, 0);
+      s_raw[r] = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(s, s_off + r * nbs, 0, 0);
+    }
+  };
+  f32x16 acc;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) acc[r] = 0.f;
+  float bias = 0.f;
+  int step = blockIdx.z * TILE_WAVES + wave;
+  if (step < steps) fetch(step);
+  for (; step < steps; step += stride) {
+    u32x4 fa[PA], fb[PB];
+    float v[8];
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+      const float x = mx_value8((int)(int8_t)c_raw[r], s_raw[r]);
+      v[r] = TANH ? mx_tanh(x) : x;
+    }
+    mx_split8<PA>(v, fa);
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+      if constexpr (S == 4) v[r] = __builtin_bit_cast(float, g_raw[r]);
+      else v[r] = MxType<T>::to(__builtin_bit_cast(T, (uint16_t)g_raw[r]));
+    }
+    mx_split8<PB>(v, fb);
+    bias += ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+    if (step + stride < steps) fetch(step + stride);
+#pragma unroll
+    for (int sum = TOP - 1; sum >= 0; --sum)
+#pragma unroll
+      for (int p = 0; p < PA; ++p)
+        if (sum - p >= 0 && sum - p < PB)
+          acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, fa[p]), __builtin_bit_cast(bf16x8, fb[sum - p]), acc, 0,
+                                                        0, 0);
+  }
+#pragma unroll
+  for (int r = 0; r < 16; ++r) lds[wave][r][lane] = acc[r];
+  lds[wave][16][lane] = bias;
+  __syncthreads();
+  // (register, lane) of the tile: row of gw 8 (r >> 2) + 4 h + (r & 3), column j; r = 16: the bias, halves to be added
+  float* part = a.part ? a.part + (int64_t)blockIdx.z * (a.k + 1) * a.n : nullptr;
+  for (int o = threadIdx.x; o < 17 * 64; o += 64 * TILE_WAVES) {
+    const int r = o >> 6, l = o & 63, col = blockIdx.y * 32 + (l & 31);
+    float v = 0.f;
+#pragma unroll
+    for (int w = 0; w < TILE_WAVES; ++w) v += lds[w][r][l];
+    if (r == 16) {
+      v = fmd_xor32_sum(v);  // one wave holds this row
+      if (block || l >= 32 || col >= a.n) continue;
+      if (part) part[a.k * a.n + col] = v;
+      else if (gb) gb[col] = MxType<T>::from(v);
+    } else {
+      const int row = block * 32 + (r & 3) + 8 * (r >> 2) + 4 * (l >> 5);
+      if (row >= a.k || col >= a.n) continue;
+      if (part) part[row * a.n + col] = v;
+      else if (gw) gw[(int64_t)row * a.n + col] = MxType<T>::from(v);
+    }
+  }
+}
+
+// gw and gb from the slices: 16 outputs a workgroup, 16 groups of slices each, added in a fixed order
 template <class T>
 __global__ __launch_bounds__(256) void gradient_sum_kernel(const float* __restrict__ part, int slices, int rows, int pitch, int k, int n,
                                                            T* __restrict__ gw, T* __restrict__ gb) {
-  __shared__ float lds[4][64];
-  const int at = blockIdx.x * 64 + (threadIdx.x & 63), q = threadIdx.x >> 6;
+  __shared__ float lds[16][17];
+  const int at = blockIdx.x * 16 + (threadIdx.x & 15), q = threadIdx.x >> 4;
   const int row = at / n, col = at - row * n;  // row k: the bias
   const bool want = row < k ? gw != nullptr : row == k && gb != nullptr;
   float v = 0.f;
   if (want) {
     const float* p = part + (int64_t)(row < k ? row : rows) * pitch + col;
     const int64_t slice = (int64_t)(rows + 1) * pitch;
-    const int s0 = slices * q / 4, s1 = slices * (q + 1) / 4;
-    for (int s = s0; s < s1; ++s) v += p[s * slice];
+    const int s1 = slices * (q + 1) / 16;
+#pragma unroll 8
+    for (int s = slices * q / 16; s < s1; ++s) v += p[s * slice];
   }
-  lds[q][threadIdx.x & 63] = v;
+  lds[q][threadIdx.x & 15] = v;
   __syncthreads();
   if (q == 0 && want) {
-    v = (lds[0][threadIdx.x] + lds[1][threadIdx.x]) + (lds[2][threadIdx.x] + lds[3][threadIdx.x]);
+    v = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v += lds[i][threadIdx.x];
     if (row < k) gw[(int64_t)row * n + col] = MxType<T>::from(v);
     else gb[col] = MxType<T>::from(v);
   }
@@ -227,7 +314,7 @@ int run(GradArgs a, bool tanh, int slices, void* gw, void* gb, hipStream_t s) {
   a.vec = ((uintptr_t)a.g & 15) == 0 && a.n % nt == 0;
   const int rc = tanh ? by_width<T, true>(a, slices, s) : by_width<T, false>(a, slices, s);
   if (rc != FMD_OK) return rc;
-  gradient_sum_kernel<T><<<((a.k + 1) * a.n + 63) / 64, 256, 0, s>>>(a.part, slices, rows, 32 * nt, a.k, a.n, (T*)gw, (T*)gb);
+  gradient_sum_kernel<T><<<((a.k + 1) * a.n + 15) / 16, 256, 0, s>>>(a.part, slices, rows, 32 * nt, a.k, a.n, (T*)gw, (T*)gb);
   return hipGetLastError() == hipSuccess ? FMD_OK : FMD_ELAUNCH;
 }
 
@@ -237,15 +324,42 @@ int slices_for(int dtype, int64_t m, int64_t k) {
   return (int)(s < most ? s : most);
 }
 
+// Which kernel: a tile at a time while the rows are few.  (Both measured at 128 x 128, fp32, tanh: see FEW.)
+constexpr int64_t FEW = 65536, FEW_WIDE = 256;
+bool by_tiles(int64_t m, int64_t n, int64_t k) { return m <= (k <= 128 && n <= 128 ? FEW : FEW_WIDE); }
+int tile_slices(int64_t m, int64_t n, int64_t k) {
+  const int64_t tiles = ((k + 31) / 32) * ((n + 31) / 32), s = (m + 32 * TILE_WAVES - 1) / (32 * TILE_WAVES), most = (512 + tiles - 1) / tiles;
+  return (int)(m <= 1024 ? 1 : s < most ? s : most);  // two steps for each wave at least
+}
+
+template <class T>
+int run_tiles(GradArgs a, bool tanh, void* gw, void* gb, hipStream_t s) {
+  const int slices = tile_slices(a.m, a.n, a.k);
+  if (slices == 1) a.part = nullptr;
+  const dim3 grid((a.k + 31) / 32, (a.n + 31) / 32, slices);
+  if (tanh) gradient_tile_kernel<T, true><<<grid, 64 * TILE_WAVES, 0, s>>>(a, (T*)gw, (T*)gb);
+  else gradient_tile_kernel<T, false><<<grid, 64 * TILE_WAVES, 0, s>>>(a, (T*)gw, (T*)gb);
+  if (slices > 1) gradient_sum_kernel<T><<<((a.k + 1) * a.n + 15) / 16, 256, 0, s>>>(a.part, slices, a.k, a.n, a.k, a.n, (T*)gw, (T*)gb);
+  return hipGetLastError() == hipSuccess ? FMD_OK : FMD_ELAUNCH;
+}
+
 }  // namespace
 
+bool mx_gradient_fits(int64_t m, int64_t n, int64_t k) { return (k <= 128 && n <= 128) || by_tiles(m, n, k); }
+
 int64_t mx_gradient_bytes(int dtype, int64_t m, int64_t n, int64_t k) {
+  if (by_tiles(m, n, k)) return tile_slices(m, n, k) > 1 ? (int64_t)tile_slices(m, n, k) * (k + 1) * n * 4 : 0;
   return (int64_t)slices_for(dtype, m, k) * ((k <= 64 ? 64 : 128) + 1) * (n <= 64 ? 64 : 128) * 4;
 }
 
 int mx_gradient(const void* g, const uint8_t* codes, const uint8_t* scales, bool tanh, int dtype, int64_t m, int64_t n, int64_t k,
                 void* gw, void* gb, void* workspace, hipStream_t s) {
   const GradArgs a{g, codes, scales, (float*)workspace, m, (int)k, (int)n, (int)mx_blocks(k), 0};
+  if (by_tiles(m, n, k)) {
+    if (dtype == FMD_F32) return run_tiles<float>(a, tanh, gw, gb, s);
+    if (dtype == FMD_F16) return run_tiles<_Float16>(a, tanh, gw, gb, s);
+    return run_tiles<mx_bf16>(a, tanh, gw, gb, s);
+  }
   const int slices = slices_for(dtype, m, k);
   if (dtype == FMD_F32) return run<float>(a, tanh, slices, gw, gb, s);
   if (dtype == FMD_F16) return run<_Float16>(a, tanh, slices, gw, gb, s);

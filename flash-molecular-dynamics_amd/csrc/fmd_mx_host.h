@@ -58,7 +58,8 @@ int64_t mx_layer_sums_bytes(int64_t m, int64_t c);
 bool mx_layer_fits(int64_t c, int64_t o);
 int mx_layer(const MxLayer& l, int dtype, int64_t m, int64_t c, int64_t o, hipStream_t s);
 
-// gw [k,n] and gb [n] (either may be null) of a layer of at most 128 x 128, one pass over the rows (fmd_mx_gradient.hip)
+// gw [k,n] and gb [n] (either may be null) of a narrow layer, or of few rows (fmd_mx_gradient.hip)
+bool mx_gradient_fits(int64_t m, int64_t n, int64_t k);
 int64_t mx_gradient_bytes(int dtype, int64_t m, int64_t n, int64_t k);
 int mx_gradient(const void* g, const uint8_t* codes, const uint8_t* scales, bool tanh, int dtype, int64_t m, int64_t n, int64_t k,
                 void* gw, void* gb, void* workspace, hipStream_t s);

@@ -30,7 +30,7 @@ struct LayerArgs {
   void* totals;
   float* sums;                // column sums of the (multiplied) input, [workgroup][c], or null
   int64_t m, sk, sn;          // sk, sn: strides of a dense weight
-  int c, o, vec, tanh, nb8;
+  int c, o, vec, wvec, tanh, nb8;
 };
 
 template <class T, int WK> struct LayerPlanes {
@@ -60,13 +60,13 @@ struct Raw {
       const uint32_t off = col < c ? (uint32_t)(lane / PER_ROW * c + col) * S : NOWHERE;
 #pragma unroll
       for (int i = 0; i < PIECES; ++i)
-        v[i] = __builtin_amdgcn_raw_buffer_load_b128(rows, off, i * (64 / PER_ROW) * cs, 0);
+        v[i] = __builtin_amdgcn_raw_buffer_load_b128(rows, off + i * (64 / PER_ROW) * cs, 0, 0);
     } else {
       const uint32_t off = col0 + lane < c ? (uint32_t)(col0 + lane) * S : NOWHERE;
 #pragma unroll
       for (int i = 0; i < 32; ++i) {
-        if constexpr (S == 4) v[i >> 2][i & 3] = __builtin_amdgcn_raw_buffer_load_b32(rows, off, i * cs, 0);
-        else v[i >> 2][i & 3] = __builtin_amdgcn_raw_buffer_load_b16(rows, off, i * cs, 0);
+        if constexpr (S == 4) v[i >> 2][i & 3] = __builtin_amdgcn_raw_buffer_load_b32(rows, off + i * cs, 0, 0);
+        else v[i >> 2][i & 3] = __builtin_amdgcn_raw_buffer_load_b16(rows, off + i * cs, 0, 0);
       }
     }
   }
@@ -159,14 +159,14 @@ __device__ __forceinline__ void put_product(char* lds, const Raw<T>& g, const Ra
 }
 
 template <class T, int WK, int NT>
-__device__ __forceinline__ void fill_weight(const LayerArgs& a, char* lds) {
+__device__ __forceinline__ void fill_weight(const LayerArgs& a, int o0, char* lds) {
   const int chunks = (a.c + 63) >> 6;
   constexpr int P = LayerPlanes<T, WK>::w;
   if constexpr (WK == W_FP4_BOTH) {  // [chunk][tile][64 lanes] codes, then scales
     const int nb = (a.c + 31) >> 5;
     for (int u = threadIdx.x; u < chunks * NT * 64; u += 64 * WAVES) {
       const int lane = u & 63, t = (u >> 6) % NT, ch = (u >> 6) / NT;
-      const int n = NT * (lane & 31) + t, b = ch * 2 + (lane >> 5);
+      const int n = o0 + NT * (lane & 31) + t, b = ch * 2 + (lane >> 5);
       u32x4 code = {0, 0, 0, 0};
       uint32_t s = 0;
       if (n < a.o && b < nb) {
@@ -176,11 +176,43 @@ __device__ __forceinline__ void fill_weight(const LayerArgs& a, char* lds) {
       *(u32x4*)(lds + u * 16) = code;
       *(uint32_t*)(lds + chunks * NT * 1024 + u * 4) = s;
     }
-  } else {  // [chunk][step][plane][tile][64 lanes] of 8 bf16
+  } else if constexpr (WK == W_DENSE) {  // [chunk][step][plane][tile][64 lanes] of 8 bf16
+    // the loads of four units first: one latency for all of them
+    constexpr int MORE = 4;
+    const T* w = (const T*)a.w;
+    const int units = chunks * 4 * NT * 64;
+    for (int u0 = threadIdx.x; u0 < units; u0 += 64 * WAVES * MORE) {
+      T raw[MORE][8];
+#pragma unroll
+      for (int i = 0; i < MORE; ++i) {
+        const int u = u0 + i * 64 * WAVES, lane = u & 63, t = (u >> 6) % NT, cs = (u >> 6) / NT;
+        const int n = o0 + NT * (lane & 31) + t, k0 = (cs >> 2) * 64 + (lane >> 5) * 32 + (cs & 3) * 8;
+        if (a.wvec && n < a.o && k0 + 8 <= a.c) {  // the contraction is contiguous
+#pragma unroll
+          for (int e = 0; e < (int)sizeof(T) / 2; ++e) ((u32x4*)raw[i])[e] = ((const u32x4*)(w + (int64_t)n * a.sn + k0))[e];
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) raw[i][e] = u < units && n < a.o && k0 + e < a.c ? w[(int64_t)(k0 + e) * a.sk + n * a.sn] : T{};
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < MORE; ++i) {
+        const int u = u0 + i * 64 * WAVES, lane = u & 63, t = (u >> 6) % NT, cs = (u >> 6) / NT;
+        if (u >= units) continue;
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = MxType<T>::to(raw[i][e]);
+        u32x4 f[P];
+        mx_split8<P>(v, f);
+#pragma unroll
+        for (int p = 0; p < P; ++p) *(u32x4*)(lds + (((cs * P + p) * NT + t) * 64 + lane) * 16) = f[p];
+      }
+    }
+  } else {
     for (int u = threadIdx.x; u < chunks * 4 * NT * 64; u += 64 * WAVES) {
       const int lane = u & 63, t = (u >> 6) % NT, cs = (u >> 6) / NT;
-      const int n = NT * (lane & 31) + t, k0 = (cs >> 2) * 64 + (lane >> 5) * 32 + (cs & 3) * 8;
-      u32x4 f[P];
+      const int n = o0 + NT * (lane & 31) + t, k0 = (cs >> 2) * 64 + (lane >> 5) * 32 + (cs & 3) * 8;
+      u32x4 f[1];
       if constexpr (WK == W_FP4) {
         const int nb = (a.c + 31) >> 5, b = k0 >> 5;
         f[0] = u32x4{0, 0, 0, 0};
@@ -190,29 +222,25 @@ __device__ __forceinline__ void fill_weight(const LayerArgs& a, char* lds) {
           if (valid < 8) code = valid > 0 ? code & ((1u << 4 * valid) - 1) : 0u;
           f[0] = mx_bf16_from4(code, mx_scale_value(a.wscales[(int64_t)n * nb + b]));
         }
-      } else if constexpr (WK == W_FP4_ACROSS) {  // weight row k, column n
+      } else {  // weight row k, column n
         const int nb = (a.o + 31) >> 5;
+        uint32_t byte[8], scale[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const bool there = n < a.o && k0 + i < a.c;
+          const int64_t r = there ? (int64_t)(k0 + i) * nb + (n >> 5) : 0;
+          byte[i] = there ? ((const uint8_t*)a.w)[r * 16 + ((n & 31) >> 1)] : 0u;
+          scale[i] = there ? a.wscales[r] : 0u;
+        }
         float v[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          v[i] = 0.f;
-          if (n < a.o && k0 + i < a.c) {
-            const int64_t r = (int64_t)(k0 + i) * nb + (n >> 5);
-            const uint32_t byte = ((const uint8_t*)a.w)[r * 16 + ((n & 31) >> 1)];
-            const u32x4 q = mx_bf16_from4(n & 1 ? byte >> 4 : byte & 15u, mx_scale_value(a.wscales[r]));
-            v[i] = __builtin_bit_cast(float, q[0] << 16);
-          }
+          const u32x4 q = mx_bf16_from4(n & 1 ? byte[i] >> 4 : byte[i] & 15u, mx_scale_value(scale[i]));
+          v[i] = __builtin_bit_cast(float, q[0] << 16);
         }
         mx_split8<1>(v, f);
-      } else {
-        float v[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          v[i] = n < a.o && k0 + i < a.c ? MxType<T>::to(((const T*)a.w)[(k0 + i) * a.sk + n * a.sn]) : 0.f;
-        mx_split8<P>(v, f);
       }
-#pragma unroll
-      for (int p = 0; p < P; ++p) *(u32x4*)(lds + (((cs * P + p) * NT + t) * 64 + lane) * 16) = f[p];
+      *(u32x4*)(lds + ((cs * NT + t) * 64 + lane) * 16) = f[0];
     }
   }
 }
@@ -234,7 +262,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void layer_kernel(const LayerArgs a)
   const bool vec = a.vec;
   char* const own = lds + wave * pass_bytes<T, PRO>();
   char* const wl = lds + WAVES * pass_bytes<T, PRO>();
-  fill_weight<T, WK, NT>(a, wl);
+  const int o0 = blockIdx.y * 32 * NT;  // few rows: the outputs are shared out, too
+  fill_weight<T, WK, NT>(a, o0, wl);
 
   const int tiles = (int)((a.m + 31) >> 5), stride = gridDim.x * WAVES;
   Raw<T> raw;
@@ -249,7 +278,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void layer_kernel(const LayerArgs a)
   if (EPI == EPI_ACT && a.bias)
 #pragma unroll
     for (int t = 0; t < NT; ++t)
-      if (NT * j + t < a.o) bias[t] = MxType<T>::to(((const T*)a.bias)[NT * j + t]);
+      if (o0 + NT * j + t < a.o) bias[t] = MxType<T>::to(((const T*)a.bias)[o0 + NT * j + t]);
   __syncthreads();
 
   f32x16 acc[NT];
@@ -277,7 +306,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void layer_kernel(const LayerArgs a)
       }
       const int next_tile = ch + 1 < chunks ? tile : tile + stride, next_ch = ch + 1 < chunks ? ch + 1 : 0;
       if (next_tile < tiles) fetch(next_tile, next_ch);
-      if (EPI == EPI_ACT && WK == W_DENSE && a.codes8) {
+      if (EPI == EPI_ACT && WK == W_DENSE && a.codes8 && blockIdx.y == 0) {
         const int64_t row = row0 + j;
         const int b = ch * 2 + h;
         uint32_t top = 0;
@@ -288,10 +317,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void layer_kernel(const LayerArgs a)
           u32x4 q[2];
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            uint32_t u = 0;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) u |= (uint32_t)(mx_code8(x[4 * i + e], byte) & 255) << (8 * e);
-            q[i >> 2][i & 3] = u;
+            q[i >> 2][i & 3] = mx_codes8(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3], byte);
           }
           u32x4* to = (u32x4*)(a.codes8 + (row * a.nb8 + b) * 32);
           to[0] = q[0];
@@ -350,28 +376,28 @@ __global__ __launch_bounds__(64 * WAVES, 2) void layer_kernel(const LayerArgs a)
     if (++ch < chunks) continue;
     ch = 0;
     tile += stride;
-    const int col = NT * j, os = mx_here(a.o), nbs = mx_here(a.nb8);
+    const int col = o0 + NT * j, os = mx_here(a.o), nbs = mx_here(a.nb8);
     const bool whole = a.o % NT == 0;
     // v of one row into out (U = T) or dact (U = fp16); a lane's columns in one store where every row starts on a multiple of NT
     auto write = [&](auto zero, Rows rows, int r, const float (&v)[NT]) {
       using U = decltype(zero);
       constexpr int SU = sizeof(U);
-      const uint32_t voff = col < a.o ? (uint32_t)(4 * h * a.o + col) * SU : NOWHERE;
-      const int soff = ((r & 3) + 8 * (r >> 2)) * os * SU;
+      const uint32_t voff = (col < a.o ? (uint32_t)(4 * h * a.o + col) * SU : NOWHERE) + ((r & 3) + 8 * (r >> 2)) * os * SU;
       if (whole) {
         U e[NT];
 #pragma unroll
         for (int t = 0; t < NT; ++t) e[t] = MxType<U>::from(v[t]);
-        if constexpr (SU * NT == 16) __builtin_amdgcn_raw_buffer_store_b128(*(u32x4*)e, rows, voff, soff, 0);
-        else if constexpr (SU * NT == 8) __builtin_amdgcn_raw_buffer_store_b64(*(u32x2*)e, rows, voff, soff, 0);
-        else __builtin_amdgcn_raw_buffer_store_b32(*(uint32_t*)e, rows, voff, soff, 0);
+        if constexpr (SU * NT == 16) __builtin_amdgcn_raw_buffer_store_b128(*(u32x4*)e, rows, voff, 0, 0);
+        else if constexpr (SU * NT == 8) __builtin_amdgcn_raw_buffer_store_b64(*(u32x2*)e, rows, voff, 0, 0);
+        else if constexpr (SU * NT == 4) __builtin_amdgcn_raw_buffer_store_b32(*(uint32_t*)e, rows, voff, 0, 0);
+        else __builtin_amdgcn_raw_buffer_store_b16(*(uint16_t*)e, rows, voff, 0, 0);
       } else {
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
           const uint32_t off = col + t < a.o ? voff + t * SU : NOWHERE;
           const U e = MxType<U>::from(v[t]);
-          if constexpr (SU == 4) __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, e), rows, off, soff, 0);
-          else __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, e), rows, off, soff, 0);
+          if constexpr (SU == 4) __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, e), rows, off, 0, 0);
+          else __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, e), rows, off, 0, 0);
         }
       }
     };
@@ -384,9 +410,10 @@ __global__ __launch_bounds__(64 * WAVES, 2) void layer_kernel(const LayerArgs a)
       for (int r = 0; r < 16; ++r) {
         const int row = (r & 3) + 8 * (r >> 2);
         uint32_t q;
-        if constexpr (NT == 4) q = __builtin_amdgcn_raw_buffer_load_b32(codes, at, row * 32 * nbs, 0);
-        else q = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(codes, at, row * 32 * nbs, 0);
-        const uint32_t byte = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(scales, sat, row * nbs, 0);
+        if constexpr (NT == 4) q = __builtin_amdgcn_raw_buffer_load_b32(codes, at + row * 32 * nbs, 0, 0);
+        else if constexpr (NT == 1) q = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(codes, at + row * 32 * nbs, 0, 0);
+        else q = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(codes, at + row * 32 * nbs, 0, 0);
+        const uint32_t byte = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(scales, sat + row * nbs, 0, 0);
         float v[NT];
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
@@ -415,7 +442,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void layer_kernel(const LayerArgs a)
     }
   }
   if constexpr (WK == W_FP4_ACROSS) {
-    if (a.sums) {  // the waves' sums, in order
+    if (a.sums && blockIdx.y == 0) {  // the waves' sums, in order
       __syncthreads();
       float* all = (float*)lds;
       all[wave * 128 + lane] = sums[0];
@@ -431,19 +458,23 @@ __global__ __launch_bounds__(64 * WAVES, 2) void layer_kernel(const LayerArgs a)
   }
 }
 
-// column totals from the workgroups' sums: 16 columns, 16 groups of workgroups, in a fixed order
+// column totals from the workgroups' sums: four columns, 64 groups of workgroups, in a fixed order
 template <class T>
 __global__ __launch_bounds__(256) void column_totals_kernel(const float* __restrict__ sums, int count, int c, T* __restrict__ out) {
-  __shared__ float lds[16][16];
-  const int col = blockIdx.x * 16 + (threadIdx.x & 15), q = threadIdx.x >> 4;
+  __shared__ float lds[64][4];
+  const int col = blockIdx.x * 4 + (threadIdx.x & 3), q = threadIdx.x >> 2;
   float v = 0.f;
-  if (col < c)
-    for (int s = count * q / 16; s < count * (q + 1) / 16; ++s) v += sums[(int64_t)s * c + col];
-  lds[q][threadIdx.x & 15] = v;
+  if (col < c) {
+    const int s1 = count * (q + 1) / 64;
+#pragma unroll 8
+    for (int s = count * q / 64; s < s1; ++s) v += sums[s * c + col];  // at most 512 x 128
+  }
+  lds[q][threadIdx.x & 3] = v;
   __syncthreads();
   if (q == 0 && col < c) {
     v = 0.f;
-    for (int i = 0; i < 16; ++i) v += lds[i][threadIdx.x];
+#pragma unroll
+    for (int i = 0; i < 64; ++i) v += lds[i][threadIdx.x];
     out[col] = MxType<T>::from(v);
   }
 }
@@ -471,13 +502,16 @@ int launch(const LayerArgs& a, hipStream_t s) {
   if (allow_lds(&layer_kernel<T, PRO, WK, EPI, NT>, most) != hipSuccess) return FMD_ELAUNCH;
   const int64_t tiles = (a.m + 31) / 32, full = 256 * (bytes <= 80 * 1024 ? 2 : 1);
   const int grid = (int)(tiles < full ? tiles : full);
-  layer_kernel<T, PRO, WK, EPI, NT><<<grid, 64 * WAVES, bytes, s>>>(a);
-  if (WK == W_FP4_ACROSS && a.sums) column_totals_kernel<T><<<(a.c + 15) / 16, 256, 0, s>>>(a.sums, grid, a.c, (T*)a.totals);
+  layer_kernel<T, PRO, WK, EPI, NT><<<dim3(grid, (a.o + 32 * NT - 1) / (32 * NT)), 64 * WAVES, bytes, s>>>(a);
+  if (WK == W_FP4_ACROSS && a.sums) column_totals_kernel<T><<<(a.c + 3) / 4, 256, 0, s>>>(a.sums, grid, a.c, (T*)a.totals);
   return hipGetLastError() == hipSuccess ? FMD_OK : FMD_ELAUNCH;
 }
 
 template <class T, int PRO, int WK, int EPI>
 int by_width(const LayerArgs& a, hipStream_t s) {
+  // A tile of rows is 10 us from one end to the other: up to 64 of them, every 32 outputs get workgroups of their own (269 rows,
+  // 128 x 128, fp32: 11.1 us against 18.2); from there on the rows fill the chip (34432 rows: 43 against 25)
+  if ((a.m + 31) / 32 <= 64) return launch<T, PRO, WK, EPI, 1>(a, s);
   return a.o <= 64 ? launch<T, PRO, WK, EPI, 2>(a, s) : launch<T, PRO, WK, EPI, 4>(a, s);
 }
 
@@ -485,6 +519,7 @@ template <class T>
 int by_kind(LayerArgs a, const MxLayer& l, hipStream_t s) {
   a.vec = ((uintptr_t)a.in & 15) == 0 && a.c * sizeof(T) % 16 == 0 &&
           (!a.aux || (((uintptr_t)a.aux & 15) == 0 && a.c * (l.pro == MX_SRC_GRAD_Y ? 4 : 2) % 16 == 0));
+  a.wvec = a.sk == 1 && ((uintptr_t)a.w & 15) == 0 && a.sn * sizeof(T) % 16 == 0;
   if (l.weight == MX_WEIGHT_FP4) return by_width<T, PRO_ID, W_FP4, EPI_ACT>(a, s);
   if (l.weight == MX_WEIGHT_FP4_BOTH) return by_width<T, PRO_ID, W_FP4_BOTH, EPI_ACT>(a, s);
   if (l.weight == MX_WEIGHT_FP4_ACROSS) {

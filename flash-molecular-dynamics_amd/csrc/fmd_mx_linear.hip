@@ -202,8 +202,9 @@ int64_t kept_backward(const Kept& c, void* base, bool run, bool want_gx, bool wa
     if (c.tanh) e.codes8 = c.codes, e.scales8 = c.scales, e.nb8 = mx_blocks(c.k);
     product_of_rows(ar, run, g, c.m, c.n, {w, c.k * pad * 2, pad * 2, p, nullptr}, c.k, c.dtype, e, s);
   }
-  if ((want_gw || want_gb) && narrow) {  // the bias's sums come along
-    void* part = ar.take(mx_gradient_bytes(c.dtype, c.m, c.n, c.k));
+  if ((want_gw || want_gb) && mx_gradient_fits(c.m, c.n, c.k)) {  // the bias's sums come along
+    const int64_t bytes = mx_gradient_bytes(c.dtype, c.m, c.n, c.k);
+    void* part = bytes ? ar.take(bytes) : nullptr;
     if (run) mx_gradient(c.g, c.codes, c.scales, c.tanh, c.dtype, c.m, c.n, c.k, c.gw, c.gb, part, s);
     return ar.used;
   }

@@ -10,7 +10,7 @@
 
 namespace {
 
-constexpr int WAVES = 8, DEPTH = 4;
+constexpr int WAVES = 8;
 
 struct RowsArgs {
   const void* x;
@@ -19,27 +19,39 @@ struct RowsArgs {
   int m, n, k, nb, vec;
 };
 
+// 32 columns of a row of x as they lie in memory
 template <class T>
-__device__ __forceinline__ void load_block(const RowsArgs& a, int row, int b, float (&v)[32]) {
-  constexpr int PER = 16 / sizeof(T);
-  const T* p = (const T*)a.x + (int64_t)row * a.k + b * 32;
-  if (row < a.m && a.vec && b * 32 + 32 <= a.k) {
+struct Block {
+  static constexpr int PER = 16 / sizeof(T), N = 32 / PER;
+  u32x4 v[N];
+  __device__ __forceinline__ void load(const RowsArgs& a, int row, int b) {
 #pragma unroll
-    for (int i = 0; i < 32 / PER; ++i) {
-      T t[PER];
-      *(u32x4*)t = *(const u32x4*)(p + i * PER);
+    for (int i = 0; i < N; ++i) v[i] = u32x4{0, 0, 0, 0};
+    if (row >= a.m || b >= a.nb) return;
+    const T* p = (const T*)a.x + (int64_t)row * a.k + b * 32;
+    if (a.vec && b * 32 + 32 <= a.k) {
 #pragma unroll
-      for (int e = 0; e < PER; ++e) v[i * PER + e] = MxType<T>::to(t[e]);
+      for (int i = 0; i < N; ++i) v[i] = *(const u32x4*)(p + i * PER);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        const bool there = b * 32 + i < a.k;  // the load itself is unconditional, of a value that exists
+        const T* at = there ? p + i : p;
+        if constexpr (sizeof(T) == 4) v[i / PER][i % PER] = there ? *(const uint32_t*)at : 0u;
+        else v[i / PER][i % PER / 2] |= (there ? (uint32_t) * (const uint16_t*)at : 0u) << 16 * (i & 1);
+      }
     }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = row < a.m && b * 32 + i < a.k ? MxType<T>::to(p[i]) : 0.f;
   }
-}
+  __device__ __forceinline__ float get(int i) const {
+    const uint32_t u = v[i / PER][sizeof(T) == 4 ? i % PER : i % PER / 2];
+    if constexpr (sizeof(T) == 4) return __builtin_bit_cast(float, u);
+    else return MxType<T>::to(__builtin_bit_cast(T, (uint16_t)(u >> 16 * (i & 1))));
+  }
+};
 
 template <class T, bool BOTH, int MT>
 __global__ __launch_bounds__(64 * WAVES) void rows_kernel(const RowsArgs a) {
-  constexpr int P = MxType<T>::planes;
+  constexpr int P = MxType<T>::planes, DEPTH = MT == 1 ? 4 : MT == 2 ? 2 : 1;
   __shared__ f32x4 lds[WAVES][MT][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, q = lane >> 4;
   const int n0 = blockIdx.x * 16, row = n0 + i;
@@ -51,9 +63,12 @@ __global__ __launch_bounds__(64 * WAVES) void rows_kernel(const RowsArgs a) {
   for (int r0 = wave; r0 < runs; r0 += WAVES * DEPTH) {
     u32x4 w[DEPTH];
     uint32_t s[DEPTH];
+    constexpr bool AHEAD = MT == 1;  // x, too, before anything is waited for; more rows are read where they are used
+    Block<T> x[AHEAD ? DEPTH : 1];
 #pragma unroll
     for (int d = 0; d < DEPTH; ++d) {
       const int b = (r0 + d * WAVES) * 4 + q;
+      if constexpr (AHEAD) x[d].load(a, i, b);
       w[d] = u32x4{0, 0, 0, 0};
       s[d] = 0;
       if (row < a.n && b < a.nb) {
@@ -65,15 +80,22 @@ __global__ __launch_bounds__(64 * WAVES) void rows_kernel(const RowsArgs a) {
     for (int d = 0; d < DEPTH; ++d) {
       const int b = (r0 + d * WAVES) * 4 + q;
       if (r0 + d * WAVES >= runs) break;  // the whole wave
+      bf16x8 fw[4];
+      if constexpr (!BOTH) {
+        const float sv = mx_scale_value(s[d]);
+        const int behind = a.k - b * 32;  // the codes behind the last column count as zeros whatever they are
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const int valid = min(max(behind - 8 * g, 0), 8);
+          fw[g] = __builtin_bit_cast(bf16x8, mx_bf16_from4(valid ? w[d][g] & (0xffffffffu >> (32 - 4 * valid)) : 0u, sv));
+        }
+      }
 #pragma unroll
       for (int t = 0; t < MT; ++t) {
         float v[32];
-        if (b < a.nb) {
-          load_block<T>(a, t * 16 + i, b, v);
-        } else {
+        if constexpr (!AHEAD) x[0].load(a, t * 16 + i, b);
 #pragma unroll
-          for (int e = 0; e < 32; ++e) v[e] = 0.f;
-        }
+        for (int e = 0; e < 32; ++e) v[e] = x[AHEAD ? d : 0].get(e);
         if constexpr (BOTH) {
           uint32_t top = 0;
 #pragma unroll
@@ -91,13 +113,8 @@ __global__ __launch_bounds__(64 * WAVES) void rows_kernel(const RowsArgs a) {
           const i32x8 fw = {(int)w[d][0], (int)w[d][1], (int)w[d][2], (int)w[d][3], 0, 0, 0, 0};
           acc[t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fw, fx, acc[t], 4, 4, 0, (int)s[d], 0, (int)byte);
         } else {
-          const float sv = mx_scale_value(s[d]);
-          const int behind = a.k - b * 32;  // the codes behind the last column count as zeros whatever they are
 #pragma unroll
           for (int g = 0; g < 4; ++g) {
-            const int valid = behind - 8 * g;
-            const uint32_t code = valid >= 8 ? w[d][g] : valid > 0 ? w[d][g] & ((1u << 4 * valid) - 1) : 0u;
-            const bf16x8 fw = __builtin_bit_cast(bf16x8, mx_bf16_from4(code, sv));
             float o[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) o[e] = v[8 * g + e];
@@ -105,7 +122,7 @@ __global__ __launch_bounds__(64 * WAVES) void rows_kernel(const RowsArgs a) {
             mx_split8<P>(o, fx);
 #pragma unroll
             for (int p = P - 1; p >= 0; --p)
-              acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fw, __builtin_bit_cast(bf16x8, fx[p]), acc[t], 0, 0, 0);
+              acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fw[g], __builtin_bit_cast(bf16x8, fx[p]), acc[t], 0, 0, 0);
           }
         }
       }

@@ -12,13 +12,13 @@ Dense tensors are float32, float16 or bfloat16, one type within a call.  The gra
 """
 from __future__ import annotations
 
+import functools
 from typing import Optional
 
 import torch
 from torch.autograd.function import once_differentiable
 
 from . import _ffi
-from ._ffi import call, ptr, stream
 
 __all__ = ["mxfp4_quantize", "mxfp4_dequantize", "mxint8_quantize", "mxint8_dequantize", "mxfp4_linear",
            "mxfp4_linear_autograd", "linear_ckpt8_autograd", "fused_tanh_linear_ckpt8_autograd"]
@@ -61,26 +61,41 @@ def _vector(b: Optional[torch.Tensor], n: int, like: torch.Tensor):
             f"bias must be {n} contiguous {like.dtype} on {like.device}"
 
 
-class _on:
-    """Launch on the tensor's device, whichever is current."""
-    __slots__ = ("guard",)
-
-    def __init__(self, t: torch.Tensor):
-        self.guard = None if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+# A call's host side costs as much as a small layer's kernels, so it is kept short: the library's functions are looked up once,
+# workspace sizes once a layer shape, pointers go through ctypes as plain integers.
 
 
-def _workspace(nbytes: int, device) -> torch.Tensor:
+@functools.lru_cache(maxsize=None)
+def _function(name: str):
+    return getattr(_ffi.lib(), name)
+
+
+@functools.lru_cache(maxsize=4096)
+def _bytes(name: str, *sizes) -> int:
+    nbytes = _function(name)(*sizes)
     if nbytes < 0:
-        raise RuntimeError(f"flashmd_amd: {_ffi.strerror(nbytes)} (layer sizes)")
-    return torch.empty(max(int(nbytes), 16), dtype=torch.uint8, device=device)
+        raise RuntimeError(f"flashmd_amd.{name}: {_ffi.strerror(nbytes)} (sizes {sizes})")
+    return nbytes
+
+
+def _workspace(like: torch.Tensor, name: str, *sizes) -> Optional[torch.Tensor]:
+    nbytes = _bytes(name, *sizes)
+    return torch.empty(nbytes, dtype=torch.uint8, device=like.device) if nbytes else None
+
+
+def _at(t: Optional[torch.Tensor]):
+    return None if t is None else t.data_ptr()
+
+
+def _launch(device: torch.device, name: str, *args):
+    """The C entry on the tensors' device, whichever is current, on torch's current stream there."""
+    if device.index == torch.cuda.current_device():
+        rc = _function(name)(*args, torch._C._cuda_getCurrentRawStream(device.index))
+    else:
+        with torch.cuda.device(device):
+            rc = _function(name)(*args, torch._C._cuda_getCurrentRawStream(device.index))
+    if rc != 0:
+        _ffi.check(rc, name)
 
 
 def _quantize(name: str, x, per_block: int, dtype) -> tuple:
@@ -90,8 +105,7 @@ def _quantize(name: str, x, per_block: int, dtype) -> tuple:
     x = _aligned(x.detach())
     codes = torch.empty((m, per_block * blocks(k)), dtype=dtype, device=x.device)
     scales = torch.empty((m, blocks(k)), dtype=torch.uint8, device=x.device)
-    with _on(x):
-        call(name, ptr(x), kind, m, k, ptr(codes), ptr(scales), stream())
+    _launch(x.device, name, _at(x), kind, m, k, _at(codes), _at(scales))
     return codes, scales
 
 
@@ -100,8 +114,7 @@ def _dequantize(name: str, codes, scales, num_columns: int, dtype, per_block: in
     assert dtype in DTYPES, f"dtype must be float32, float16 or bfloat16, got {dtype}"
     codes = _aligned(codes)
     out = torch.empty((codes.shape[0], num_columns), dtype=dtype, device=codes.device)
-    with _on(codes):
-        call(name, ptr(codes), ptr(scales), codes.shape[0], num_columns, ptr(out), DTYPES[dtype], stream())
+    _launch(codes.device, name, _at(codes), _at(scales), codes.shape[0], num_columns, _at(out), DTYPES[dtype])
     return out
 
 
@@ -146,10 +159,9 @@ def _linear(x, codes, scales, bias, kind: int, tanh: bool, quantize_input: bool,
     y = torch.empty((m, n), dtype=x.dtype, device=x.device)
     dact = torch.empty((m, n), dtype=torch.float16, device=x.device) if want_dact else None
     if m:
-        with _on(x):
-            ws = _workspace(_ffi.lib().fmd_mxfp4_linear_workspace_bytes(kind, m, n, k, int(quantize_input)), x.device)
-            call("fmd_mxfp4_linear", ptr(x), kind, ptr(codes), ptr(scales), ptr(bias), ptr(y), ptr(dact), m, n, k, int(tanh),
-                 int(quantize_input), ptr(ws), stream())
+        ws = _workspace(x, "fmd_mxfp4_linear_workspace_bytes", kind, m, n, k, quantize_input)
+        _launch(x.device, "fmd_mxfp4_linear", _at(x), kind, _at(codes), _at(scales), _at(bias), _at(y), _at(dact), m, n, k, tanh,
+                quantize_input, _at(ws))
     return y, dact
 
 
@@ -188,10 +200,9 @@ class MXFP4LinearFunction(torch.autograd.Function):
         gb = torch.empty(n, dtype=g.dtype, device=g.device) if want_b else None
         codes = _aligned(codes)
         if m or want_b:
-            with _on(g):
-                ws = _workspace(_ffi.lib().fmd_mxfp4_linear_bwd_workspace_bytes(kind, m, n, ctx.k, int(want_x), int(want_b)), g.device)
-                call("fmd_mxfp4_linear_bwd", ptr(g), kind, ptr(aux), ctx.aux_kind, ptr(codes), ptr(scales), ptr(gx), ptr(gb), m, n,
-                     ctx.k, ptr(ws), stream())
+            ws = _workspace(g, "fmd_mxfp4_linear_bwd_workspace_bytes", kind, m, n, ctx.k, want_x, want_b)
+            _launch(g.device, "fmd_mxfp4_linear_bwd", _at(g), kind, _at(aux), ctx.aux_kind, _at(codes), _at(scales), _at(gx), _at(gb),
+                    m, n, ctx.k, _at(ws))
         return gx, None, None, gb, None, None
 
 
@@ -224,10 +235,9 @@ class LinearCkpt8Function(torch.autograd.Function):
         codes = torch.empty((m, BLOCK * blocks(k)), dtype=torch.int8, device=x.device) if keep else None
         scales = torch.empty((m, blocks(k)), dtype=torch.uint8, device=x.device) if keep else None
         if m:
-            with _on(x):
-                ws = _workspace(_ffi.lib().fmd_linear_ckpt8_workspace_bytes(kind, m, n, k), x.device)
-                call("fmd_linear_ckpt8", ptr(x), kind, ptr(w), ptr(bias), ptr(y), ptr(codes), ptr(scales), m, n, k, int(tanh),
-                     ptr(ws), stream())
+            ws = _workspace(x, "fmd_linear_ckpt8_workspace_bytes", kind, m, n, k)
+            _launch(x.device, "fmd_linear_ckpt8", _at(x), kind, _at(w), _at(bias), _at(y), _at(codes), _at(scales), m, n, k, tanh,
+                    _at(ws))
         ctx.save_for_backward(codes, scales, weight)
         ctx.tanh = tanh
         return y
@@ -245,11 +255,9 @@ class LinearCkpt8Function(torch.autograd.Function):
         gb = new(n, dtype=g.dtype, device=g.device) if want_b else None
         if m:
             kind, w = DTYPES[g.dtype], _aligned(weight)
-            with _on(g):
-                ws = _workspace(_ffi.lib().fmd_linear_ckpt8_bwd_workspace_bytes(kind, m, n, k, int(ctx.tanh), int(want_x), int(want_w),
-                                                                                int(want_b)), g.device)
-                call("fmd_linear_ckpt8_bwd", ptr(g), kind, ptr(codes), ptr(scales), ptr(w), ptr(gx), ptr(gw), ptr(gb), m, n, k,
-                     int(ctx.tanh), ptr(ws), stream())
+            ws = _workspace(g, "fmd_linear_ckpt8_bwd_workspace_bytes", kind, m, n, k, ctx.tanh, want_x, want_w, want_b)
+            _launch(g.device, "fmd_linear_ckpt8_bwd", _at(g), kind, _at(codes), _at(scales), _at(w), _at(gx), _at(gw), _at(gb), m, n, k,
+                    ctx.tanh, _at(ws))
         return gx, gw, gb, None
 
 
