@@ -107,10 +107,17 @@ class MLP(torch.nn.Module):
             layers += [torch.nn.Linear(w_in, w_out, bias=True), activation_func]
         layers.append(torch.nn.Linear(layer_widths[-2], layer_widths[-1], bias=last_bias))
         self.layers = torch.nn.Sequential(*layers)
+        self.checkpoint_bits = None  # set_activation_checkpoints
         for layer in self.layers:
             init_xavier_uniform(layer)
 
     def forward(self, x, data=None):
+        if self.checkpoint_bits == 8:
+            # Linear, then (tanh, Linear) pairs: each keeps its input for the backward pass in 8-bit blocks
+            for i, linear in enumerate(self.layers[0::2]):
+                op = K.fused_tanh_linear_ckpt8_autograd if i else K.linear_ckpt8_autograd
+                x = op(x.contiguous(), linear.weight.t().contiguous(), linear.bias)
+            return x
         return self.layers(x)
 
 
@@ -198,10 +205,13 @@ class InteractionBlock(torch.nn.Module):
         self.activation = activation or torch.nn.Tanh()
         self.lin = torch.nn.Linear(hidden_channels, hidden_channels)
         self.use_fused_tanh_linear = USE_FUSED_TANH_LINEAR and isinstance(self.activation, torch.nn.Tanh)
+        self.checkpoint_bits = None  # set_activation_checkpoints
         init_xavier_uniform(self.lin)
 
     def forward(self, x, edge_index, edge_weight, edge_attr, *args, csr_data: dict = None):
         x = self.conv(x, edge_index, edge_weight, edge_attr, csr_data=csr_data)
+        if self.checkpoint_bits == 8:
+            return K.fused_tanh_linear_ckpt8_autograd(x.contiguous(), self.lin.weight.t().contiguous(), self.lin.bias)
         if self.use_fused_tanh_linear:  # reference :534-541
             _need_gpu(x, "InteractionBlock")
             return K.fused_tanh_linear_autograd(x.contiguous(), self.lin.weight.t().contiguous(),
@@ -323,6 +333,27 @@ class StandardSchNet(SchNet):
         output_network = MLP([hidden_channels] + list(output_hidden_layer_widths) + [1], activation,
                              last_bias=False)
         super().__init__(embedding_layer, blocks, rbf_layer, output_network, max_num_neighbors)
+
+
+def set_activation_checkpoints(model: torch.nn.Module, bits: Optional[int] = 8) -> torch.nn.Module:
+    """Training with 8-bit activation checkpoints: the MLPs (filter and output networks) and the interaction blocks' output
+    layers of ``model`` keep their layers' inputs for the backward pass in 8-bit blocks (33 bytes for 32 values) instead of
+    in full; ``bits=None`` goes back.  Forward results are those of the layers without checkpoints up to fp32 rounding; the
+    weights' gradients, and the gradients that pass a tanh, come from the rounded values.  Parameters and their names stay as
+    they are.  Not in the reference.  Works on the operator path; the fused engine, which computes forces and nothing for
+    training, is not concerned.  W16A16 and MXFP4 networks are left alone."""
+    if bits not in (8, None):
+        raise ValueError(f"activation checkpoints in {bits} bits are not built: 8 or None")
+    found = [m for m in model.modules() if isinstance(m, (MLP, InteractionBlock))]
+    if not found:
+        raise ValueError("no MLP or InteractionBlock in this model")
+    for m in found:
+        acts = list(m.layers[1::2]) if isinstance(m, MLP) else [m.activation]
+        if bits == 8 and not all(isinstance(a, torch.nn.Tanh) for a in acts):
+            raise ValueError("8-bit activation checkpoints need tanh activations")
+    for m in found:
+        m.checkpoint_bits = bits
+    return model
 
 
 class GradientsOut(torch.nn.Module):

@@ -1,0 +1,142 @@
+"""Block-scaled layers without a GPU: refusals of the Python and of the C entry points, the oracle's own consistency, and what
+the module swaps do to a model's structure."""
+import ctypes
+
+import pytest
+import torch
+
+from oracle import mx_oracle as mo
+
+FP4 = torch.uint8
+
+
+def test_oracle_blocks_by_hand():
+    x = torch.tensor([[0.3, -0.3, 7.9, 1.0] + [0.0] * 28 + [1e-3]])
+    codes, scales, values = mo.mxfp4(x)
+    # amax 7.9: E = 2 - 2 = 0, so 0.3 -> 0.5, 7.9 -> 6, 1 -> 1; the short second block: 1e-3 = 1.024 * 2^-10, E = -12
+    assert values[0, :4].tolist() == [0.5, -0.5, 6.0, 1.0] and scales.tolist() == [[127, 115]]
+    assert codes[0, :2].tolist() == [0x1 | 0x9 << 4, 0x7 | 0x2 << 4] and float(values[0, 32]) == 4 * 2.0 ** -12
+    codes, scales, values = mo.mxint8(x)
+    assert scales.tolist() == [[129, 117]] and codes[0, :4].tolist() == [5, -5, 126, 16] and codes.shape == (1, 64)
+    assert float(values[0, 2]) == 126 / 64 * 4
+
+
+def test_cpu_tensors_are_refused():
+    import flashmd_amd.kernels as K
+
+    x, w, b = torch.zeros(4, 32), torch.zeros(32, 8), torch.zeros(8)
+    codes, scales = torch.zeros(8, 16, dtype=FP4), torch.zeros(8, 1, dtype=torch.uint8)
+    for f in (lambda: K.mxfp4_quantize(x), lambda: K.mxint8_quantize(x), lambda: K.mxfp4_dequantize(codes, scales, 32),
+              lambda: K.mxint8_dequantize(torch.zeros(8, 32, dtype=torch.int8), scales, 32), lambda: K.mxfp4_linear(x, codes, scales),
+              lambda: K.mxfp4_linear_autograd(x, codes, scales, b), lambda: K.linear_ckpt8_autograd(x, w, b),
+              lambda: K.fused_tanh_linear_ckpt8_autograd(x, w, b)):
+        with pytest.raises(RuntimeError, match="GPU"):
+            f()
+
+
+def test_names_are_public():
+    import flashmd_amd.kernels as K
+
+    for name in ("mxfp4_quantize", "mxfp4_dequantize", "mxint8_quantize", "mxint8_dequantize", "mxfp4_linear", "mxfp4_linear_autograd",
+                 "linear_ckpt8_autograd", "fused_tanh_linear_ckpt8_autograd"):
+        assert name in K.__all__ and callable(getattr(K, name))
+
+
+def test_c_entries_refuse_bad_arguments():
+    """Before anything is launched: sizes, types, null and misaligned pointers (the addresses are never read)."""
+    from flashmd_amd import _ffi
+
+    lib = _ffi.lib()
+    p, odd = ctypes.c_void_p(4096), ctypes.c_void_p(4097)
+    BAD, OK = -1, 0
+    for f in (lib.fmd_mxfp4_quantize, lib.fmd_mxint8_quantize):
+        assert f(p, 3, 4, 32, p, p, None) == BAD and f(p, 0, -1, 32, p, p, None) == BAD and f(p, 0, 4, 0, p, p, None) == BAD
+        assert f(None, 0, 4, 32, p, p, None) == BAD and f(odd, 0, 4, 32, p, p, None) == BAD and f(p, 0, 4, 32, odd, p, None) == BAD
+        assert f(p, 0, 4, 32, p, None, None) == BAD and f(None, 0, 0, 32, None, None, None) == OK
+    for f in (lib.fmd_mxfp4_dequantize, lib.fmd_mxint8_dequantize):
+        assert f(p, p, 4, 32, p, 5, None) == BAD and f(p, p, 4, 0, p, 0, None) == BAD and f(p, None, 4, 32, p, 0, None) == BAD
+        assert f(p, p, 4, 32, odd, 0, None) == BAD and f(None, None, 0, 32, None, 0, None) == OK
+
+    ws = lib.fmd_mxfp4_linear_workspace_bytes
+    assert ws(9, 4, 8, 32, 0) == BAD and ws(0, 4, 0, 32, 0) == BAD and ws(0, -4, 8, 32, 0) == BAD and ws(0, 4, 8, 1 << 25, 0) == BAD
+    assert ws(0, 0, 8, 32, 0) == 0 and ws(0, 1000, 128, 128, 1) == 0 and ws(2, 64, 4096, 4096, 0) == 0 and ws(2, 65, 4096, 4096, 0) > 0
+    f = lib.fmd_mxfp4_linear
+    assert f(None, 0, p, p, None, p, None, 4, 8, 32, 0, 0, None, None) == BAD and f(odd, 0, p, p, None, p, None, 4, 8, 32, 0, 0, None, None) == BAD
+    assert f(p, 0, odd, p, None, p, None, 4, 8, 32, 0, 0, None, None) == BAD and f(p, 0, p, None, None, p, None, 4, 8, 32, 0, 0, None, None) == BAD
+    assert f(p, 0, p, p, None, p, p, 4, 8, 32, 0, 0, None, None) == BAD                       # dact without tanh
+    assert f(p, 0, p, p, None, p, None, 1000, 8, 300, 0, 0, None, None) == BAD                # a workspace is needed
+    assert f(p, 0, p, p, None, p, None, 1000, 8, 300, 0, 0, odd, None) == BAD
+    assert f(p, 0, p, p, None, p, None, 1 << 31, 8, 300, 0, 1, p, None) == BAD                # rows of a 4-bit x are counted in 32 bits
+    assert f(None, 0, None, None, None, None, None, 0, 8, 32, 0, 0, None, None) == OK
+
+    f = lib.fmd_mxfp4_linear_bwd
+    assert f(p, 0, None, 3, p, p, p, p, 4, 8, 32, p, None) == BAD and f(p, 0, None, 1, p, p, p, p, 4, 8, 32, p, None) == BAD
+    assert f(p, 0, p, 2, p, p, p, p, 4, 8, 32, p, None) == BAD and f(p, 1, p, 1, p, p, p, p, 4, 8, 32, p, None) == BAD
+    assert f(None, 0, None, 0, p, p, p, p, 4, 8, 32, p, None) == BAD and f(p, 0, None, 0, None, p, p, p, 4, 8, 32, p, None) == BAD
+    assert f(p, 0, None, 0, p, p, p, None, 1000, 8, 300, None, None) == BAD
+    assert f(p, 0, None, 0, p, p, None, None, 4, 8, 32, None, None) == OK                     # nothing is wanted
+
+    f = lib.fmd_linear_ckpt8
+    assert f(p, 0, p, None, p, p, None, 4, 8, 32, 0, None, None) == BAD                       # codes without scales
+    assert f(p, 0, None, None, p, p, p, 4, 8, 32, 0, None, None) == BAD and f(p, 0, p, None, odd, p, p, 4, 8, 32, 0, None, None) == BAD
+    assert f(p, 0, p, None, p, p, p, 4, 8, 300, 0, None, None) == BAD and f(None, 0, None, None, None, None, None, 0, 8, 32, 0, None, None) == OK
+    f = lib.fmd_linear_ckpt8_bwd
+    assert f(p, 0, p, p, p, p, p, p, 0, 8, 32, 0, None, None) == BAD and f(p, 0, None, None, p, None, p, None, 4, 8, 32, 0, p, None) == BAD
+    assert f(p, 0, None, None, p, p, None, None, 4, 8, 32, 1, p, None) == BAD                 # tanh' needs the checkpoint
+    assert f(p, 0, None, None, None, p, None, None, 4, 8, 32, 0, p, None) == BAD              # gx needs the weight
+    assert f(p, 0, p, p, p, None, None, None, 4, 8, 32, 0, None, None) == OK
+    assert lib.fmd_linear_ckpt8_bwd_workspace_bytes(0, 0, 8, 32, 0, 1, 1, 1) == 0
+    assert lib.fmd_linear_ckpt8_bwd_workspace_bytes(0, 4, 8, -2, 0, 1, 1, 1) == BAD
+
+
+def test_workspaces_do_not_grow_with_the_rows():
+    """Large batches go through the wide path in chunks: what the planes of one take, not of all."""
+    from flashmd_amd import _ffi
+
+    lib = _ffi.lib()
+    one = lib.fmd_linear_ckpt8_workspace_bytes(0, 1 << 20, 256, 256)
+    assert 0 < one < 1 << 29 and lib.fmd_linear_ckpt8_workspace_bytes(0, 1 << 26, 256, 256) <= one + (1 << 20)
+
+
+def _model(activation=None):
+    import flashmd_amd.schnet as S
+
+    return S.StandardSchNet(S.GaussianBasis(S.CosineCutoff(0.0, 5.0), 20), S.CosineCutoff(0.0, 5.0), [16, 8], hidden_channels=16,
+                            embedding_size=10, num_filters=16, num_interactions=2, activation=activation)
+
+
+def test_activation_checkpoints_setting():
+    import flashmd_amd.schnet as S
+
+    model = _model()
+    names = list(model.state_dict())
+    with pytest.raises(ValueError, match="4 bits"):
+        S.set_activation_checkpoints(model, bits=4)
+    with pytest.raises(ValueError, match="no MLP"):
+        S.set_activation_checkpoints(torch.nn.Linear(2, 2))
+    assert S.set_activation_checkpoints(model) is model
+    marked = [m for m in model.modules() if isinstance(m, (S.MLP, S.InteractionBlock))]
+    assert len(marked) == 5 and all(m.checkpoint_bits == 8 for m in marked) and list(model.state_dict()) == names
+    with pytest.raises(RuntimeError, match="GPU"):
+        model.output_network(torch.zeros(3, 16))
+    S.set_activation_checkpoints(model, bits=None)
+    assert all(m.checkpoint_bits is None for m in marked) and model.output_network(torch.zeros(3, 16)).shape == (3, 1)
+    other = _model(torch.nn.SiLU())
+    with pytest.raises(ValueError, match="tanh"):
+        S.set_activation_checkpoints(other)
+    assert all(m.checkpoint_bits is None for m in other.modules() if isinstance(m, (S.MLP, S.InteractionBlock)))
+
+
+def test_mxfp4_swap_refusals():
+    from flashmd_amd.mxfp4 import MXFP4MLP, apply_mxfp4_to_model
+
+    model = _model()
+    with pytest.raises(RuntimeError, match="GPU"):
+        apply_mxfp4_to_model(model)
+    assert hasattr(model.output_network, "layers")           # nothing was swapped
+    with pytest.raises(RuntimeError, match="No filter networks"):
+        apply_mxfp4_to_model(torch.nn.Linear(2, 2))
+    with pytest.raises(ValueError, match="tanh"):
+        MXFP4MLP.from_mlp(_model(torch.nn.SiLU()).output_network)
+    with pytest.raises(RuntimeError, match="GPU"):
+        MXFP4MLP()(torch.zeros(2, 3))

@@ -201,3 +201,324 @@ def test_no_rows(K):
     y = K.mxfp4_linear_autograd(x, c, s, b, "tanh")
     gx, gb = torch.autograd.grad(y, (x, b), torch.empty(0, 7, device=DEV))
     assert y.shape == (0, 7) and gx.shape == (0, 40) and float(gb.abs().max()) == 0.0
+
+
+# ---------------------------------------------------------------------------------------- refusals and how a call may be made
+def test_refusals(K):
+    x, w, b = rand(4, 40).to(DEV), rand(40, 8).to(DEV), rand(8).to(DEV)
+    codes, scales = K.mxfp4_quantize(w.t().contiguous())
+    bad = [lambda: K.mxfp4_quantize(x.double()), lambda: K.mxfp4_quantize(x[0]), lambda: K.mxfp4_quantize(x[:, ::2]),
+           lambda: K.mxint8_quantize(x.t()), lambda: K.mxfp4_dequantize(codes, scales, 65), lambda: K.mxfp4_dequantize(codes, scales, 40, torch.int8),
+           lambda: K.mxint8_dequantize(codes, scales, 40), lambda: K.mxfp4_linear(x, codes, scales, activation="relu"),
+           lambda: K.mxfp4_linear(x[:, :31].contiguous(), codes, scales), lambda: K.mxfp4_linear(x, codes, scales, b.half()),
+           lambda: K.mxfp4_linear(x, codes, scales, b[:7]), lambda: K.mxfp4_linear(x, codes.cpu(), scales.cpu()),
+           lambda: K.mxfp4_linear(x, codes[:, :16].contiguous(), scales), lambda: K.mxfp4_linear(x, codes.char(), scales),
+           lambda: K.linear_ckpt8_autograd(x, w.half()), lambda: K.linear_ckpt8_autograd(x, w.t()), lambda: K.linear_ckpt8_autograd(x, w[:39].contiguous()),
+           lambda: K.linear_ckpt8_autograd(x.view(2, 2, 40), w), lambda: K.fused_tanh_linear_ckpt8_autograd(x, w, b[::2]),
+           lambda: K.linear_ckpt8_autograd(x[:, :0].contiguous(), w[:0].contiguous())]
+    for i, f in enumerate(bad):
+        with pytest.raises((AssertionError, RuntimeError)):
+            f()
+            print("not refused:", i)
+    xg = x.clone().requires_grad_()
+    (gx,) = torch.autograd.grad(K.linear_ckpt8_autograd(xg, w, b).sum(), xg, create_graph=True)
+    with pytest.raises(RuntimeError):
+        gx.sum().backward()                                  # not differentiable again
+
+
+def test_expanded_gradients_and_backward(K):
+    """.sum().backward(): a gradient of stride 0; leaves accumulate over two passes."""
+    x, w, b = (t.to(DEV).requires_grad_() for t in (rand(50, 40, seed=1), rand(40, 33, seed=2), rand(33, seed=3)))
+    for _ in range(2):
+        K.fused_tanh_linear_ckpt8_autograd(x, w, b).sum().backward()
+    _, gx, gw, gb = mo.linear_ckpt8(x.detach().cpu(), w.detach().cpu(), b.detach().cpu(), True, torch.full((50, 33), 2.0))
+    near(x.grad, gx, 33)
+    near(w.grad, gw, 50)
+    near(b.grad, gb, 50)
+
+
+def test_gradients_against_differences(K):
+    """Central differences of the operators themselves along a direction, at step d: off by d^2/6 of the third derivative (tanh'''
+    is at most 2: d^2/3 of the direction's cube) and by the outputs' rounding over d.  With d = 2^-6 both are below 1e-3 of the
+    derivative's scale; the 8-bit checkpoints add at most 2^-7 of a block's largest value to x."""
+    m, k, n, d = 64, 50, 40, 2.0 ** -6
+    x, w, b, v = rand(m, k, seed=1), rand(n, k, seed=2, scale=0.2), rand(n, seed=3, scale=0.1), rand(m, k, seed=4)
+    g = rand(m, n, seed=5)
+    codes, scales, _ = mo.mxfp4(w)
+    c, s, bg, G = codes.to(DEV), scales.to(DEV), b.to(DEV), g.to(DEV)
+
+    def f(t):
+        return float((K.mxfp4_linear(t.to(DEV), c, s, bg, "tanh").double() * G.double()).sum())
+
+    xg = x.to(DEV).requires_grad_()
+    (gx,) = torch.autograd.grad(K.mxfp4_linear_autograd(xg, c, s, bg, "tanh"), xg, G)
+    diff, grad = (f(x + d * v) - f(x - d * v)) / (2 * d), float((gx.double().cpu() * v.double()).sum())
+    scale = float(gx.double().norm()) * float(v.double().norm())
+    assert abs(diff - grad) < 1e-3 * scale
+
+    wt = w.t().contiguous()
+    for tanh, op in ((False, K.linear_ckpt8_autograd), (True, K.fused_tanh_linear_ckpt8_autograd)):
+        leaves = [t.to(DEV).requires_grad_() for t in (x, wt, b)]
+        got = torch.autograd.grad(op(*leaves), leaves, G)
+        for i, base in enumerate((x, wt, b)):
+            u = rand(*base.shape, seed=6 + i)
+
+            def at(sign):
+                moved = [t.to(DEV) for t in (x, wt, b)]
+                moved[i] = (base + sign * d * u).to(DEV)
+                return float((op(*moved).double() * G.double()).sum())
+
+            diff, grad = (at(1) - at(-1)) / (2 * d), float((got[i].double().cpu() * u.double()).sum())
+            scale = float(got[i].double().norm()) * float(u.double().norm())
+            # a kept value is off by at most 2^-7 of its block's largest: of a gradient's 2-norm at most 2^-7 amax/rms (below 4
+            # here), twice over where tanh' and the difference meet
+            assert abs(diff - grad) < (1e-3 + (2 * 4 * 2.0 ** -7 if i < 2 else 0.0)) * scale, (tanh, i)
+
+
+def test_rows_behind_the_last_are_left_alone(K):
+    """The C entries write m rows and nothing behind them, in every path that stores rows."""
+    from flashmd_amd import _ffi
+    from flashmd_amd._ffi import call, ptr, stream
+
+    lib = _ffi.lib()
+    for m, k, n in ((1, 50, 33), (33, 128, 128), (37, 64, 20), (45, 40, 64), (20, 300, 70), (100, 300, 131), (300, 130, 64)):
+        x, w, g = rand(m, k, seed=1).to(DEV), rand(k, n, seed=2).to(DEV), rand(m, n, seed=3).to(DEV)
+        nb, nbn = (k + 31) // 32, (n + 31) // 32
+        wc, wsc = K.mxfp4_quantize(w.t().contiguous())
+        more = 40
+
+        def room(*shape, dtype=torch.float32):
+            return torch.full(shape, 77, dtype=dtype, device=DEV)
+
+        def behind(t):
+            return bool((t[m:] == 77).all())
+
+        for tanh in (0, 1):
+            y, c8, s8 = room(m + more, n), room(m + more, 32 * nb, dtype=torch.int8), room(m + more, nb, dtype=torch.uint8)
+            ws = torch.empty(max(16, lib.fmd_linear_ckpt8_workspace_bytes(0, m, n, k)), dtype=torch.uint8, device=DEV)
+            call("fmd_linear_ckpt8", ptr(x), 0, ptr(w), None, ptr(y), ptr(c8), ptr(s8), m, n, k, tanh, ptr(ws), stream())
+            assert behind(y) and behind(c8) and behind(s8)
+            gx, gw, gb = room(m + more, k), room(k + more, n), room(n + more)
+            ws = torch.empty(max(16, lib.fmd_linear_ckpt8_bwd_workspace_bytes(0, m, n, k, tanh, 1, 1, 1)), dtype=torch.uint8, device=DEV)
+            call("fmd_linear_ckpt8_bwd", ptr(g), 0, ptr(c8), ptr(s8), ptr(w), ptr(gx), ptr(gw), ptr(gb), m, n, k, tanh, ptr(ws), stream())
+            assert behind(gx) and bool((gw[k:] == 77).all()) and bool((gb[n:] == 77).all())
+            for both in (0, 1):
+                y = room(m + more, n)
+                ws = torch.empty(max(16, lib.fmd_mxfp4_linear_workspace_bytes(0, m, n, k, both)), dtype=torch.uint8, device=DEV)
+                call("fmd_mxfp4_linear", ptr(x), 0, ptr(wc), ptr(wsc), None, ptr(y), None, m, n, k, tanh, both, ptr(ws), stream())
+                assert behind(y)
+            gx, gb = room(m + more, k), room(n + more)
+            ws = torch.empty(max(16, lib.fmd_mxfp4_linear_bwd_workspace_bytes(0, m, n, k, 1, 1)), dtype=torch.uint8, device=DEV)
+            call("fmd_mxfp4_linear_bwd", ptr(g), 0, ptr(y), tanh, ptr(wc), ptr(wsc), ptr(gx), ptr(gb), m, n, k, ptr(ws), stream())
+            assert behind(gx) and bool((gb[n:] == 77).all())
+        for q, dq, per, dt in ((K.mxfp4_quantize, "fmd_mxfp4_dequantize", 16, torch.uint8), (K.mxint8_quantize, "fmd_mxint8_dequantize", 32, torch.int8)):
+            c, s = q(x)
+            out = room(m + more, k)
+            call(dq, ptr(c), ptr(s), m, k, ptr(out), 0, stream())
+            c2, s2 = room(m + more, per * nb, dtype=dt), room(m + more, nb, dtype=torch.uint8)
+            call(dq.replace("dequantize", "quantize"), ptr(x), 0, m, k, ptr(c2), ptr(s2), stream())
+            assert behind(out) and behind(c2) and behind(s2) and torch.equal(c2[:m], c) and torch.equal(s2[:m], s)
+
+
+SIZES = [(77, 50, 128), (300, 128, 128), (40, 300, 130), (300, 300, 130)]
+
+
+def _step(K, x, w, b, codes, scales, g):
+    y = K.fused_tanh_linear_ckpt8_autograd(x, w, b)
+    gx, gw, gb = torch.autograd.grad(y, (x, w, b), g)
+    z = K.mxfp4_linear_autograd(x, codes, scales, b, "tanh")
+    hx, hb = torch.autograd.grad(z, (x, b), g)
+    q = K.mxfp4_linear(x.detach(), codes, scales, quantize_input=True)
+    return y.detach(), gx, gw, gb, z.detach(), hx, hb, q
+
+
+def _inputs(K, m, k, n, seed=0):
+    x, w, b, g = rand(m, k, seed=seed), rand(k, n, seed=seed + 1, scale=0.2), rand(n, seed=seed + 2), rand(m, n, seed=seed + 3)
+    codes, scales = K.mxfp4_quantize(w.t().contiguous().to(DEV))
+    return [t.to(DEV).requires_grad_() for t in (x, w, b)] + [codes, scales, g.to(DEV)]
+
+
+@pytest.mark.parametrize("m,k,n", SIZES)
+def test_repeats_and_other_streams(K, m, k, n):
+    """Bitwise the same again, on another stream, and with two streams at work at once (nothing is shared between calls)."""
+    one, two = _inputs(K, m, k, n), _inputs(K, m, k, n, seed=10)
+    want_one, want_two = _step(K, *one), _step(K, *two)
+    assert all(torch.equal(a, b) for a, b in zip(want_one, _step(K, *one)))
+    torch.cuda.synchronize()
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    for _ in range(5):
+        with torch.cuda.stream(s1):
+            got_one = _step(K, *one)
+        with torch.cuda.stream(s2):
+            got_two = _step(K, *two)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(want_one, got_one)) and all(torch.equal(a, b) for a, b in zip(want_two, got_two))
+
+
+@pytest.mark.parametrize("m,k,n", SIZES)
+def test_captured_and_replayed(K, m, k, n):
+    """Forward and backward in one graph; replays with new inputs, eager work between them."""
+    ins = _inputs(K, m, k, n)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            _step(K, *ins)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = _step(K, *ins)
+    for i in range(4):
+        new = _inputs(K, m, k, n, seed=20 + 10 * i)
+        with torch.no_grad():
+            for a, b in zip(ins, new):
+                a.copy_(b)
+        graph.replay()
+        torch.cuda.synchronize()
+        want = _step(K, *new)
+        assert all(torch.equal(a, b) for a, b in zip(out, want)), i
+
+
+def test_offsets_beyond_32_bits(K):
+    """2^31 elements and more: the last rows of a tensor whose byte (quantise, layer) and element offsets pass 2^32 and 2^31."""
+    m, k = 17_000_003, 128
+    x = torch.zeros(m, k, dtype=torch.bfloat16, device=DEV)
+    tail = rand(70, k, seed=1, dtype=torch.bfloat16)
+    x[-70:] = tail.to(DEV)
+    codes, scales = K.mxfp4_quantize(x)
+    assert torch.equal(codes[-70:].cpu(), mo.mxfp4(tail)[0]) and torch.equal(scales[-70:].cpu(), mo.mxfp4(tail)[1])
+    assert int(codes[:-70].max()) == 0
+    values = K.mxfp4_dequantize(codes, scales, k, dtype=torch.bfloat16)
+    assert torch.equal(values[-70:].cpu().double(), mo.mxfp4(tail)[2])
+    del values, codes, scales
+    w, b = rand(k, 8, seed=2, dtype=torch.bfloat16), rand(8, seed=3, dtype=torch.bfloat16)
+    xg, wg = x.requires_grad_(), w.to(DEV).requires_grad_()
+    y = K.fused_tanh_linear_ckpt8_autograd(xg, wg, b.to(DEV))
+    g = torch.zeros(m, 8, dtype=torch.bfloat16, device=DEV)
+    gt = rand(70, 8, seed=4, dtype=torch.bfloat16)
+    g[-70:] = gt.to(DEV)
+    gx, gw = torch.autograd.grad(y, (xg, wg), g)
+    y_ref, gx_ref, gw_ref, _ = mo.linear_ckpt8(tail, w, b, True, gt)
+    near(y[-70:], y_ref, k)
+    near(gx[-70:], gx_ref, 8)
+    near(gw, gw_ref, 70)
+    wc, wsc, wv = mo.mxfp4(w.t().contiguous().float())
+    near(K.mxfp4_linear(x.detach(), wc.to(DEV), wsc.to(DEV))[-70:], mo.linear(tail, wv), k)
+
+
+@pytest.mark.parametrize("m,k,n", [(70000, 128, 128), (70001, 50, 128), (66000, 100, 30), (300_000, 130, 40), (70016, 64, 64)])
+def test_many_rows(K, m, k, n):
+    """Where the weight gradient sums over slices of the rows, and the wide path goes in chunks; small whole numbers, so that every
+    product and sum is exact and the result has to be equal to the last bit."""
+    gen = torch.Generator().manual_seed(m)
+    x = torch.randint(-2, 3, (m, k), generator=gen).float()
+    x[:, 0] = 64.0                                            # with 64 the largest of its block, whole numbers are kept whole
+    x[:, 32::32] = 64.0
+    w, b = torch.randint(-2, 3, (k, n), generator=gen).float(), torch.randint(-3, 4, (n,), generator=gen).float()
+    g = torch.randint(-1, 2, (m, n), generator=gen).float()
+    leaves = [t.to(DEV).requires_grad_() for t in (x, w, b)]
+    y = K.linear_ckpt8_autograd(*leaves)
+    gx, gw, gb = torch.autograd.grad(y, leaves, g.to(DEV))
+    X, W, G = x.to(DEV).double(), w.to(DEV).double(), g.to(DEV).double()
+    assert torch.equal(y.detach().double(), X @ W + b.to(DEV).double()) and torch.equal(gx.double(), G @ W.t().contiguous())
+    assert torch.equal(gw.double(), X.t().contiguous() @ G) and torch.equal(gb.double(), G.sum(0))
+
+
+# ---------------------------------------------------------------------------------------- together, in a model
+def _schnet(hidden=32, filters=32, rbf=20):
+    import flashmd_amd.schnet as S
+
+    torch.manual_seed(3)
+    return S.StandardSchNet(S.GaussianBasis(S.CosineCutoff(0.0, 5.0), rbf), S.CosineCutoff(0.0, 5.0), [32, 16], hidden_channels=hidden,
+                            embedding_size=30, num_filters=filters, num_interactions=2)
+
+
+def _batch(S, dev=DEV, dtype=torch.float32):
+    from oracle import schnet_oracle as so
+
+    pos, types, ptr_ = so.synth_batch(3, 37, 5.0)
+    return S.Batch(pos.to(dev, dtype), types.to(dev), ptr_.to(dev), max_beads_per_mol=37)
+
+
+def _plain_run(model, S, params=None):
+    """The model in 64 bits on the CPU with plain torch operations; energies, forces, gradients of `params` for sum(energy^2)"""
+    from oracle import schnet_oracle as so
+
+    data = _batch(S, "cpu", torch.float64)
+    src, dst = so.radius_graph(data.pos.float(), data.ptr, 5.0)
+    data.pos.requires_grad_(True)
+    x = model.embedding_layer(data.atom_types)
+    d = (data.pos[dst] - data.pos[src]).norm(dim=1)
+    rbf = model.rbf_layer(d)
+    for blk in model.interaction_blocks:
+        h = blk.conv.lin1(x)
+        wf = blk.conv.filter_network.layers(rbf) * blk.conv.cutoff(d).view(-1, 1)
+        h = blk.conv.lin2(torch.zeros_like(h).index_add_(0, dst, h[src] * wf))
+        x = x + blk.lin(torch.tanh(h))
+    e = torch.zeros(3, dtype=torch.float64).index_add_(0, data.batch, model.output_network.layers(x).flatten())
+    forces = -torch.autograd.grad(e.sum(), data.pos, retain_graph=True)[0]
+    grads = torch.autograd.grad((e * e).sum(), params) if params else None
+    return e.detach(), forces, grads
+
+
+def test_mxfp4_model_is_the_model_with_rounded_weights():
+    """apply_mxfp4_to_model: energies and forces equal those of the same model in 64 bits with the blocks' values as weights (the
+    operator path's fp32 budget for them is 1e-5); an engine made before the swap is not used again."""
+    import copy
+
+    import flashmd_amd.schnet as S
+    from flashmd_amd.mxfp4 import MXFP4MLP, apply_mxfp4_to_model
+
+    model = _schnet().to(DEV).eval()
+    plain = copy.deepcopy(model).cpu()
+    before = S.GradientsOut(model)(_batch(S)).out["SchNet"]["energy"]     # makes the engine
+    apply_mxfp4_to_model(model)
+    nets = [(p, q) for p, q in zip([b.conv.filter_network for b in plain.interaction_blocks] + [plain.output_network],
+                                   [b.conv.filter_network for b in model.interaction_blocks] + [model.output_network])]
+    with torch.no_grad():
+        for p, q in nets:
+            assert isinstance(q, MXFP4MLP)
+            for i, linear in enumerate(p.layers[0::2]):
+                linear.weight.copy_(q.weight(i).cpu())
+                assert torch.equal(linear.weight.double(), mo.mxfp4(linear.weight.detach())[2])  # blocks of blocks are themselves
+    e_ref, f_ref, _ = _plain_run(plain.double(), S)
+    out = S.GradientsOut(model)(_batch(S)).out["SchNet"]
+    assert not torch.equal(out["energy"].detach(), before.detach())
+    assert rel(out["energy"], e_ref) < 1e-5 and rel(out["forces"], f_ref) < 1e-5
+    # a copy with narrow activations, too, runs and stays finite
+    narrow = _schnet().to(DEV).eval()
+    apply_mxfp4_to_model(narrow, quantize_activations=True)
+    out = S.GradientsOut(narrow)(_batch(S)).out["SchNet"]
+    assert bool(torch.isfinite(out["energy"]).all()) and bool(torch.isfinite(out["forces"]).all())
+
+
+def test_training_step_with_activation_checkpoints():
+    """set_activation_checkpoints: energies as without; the parameters' gradients of a loss of the energies against 64 bits.  A
+    kept value is off by at most 2^-7 of its block's largest, uniformly: 2^-7 / sqrt(3) of amax in the root mean square, with
+    amax at most 4 times the block's rms about 2% of x, and that much of a gradient that is linear in it; a chain of five
+    such layers at most 5 times that."""
+    import copy
+
+    import flashmd_amd.schnet as S
+
+    model = _schnet().to(DEV).train()
+    plain = copy.deepcopy(model).cpu().double()
+    names = [n for n, p in model.named_parameters()]
+    e_ref, _, want = _plain_run(plain, S, list(plain.parameters()))
+
+    def step():
+        e = model(_batch(S)).out["SchNet"]["energy"]
+        return e.detach(), torch.autograd.grad((e * e).sum(), list(model.parameters()))
+
+    e0, exact = step()
+    S.set_activation_checkpoints(model)
+    e8, got = step()
+    S.set_activation_checkpoints(model, None)
+    assert rel(e0, e_ref) < 1e-5 and rel(e8, e_ref) < 1e-5
+    off = {n: rel(g, w) for n, g, w in zip(names, got, want)}
+    assert max(off.values()) < 0.1, off
+    assert max(rel(g, w) for g, w in zip(exact, want)) < 1e-4
+    assert any(v > 1e-4 for v in off.values())               # the checkpoints were used
+    e1, again = step()
+    assert torch.equal(e1, e0) and all(rel(a, b) < 1e-5 for a, b in zip(again, exact))
