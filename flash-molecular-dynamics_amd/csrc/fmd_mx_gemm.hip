@@ -113,6 +113,36 @@ __global__ __launch_bounds__(256) void planes_kernel(S src, int64_t rows, int64_
   }
 }
 
+// the same of p(x), and x in 8-bit blocks (four neighbouring lanes hold a block and are active together: pad is a multiple of 64)
+template <class T, bool TANH, int P>
+__global__ __launch_bounds__(256) void planes_keep_kernel(SrcDense<T, false> src, int64_t rows, int64_t pad, uint16_t* __restrict__ out,
+                                                          int64_t nb, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
+  const int64_t per = pad >> 3, total = rows * per;
+  for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < total; t += (int64_t)gridDim.x * 256) {
+    const int64_t row = t / per, q = t - row * per, b = q >> 2;
+    float v[8];
+    src.load(row, q * 8, v);
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = max(top, __builtin_bit_cast(uint32_t, v[i]) & 0x7fffffffu);
+    top = max(top, (uint32_t)__shfl_xor((int)top, 1, 64));
+    top = max(top, (uint32_t)__shfl_xor((int)top, 2, 64));
+    const uint32_t byte = mx_scale_byte<8>(top);
+    if (b < nb) {
+      *(u32x2*)(codes + (row * nb + b) * 32 + (q & 3) * 8) =
+          u32x2{mx_codes8(v[0], v[1], v[2], v[3], byte), mx_codes8(v[4], v[5], v[6], v[7], byte)};
+      if ((q & 3) == 0) scales[row * nb + b] = (uint8_t)byte;
+    }
+    if constexpr (TANH)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = mx_tanh(v[i]);
+    u32x4 o[P];
+    mx_split8<P>(v, o);
+#pragma unroll
+    for (int p = 0; p < P; ++p) *(u32x4*)(out + (int64_t)p * rows * pad + row * pad + q * 8) = o[p];
+  }
+}
+
 // rows x cols -> planes [P][cols][pad] of the transposed matrix (pad = rows rounded up to 64, zeros behind rows); 64 x 64 tiles
 // through LDS, rows 66 halves apart so that neither side meets a bank twice more than it has to
 template <class S, int P>
@@ -155,15 +185,18 @@ __global__ __launch_bounds__(256) void planes_t_kernel(S src, int64_t rows, int6
   }
 }
 
-// scales [rows][nb] -> [tile of 8 blocks][rows][8], zeros behind nb
-__global__ __launch_bounds__(256) void scale_tiles_kernel(const uint8_t* __restrict__ s, int64_t rows, int64_t nb, int64_t kt,
-                                                          uint64_t* __restrict__ out) {
-  for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < rows * kt; t += (int64_t)gridDim.x * 256) {
+// scales [rows][nb] -> [tile of 8 blocks][half][row][4], zeros behind nb: block 2 s + half of a tile is byte s, what one half of a wave
+// needs in the four steps of a tile
+__global__ __launch_bounds__(256) void scale_tiles_kernel(const uint8_t* __restrict__ s, int64_t rows, int64_t pad, int64_t nb, int64_t kt,
+                                                          uint32_t* __restrict__ out) {
+  for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < rows * kt * 2; t += (int64_t)gridDim.x * 256) {
     const int64_t q = t / rows, row = t - q * rows;
-    uint64_t v = 0;
-    for (int i = 0; i < 8; ++i)
-      if (q * 8 + i < nb) v |= (uint64_t)s[row * nb + q * 8 + i] << (8 * i);
-    out[t] = v;
+    uint32_t v = 0;
+    for (int i = 0; i < 4; ++i) {
+      const int64_t b = (q >> 1) * 8 + 2 * i + (q & 1);
+      if (b < nb) v |= (uint32_t)s[row * nb + b] << (8 * i);
+    }
+    out[q * pad + row] = v;
   }
 }
 
@@ -176,12 +209,10 @@ __global__ __launch_bounds__(256) void scale_tiles_kernel(const uint8_t* __restr
 // neighbouring lanes meet 16 different slots.  That row order also gives a lane T neighbouring columns of C.  (With the two rows
 // of a line swizzled apart, half the banks served a read: 4 conflict cycles on 4.)
 // =====================================================================================================================
-__device__ u32x4 mx_zero_granule;
-
 struct GemmArgs {
   const char *a, *b;
   int64_t a_plane, b_plane, a_pitch, b_pitch;  // bytes
-  const uint64_t *sa, *sb;                     // 4-bit operands: scales [tile][row][8]
+  const char *sa, *sb;                         // 4-bit operands: scales [tile][half][row][4]
   int m, n, kt, granules, tiles_m, tiles_n, splits, npairs;
   uint32_t pa, pb;                             // planes of pair i: bits 2i, 2i+1
   MxEpilogue e;
@@ -205,7 +236,7 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_kernel(const GemmArgs g) {
   static_assert(TM % 2 == 0 && TN % 2 == 0, "two rows of a line belong to one lane");
   constexpr int BM = 32 * WM * TM, BN = 32 * WN * TN, NW = WM * WN, SLOTS = (BM + BN) * 8, LOADS = SLOTS / (64 * NW);
   __shared__ __attribute__((aligned(16))) char lds[2 * (BM + BN) * 128];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, j = lane & 31, h = lane >> 5;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), j = lane & 31, h = lane >> 5;
   const int wm = wave / WN, wn = wave % WN;
   // one XCD gets a run of neighbouring tiles (workgroups are dealt to the eight XCDs in turn), eight tile rows at a time
   int bid = blockIdx.x;
@@ -226,19 +257,20 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_kernel(const GemmArgs g) {
     const int id = (slot & 15) ^ ((is_a ? 2 * line / TM : 2 * line / TN) & 15), rr = 2 * line + (id >> 3);
     gran[i] = id & 7;
     const int row = is_a ? min(m0 + rr, g.m - 1) : min(n0 + rr, g.n - 1);
-    off[i] = (int64_t)row * (is_a ? g.a_pitch : g.b_pitch) + gran[i] * 16;
+    off[i] = (int64_t)row * (is_a ? g.a_pitch : g.b_pitch) + (FP4 ? 0 : gran[i] * 16);
   }
   auto issue = [&](int pair, int t, char* buf) {
-    const char* pa = g.a + (g.pa >> 2 * pair & 3) * g.a_plane + (int64_t)t * 128;
-    const char* pb = g.b + (g.pb >> 2 * pair & 3) * g.b_plane + (int64_t)t * 128;
-#pragma unroll
-    for (int i = 0; i < LOADS; ++i) {
-      const bool is_a = (i * NW + wave) * 64 < BM * 8;
-      const char* src = (is_a ? pa : pb) + off[i];
-      if (FP4 && t * 8 + gran[i] >= g.granules) src = (const char*)&mx_zero_granule;
+    // 4-bit rows may end inside a tile: the granules behind stand for the last one again, under scales of 2^-127 on either side
+    const char *pa = g.a + (FP4 ? 0 : (int64_t)t * 128), *pb = g.b + (FP4 ? 0 : (int64_t)t * 128);
+    if constexpr (!FP4) pa += (g.pa >> 2 * pair & 3) * g.a_plane, pb += (g.pb >> 2 * pair & 3) * g.b_plane;
+    auto direct = [&](int i, const char* src) {
       __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
                                        (__attribute__((address_space(3))) void*)(buf + (i * NW + wave) * 1024), 16, 0, 0);
-    }
+    };
+    auto place = [&](int i) { return ((i * NW + wave) * 64 < BM * 8 ? pa : pb) + off[i]; };
+    // one straight line, so that the loads can be laid between the matrix instructions
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) direct(i, place(i) + (FP4 ? (uint32_t)min(t * 8 + gran[i], g.granules - 1) * 16 : 0));
   };
   f32x16 acc[TM][TN];
 #pragma unroll
@@ -248,46 +280,72 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_kernel(const GemmArgs g) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[a][b][r] = 0.f;
 
-  uint64_t sa_next[TM], sb_next[TN];
+  // scales: the TM (TN) neighbouring rows of a lane, four steps each, in one load
+  typedef uint32_t ScalesA __attribute__((ext_vector_type(TM)));
+  typedef uint32_t ScalesB __attribute__((ext_vector_type(TN)));
+  ScalesA sa_next;
+  ScalesB sb_next;
+  const int pad_m = (g.m + 3) & ~3, pad_n = (g.n + 3) & ~3;
+  const int64_t off_sa = 4 * ((int64_t)h * pad_m + min(m0 + (wm * 32 + j) * TM, pad_m - TM));
+  const int64_t off_sb = 4 * ((int64_t)h * pad_n + min(n0 + (wn * 32 + j) * TN, pad_n - TN));
   auto load_scales = [&](int t) {
     if constexpr (FP4) {
-#pragma unroll
-      for (int a = 0; a < TM; ++a) sa_next[a] = g.sa[(int64_t)t * g.m + min(m0 + (wm * 32 + j) * TM + a, g.m - 1)];
-#pragma unroll
-      for (int b = 0; b < TN; ++b) sb_next[b] = g.sb[(int64_t)t * g.n + min(n0 + (wn * 32 + j) * TN + b, g.n - 1)];
+      sa_next = *(const ScalesA*)(g.sa + (int64_t)t * pad_m * 8 + off_sa);
+      sb_next = *(const ScalesB*)(g.sb + (int64_t)t * pad_n * 8 + off_sb);
     }
   };
-  uint32_t sa[TM], sb[TN];
+  ScalesA sa;
+  ScalesB sb;
   auto take_scales = [&]() {
-    if constexpr (FP4) {  // bytes h, h+2, h+4, h+6: the scales of this half wave's block in each of the four steps
-      const uint32_t pick = h ? 0x07050301u : 0x06040200u;
-#pragma unroll
-      for (int a = 0; a < TM; ++a) sa[a] = __builtin_amdgcn_perm((uint32_t)(sa_next[a] >> 32), (uint32_t)sa_next[a], pick);
-#pragma unroll
-      for (int b = 0; b < TN; ++b) sb[b] = __builtin_amdgcn_perm((uint32_t)(sb_next[b] >> 32), (uint32_t)sb_next[b], pick);
-    }
+    if constexpr (FP4) sa = sa_next, sb = sb_next;
   };
-  auto compute = [&](const char* buf) {
+  auto compute = [&](const char* buf, auto between) {  // between: what is done once the matrix unit has work
     const char* la = buf + (wm * 32 + j) * TM * 128;
     const char* lb = buf + BM * 128 + (wn * 32 + j) * TN * 128;
+    // the fragments of the next step are read while this one's matrix instructions run
+    u32x4 fa[2][TM], fb[2][TN];
+    auto read = [&](int s) {
+      const int q = s * 2 + h, at = (q ^ (j & 15)) * 16, odd = ((8 + q) ^ (j & 15)) * 16;
+#pragma unroll
+      for (int a = 0; a < TM; ++a) fa[s & 1][a] = *(const u32x4*)(la + (a >> 1) * 256 + (a & 1 ? odd : at));
+#pragma unroll
+      for (int b = 0; b < TN; ++b) fb[s & 1][b] = *(const u32x4*)(lb + (b >> 1) * 256 + (b & 1 ? odd : at));
+    };
+    read(0);
 #define MX_STEP(s)                                                                                                          \
   {                                                                                                                         \
-    const int q = (s) * 2 + h, at = (q ^ (j & 15)) * 16, odd = ((8 + q) ^ (j & 15)) * 16;                                   \
-    u32x4 fa[TM], fb[TN];                                                                                                   \
-    _Pragma("unroll") for (int a = 0; a < TM; ++a) fa[a] = *(const u32x4*)(la + (a >> 1) * 256 + (a & 1 ? odd : at));        \
-    _Pragma("unroll") for (int b = 0; b < TN; ++b) fb[b] = *(const u32x4*)(lb + (b >> 1) * 256 + (b & 1 ? odd : at));        \
+    if (s < 3) read(s + 1);                                                                                                 \
     _Pragma("unroll") for (int a = 0; a < TM; ++a) _Pragma("unroll") for (int b = 0; b < TN; ++b) {                         \
+      const u32x4 ua = fa[s & 1][a], ub = fb[s & 1][b];                                                                     \
       if constexpr (FP4) {                                                                                                  \
-        const i32x8 xa = {(int)fa[a][0], (int)fa[a][1], (int)fa[a][2], (int)fa[a][3], 0, 0, 0, 0};                          \
-        const i32x8 xb = {(int)fb[b][0], (int)fb[b][1], (int)fb[b][2], (int)fb[b][3], 0, 0, 0, 0};                          \
-        acc[a][b] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(xa, xb, acc[a][b], 4, 4, (s), (int)sa[a], (s), (int)sb[b]); \
+        const i32x8 xa = {(int)ua[0], (int)ua[1], (int)ua[2], (int)ua[3], 0, 0, 0, 0};                                      \
+        const i32x8 xb = {(int)ub[0], (int)ub[1], (int)ub[2], (int)ub[3], 0, 0, 0, 0};                                      \
+        acc[a][b] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(xa, xb, acc[a][b], 4, 4, s, (int)sa[a], s, (int)sb[b]); \
       } else {                                                                                                              \
-        acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, fa[a]), __builtin_bit_cast(bf16x8, fb[b]), \
+        acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, ua), __builtin_bit_cast(bf16x8, ub), \
                                                             acc[a][b], 0, 0, 0);                                            \
       }                                                                                                                     \
     }                                                                                                                       \
   }
-    MX_STEP(0) MX_STEP(1) MX_STEP(2) MX_STEP(3)
+    // the order: after the first fragments a matrix instruction, a fragment of the next step, a direct load of the next tile, and so on;
+    // all direct loads in the first step, so that they have the other three to land
+    MX_STEP(0)
+    between();
+    MX_STEP(1) MX_STEP(2) MX_STEP(3)
+    __builtin_amdgcn_sched_group_barrier(0x100, TM + TN, 0);
+#pragma unroll
+    for (int i = 0; i < TM * TN; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      if (i < TM + TN) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x020, LOADS / (TM * TN), 0);
+    }
+#pragma unroll
+    for (int s = 1; s < 4; ++s)
+#pragma unroll
+      for (int i = 0; i < TM * TN; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        if (s < 3 && i < TM + TN) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      }
 #undef MX_STEP
   };
 
@@ -301,90 +359,106 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_kernel(const GemmArgs g) {
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
     take_scales();
-    if (++t == g.kt) t = 0, ++pair;
-    if (it + 1 < end) {
+    compute(lds + half, [&]() {
+      // behind the last tile the same one once more, into a buffer that nobody reads
+      t += it + 1 < end;
+      const int wrap = !FP4 && t == g.kt;  // 4-bit operands: one pair
+      t = wrap ? 0 : t;
+      pair += wrap;
       issue(pair, t, lds + ((BM + BN) * 128 - half));
       load_scales(t);
-    }
-    compute(lds + half);
+    });
     half = (BM + BN) * 128 - half;
   }
+  __builtin_amdgcn_s_waitcnt(0);  // no load is left on its way into LDS when the workgroup ends
 
-  // a lane's TN columns are neighbours: stored together where every row starts on a multiple of them
-  const int64_t ld = g.n, col = n0 + (wn * 32 + j) * TN;
-  const bool whole = g.n % TN == 0 && col < g.n;
-  auto store = [&](auto finish) {
+  // A lane's TN columns are neighbours: stored together where every row starts on a multiple of them.  Tiles that lie inside C are
+  // stored without comparisons.
+  const int64_t ld = g.n, col = n0 + (wn * 32 + j) * TN, row0 = m0 + (wm * 32 + 4 * h) * TM;
+  auto epilogue = [&](auto inside_) {
+    constexpr bool INSIDE = decltype(inside_)::value;
+    auto row_of = [&](int a, int r) { return row0 + ((r & 3) + 8 * (r >> 2)) * TM + a; };
+    auto write = [&](auto* p, const float (&v)[TN]) {  // p: (row, col) of the output
+      using U = typename std::remove_reference<decltype(*p)>::type;
+      if constexpr (INSIDE) {
+        struct alignas(sizeof(U) * TN) Vec { U e[TN]; } o;
 #pragma unroll
-    for (int a = 0; a < TM; ++a) {
-      // 256 sums stay where they are until a row of tiles is stored: the compiler would copy all of them first (the nops: a
-      // matrix result is read at the earliest 18 states after its instruction)
-      if constexpr (TM * TN == 16)
+        for (int b = 0; b < TN; ++b) o.e[b] = MxType<U>::from(v[b]);
+        *(Vec*)p = o;
+      } else {
 #pragma unroll
-        for (int b = 0; b < TN; ++b) asm volatile("s_nop 15\n\ts_nop 15" : "+a"(acc[a][b]));
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int64_t row = m0 + (wm * 32 + (r & 3) + 8 * (r >> 2) + 4 * h) * TM + a;
-        if (row >= g.m) continue;
-        finish(row, &acc[a], r);
+        for (int b = 0; b < TN; ++b)
+          if (col + b < g.n) p[b] = MxType<U>::from(v[b]);
       }
-    }
-  };
-  auto write = [&](auto* p, const float (&v)[TN]) {  // p: (row, col) of the output
-    using U = typename std::remove_reference<decltype(*p)>::type;
-    if (whole) {
-      struct alignas(sizeof(U) * TN) Vec { U e[TN]; } o;
+    };
+    auto each = [&](auto finish) {
 #pragma unroll
-      for (int b = 0; b < TN; ++b) o.e[b] = MxType<U>::from(v[b]);
-      *(Vec*)p = o;
-    } else {
+      for (int a = 0; a < TM; ++a)
 #pragma unroll
-      for (int b = 0; b < TN; ++b)
-        if (col + b < g.n) p[b] = MxType<U>::from(v[b]);
-    }
-  };
-  float v[TN];
-  if (g.partial) {
-    store([&](int64_t row, const f32x16(*c)[TN], int r) {
+        for (int r = 0; r < 16; ++r) {
+          const int64_t row = row_of(a, r);
+          if (!INSIDE && row >= g.m) continue;
+          float v[TN];
 #pragma unroll
-      for (int b = 0; b < TN; ++b) v[b] = (*c)[b][r];
-      write(g.partial + ((int64_t)split * g.m + row) * ld + col, v);
-    });
-  } else if (g.e.codes8) {
-    store([&](int64_t row, const f32x16(*c)[TN], int r) {
-      if (col >= g.n) return;
-      const uint32_t byte = g.e.scales8[row * g.e.nb8 + (col >> 5)];
-#pragma unroll
-      for (int b = 0; b < TN; ++b) {  // col is a multiple of TN: one block
-        const float x = mx_tanh(mx_value8((int)(int8_t)g.e.codes8[row * g.e.nb8 * 32 + col + b], byte));
-        v[b] = (*c)[b][r] * (1.f - x * x);
-      }
-      write((T*)g.e.out + row * ld + col, v);
-    });
-  } else {
-    float bias[TN] = {};
-    if (g.e.bias)
-#pragma unroll
-      for (int b = 0; b < TN; ++b)
-        if (col + b < g.n) bias[b] = MxType<T>::to(((const T*)g.e.bias)[col + b]);
-    if (g.e.tanh) {
-      store([&](int64_t row, const f32x16(*c)[TN], int r) {
-#pragma unroll
-        for (int b = 0; b < TN; ++b) v[b] = mx_tanh((*c)[b][r] + bias[b]);
-        write((T*)g.e.out + row * ld + col, v);
-        if (g.e.dact) {
-#pragma unroll
-          for (int b = 0; b < TN; ++b) v[b] = 1.f - v[b] * v[b];
-          write((_Float16*)g.e.dact + row * ld + col, v);
+          for (int b = 0; b < TN; ++b) v[b] = acc[a][b][r];
+          finish(row * ld + col, v);
         }
-      });
-    } else {
-      store([&](int64_t row, const f32x16(*c)[TN], int r) {
+    };
+    if (g.partial) {
+      float* const p = g.partial + (int64_t)split * g.m * ld;
+      each([&](int64_t at, float (&v)[TN]) { write(p + at, v); });
+    } else if (g.e.codes8) {
 #pragma unroll
-        for (int b = 0; b < TN; ++b) v[b] = (*c)[b][r] + bias[b];
-        write((T*)g.e.out + row * ld + col, v);
-      });
+      for (int a = 0; a < TM; ++a) {
+        // the checkpoint's values of 16 rows before any of them is used: one latency for all
+        uint32_t code[16], byte[16];
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int64_t row = INSIDE ? row_of(a, r) : min(row_of(a, r), (int64_t)g.m - 1);
+          const int64_t at = INSIDE || col < g.n ? col : 0;  // col is a multiple of TN: one block
+          code[r] = TN == 4 ? *(const uint32_t*)(g.e.codes8 + row * g.e.nb8 * 32 + at) : *(const uint16_t*)(g.e.codes8 + row * g.e.nb8 * 32 + at);
+          byte[r] = g.e.scales8[row * g.e.nb8 + (at >> 5)];
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          if (!INSIDE && (row_of(a, r) >= g.m || col >= g.n)) continue;
+          float v[TN];
+#pragma unroll
+          for (int b = 0; b < TN; ++b) {
+            const float x = mx_tanh(mx_value8((int)(int8_t)(code[r] >> 8 * b), byte[r]));
+            v[b] = acc[a][b][r] * (1.f - x * x);
+          }
+          write((T*)g.e.out + row_of(a, r) * ld + col, v);
+        }
+      }
+    } else {
+      float bias[TN] = {};
+      if (g.e.bias)
+#pragma unroll
+        for (int b = 0; b < TN; ++b)
+          if (INSIDE || col + b < g.n) bias[b] = MxType<T>::to(((const T*)g.e.bias)[col + b]);
+      if (g.e.tanh) {
+        each([&](int64_t at, float (&v)[TN]) {
+#pragma unroll
+          for (int b = 0; b < TN; ++b) v[b] = mx_tanh(v[b] + bias[b]);
+          write((T*)g.e.out + at, v);
+          if (g.e.dact) {
+#pragma unroll
+            for (int b = 0; b < TN; ++b) v[b] = 1.f - v[b] * v[b];
+            write((_Float16*)g.e.dact + at, v);
+          }
+        });
+      } else {
+        each([&](int64_t at, float (&v)[TN]) {
+#pragma unroll
+          for (int b = 0; b < TN; ++b) v[b] += bias[b];
+          write((T*)g.e.out + at, v);
+        });
+      }
     }
-  }
+  };
+  if (m0 + BM <= g.m && n0 + BN <= g.n && g.n % TN == 0) epilogue(std::true_type{});
+  else epilogue(std::false_type{});
 }
 
 // out = epi(sum over parts), in the parts' order
@@ -423,6 +497,28 @@ __global__ __launch_bounds__(256) void column_sums_kernel(S src, int64_t rows, i
     float v = 0.f;
     for (int i = 0; i < 32; ++i) v += lds[i][t];
     part[(int64_t)blockIdx.y * cols + c0 + t] = v;
+  }
+}
+
+// their totals: four columns, 64 groups of parts, in a fixed order
+template <class T>
+__global__ __launch_bounds__(256) void column_parts_kernel(const float* __restrict__ part, int count, int64_t cols, T* __restrict__ out) {
+  __shared__ float lds[64][4];
+  const int64_t col = (int64_t)blockIdx.x * 4 + (threadIdx.x & 3);
+  const int q = threadIdx.x >> 2;
+  float v = 0.f;
+  if (col < cols) {
+    const int s1 = count * (q + 1) / 64;
+#pragma unroll 4
+    for (int s = count * q / 64; s < s1; ++s) v += part[s * cols + col];
+  }
+  lds[q][threadIdx.x & 3] = v;
+  __syncthreads();
+  if (q == 0 && col < cols) {
+    v = 0.f;
+#pragma unroll
+    for (int i = 0; i < 64; ++i) v += lds[i][threadIdx.x];
+    out[col] = MxType<T>::from(v);
   }
 }
 
@@ -477,9 +573,24 @@ void mx_planes(const MxSource& q, int64_t rows, int64_t cols, bool transposed, v
 #undef MX_ARG
 }
 
+void mx_planes_keep(const MxSource& q, int64_t rows, int64_t cols, void* out, uint8_t* codes, uint8_t* scales, hipStream_t s) {
+  const int64_t pad = mx_up(cols, 64), nb = mx_blocks(cols);
+  const int grid = grid_for(rows * (pad >> 3));
+#define MX_TYPED(T, P)                                                                                                            \
+  do {                                                                                                                            \
+    const SrcDense<T, false> src{(const T*)q.p, cols, vec_ok(q.p, cols, sizeof(T))};                                              \
+    if (q.kind == MX_SRC_TANH) planes_keep_kernel<T, true, P><<<grid, 256, 0, s>>>(src, rows, pad, (uint16_t*)out, nb, codes, scales); \
+    else planes_keep_kernel<T, false, P><<<grid, 256, 0, s>>>(src, rows, pad, (uint16_t*)out, nb, codes, scales);                 \
+  } while (0)
+  if (q.dtype == FMD_F32) MX_TYPED(float, 3);
+  else if (q.dtype == FMD_F16) MX_TYPED(_Float16, 2);
+  else MX_TYPED(mx_bf16, 1);
+#undef MX_TYPED
+}
+
 void mx_scale_tiles(const void* scales, int64_t rows, int64_t nb, void* out, hipStream_t s) {
   const int64_t kt = (nb + 7) / 8;
-  scale_tiles_kernel<<<grid_for(rows * kt), 256, 0, s>>>((const uint8_t*)scales, rows, nb, kt, (uint64_t*)out);
+  scale_tiles_kernel<<<grid_for(rows * kt * 2), 256, 0, s>>>((const uint8_t*)scales, rows, mx_up(rows, 4), nb, kt, (uint32_t*)out);
 }
 
 // rows of a large matrix tile are worth it once they fill the chip; else the small tile, and the contraction in parts
@@ -492,7 +603,7 @@ MxProductPlan mx_product_plan(int64_t m, int64_t n, int64_t kt, int npairs) {
   int64_t s = p.tiles >= 192 ? 1 : 512 / p.tiles;
   if (s > its / 4) s = its / 4;
   if (s > 64) s = 64;
-  p.splits = (int)(s < 1 ? 1 : s);
+  p.splits = p.most = (int)(s < 1 ? 1 : s);
   return p;
 }
 
@@ -508,7 +619,7 @@ void mx_product(const MxOperand& a, const MxOperand& b, int64_t m, int64_t n, in
   GemmArgs g{};
   g.a = (const char*)a.p, g.b = (const char*)b.p;
   g.a_plane = a.plane, g.b_plane = b.plane, g.a_pitch = a.pitch, g.b_pitch = b.pitch;
-  g.sa = (const uint64_t*)a.scales, g.sb = (const uint64_t*)b.scales;
+  g.sa = (const char*)a.scales, g.sb = (const char*)b.scales;
   g.m = (int)m, g.n = (int)n, g.kt = (int)kt, g.granules = (int)(a.pitch / 16);
   const int side = plan.big ? 256 : 128;
   g.tiles_m = (int)((m + side - 1) / side), g.tiles_n = (int)((n + side - 1) / side), g.splits = plan.splits;
@@ -548,4 +659,11 @@ void mx_column_sums(const MxSource& q, int64_t rows, int64_t cols, int64_t parts
   else if (q.dtype == FMD_F16) MX_TYPED(_Float16);
   else MX_TYPED(mx_bf16);
 #undef MX_TYPED
+}
+
+void mx_column_totals(const float* parts, int64_t count, int64_t cols, int dtype, void* out, hipStream_t s) {
+  const unsigned grid = (unsigned)((cols + 3) / 4);
+  if (dtype == FMD_F32) column_parts_kernel<float><<<grid, 256, 0, s>>>(parts, (int)count, cols, (float*)out);
+  else if (dtype == FMD_F16) column_parts_kernel<_Float16><<<grid, 256, 0, s>>>(parts, (int)count, cols, (_Float16*)out);
+  else column_parts_kernel<mx_bf16><<<grid, 256, 0, s>>>(parts, (int)count, cols, (mx_bf16*)out);
 }

@@ -281,23 +281,11 @@ __global__ __launch_bounds__(256) void gradient_sum_kernel(const float* __restri
   }
 }
 
-template <class K>
-hipError_t allow_lds(K kernel, int bytes) {
-  static bool done[64] = {};
-  int dev = 0;
-  hipError_t e = hipGetDevice(&dev);
-  if (e != hipSuccess) return e;
-  if (dev >= 0 && dev < 64 && done[dev]) return hipSuccess;
-  e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (e == hipSuccess && dev >= 0 && dev < 64) done[dev] = true;
-  return e;
-}
-
 template <class T, bool TANH, int KT, int NT>
 int launch(const GradArgs& a, int slices, hipStream_t s) {
   constexpr int bytes = (KT * NT * 16 * 64 + 32 * NT) * 4;
   static_assert(bytes * PER_CU<T, KT> <= 160 * 1024, "LDS of a CU");
-  if (allow_lds(&gradient_kernel<T, TANH, KT, NT>, bytes) != hipSuccess) return FMD_ELAUNCH;
+  if (mx_allow_lds(&gradient_kernel<T, TANH, KT, NT>, bytes) != hipSuccess) return FMD_ELAUNCH;
   gradient_kernel<T, TANH, KT, NT><<<slices, 64 * WAVES, bytes, s>>>(a);
   return hipGetLastError() == hipSuccess ? FMD_OK : FMD_ELAUNCH;
 }

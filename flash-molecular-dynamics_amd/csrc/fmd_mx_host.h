@@ -21,23 +21,26 @@ struct MxOperand {  // K-contiguous rows
   const void* p;
   int64_t plane, pitch;  // bytes
   int planes;
-  const void* scales;  // 4-bit operand: [tile][row][8], else null
+  const void* scales;  // 4-bit operand: [tile of 8 blocks][half][row][4], else null
 };
 
 struct MxProductPlan {
   int64_t tiles;
-  int splits;
+  int splits, most;  // parts of the contraction; what a shorter one of the same shape has at most
   bool big;
 };
 
 // rows x cols (or its transposed) as bf16 planes [planes][rows][cols up to 64]
 void mx_planes(const MxSource& q, int64_t rows, int64_t cols, bool transposed, void* out, hipStream_t s);
+// p(x) (kind: MX_SRC_DENSE or _TANH) as planes, and x in 8-bit blocks, from one read
+void mx_planes_keep(const MxSource& q, int64_t rows, int64_t cols, void* out, uint8_t* codes, uint8_t* scales, hipStream_t s);
 void mx_scale_tiles(const void* scales, int64_t rows, int64_t nb, void* out, hipStream_t s);
 int mx_quantize4_for_product(const void* x, int dtype, int64_t m, int64_t k, void* codes, void* scales, hipStream_t s);
 MxProductPlan mx_product_plan(int64_t m, int64_t n, int64_t kt, int npairs);
 void mx_product(const MxOperand& a, const MxOperand& b, int64_t m, int64_t n, int64_t kt, const MxProductPlan& plan, int dtype,
                 const MxEpilogue& e, float* parts, hipStream_t s);
 void mx_sum_parts(const float* parts, int64_t count, int64_t m, int64_t n, int dtype, const MxEpilogue& e, hipStream_t s);
+void mx_column_totals(const float* parts, int64_t count, int64_t cols, int dtype, void* out, hipStream_t s);
 void mx_column_sums(const MxSource& q, int64_t rows, int64_t cols, int64_t parts, float* out, hipStream_t s);
 
 // a layer of at most 128 x 128 in one pass over the rows (fmd_mx_layer.hip)
@@ -68,6 +71,19 @@ int mx_gradient(const void* g, const uint8_t* codes, const uint8_t* scales, bool
 bool mx_rows_fits(int64_t m);
 int mx_rows(const void* x, int dtype, const void* codes, const void* scales, bool both, int64_t m, int64_t n, int64_t k,
             const MxEpilogue& e, hipStream_t s);
+
+// the dynamic-LDS ceiling of a kernel, raised once on each device
+template <class K>
+hipError_t mx_allow_lds(K kernel, int bytes) {
+  static bool done[64] = {};
+  int dev = 0;
+  hipError_t e = hipGetDevice(&dev);
+  if (e != hipSuccess) return e;
+  if (dev >= 0 && dev < 64 && done[dev]) return hipSuccess;
+  e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == hipSuccess && dev >= 0 && dev < 64) done[dev] = true;
+  return e;
+}
 
 static inline int mx_dtype_size(int dtype) { return dtype == FMD_F32 ? 4 : 2; }
 static inline int mx_dtype_planes(int dtype) { return dtype == FMD_F32 ? 3 : dtype == FMD_F16 ? 2 : 1; }

@@ -479,19 +479,6 @@ __global__ __launch_bounds__(256) void column_totals_kernel(const float* __restr
   }
 }
 
-// the dynamic-LDS ceiling of a kernel, raised once on each device
-template <class K>
-hipError_t allow_lds(K kernel, int bytes) {
-  static bool done[64] = {};
-  int dev = 0;
-  hipError_t e = hipGetDevice(&dev);
-  if (e != hipSuccess) return e;
-  if (dev >= 0 && dev < 64 && done[dev]) return hipSuccess;
-  e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (e == hipSuccess && dev >= 0 && dev < 64) done[dev] = true;
-  return e;
-}
-
 template <class T, int PRO, int WK, int EPI, int NT>
 int launch(const LayerArgs& a, hipStream_t s) {
   const int chunks = (a.c + 63) >> 6;
@@ -499,7 +486,7 @@ int launch(const LayerArgs& a, hipStream_t s) {
   const int bytes = WAVES * pass_bytes<T, PRO>() + wbytes;
   constexpr int most = WAVES * pass_bytes<T, PRO>() + (WK == W_FP4_BOTH ? 2 * NT * 64 * 20 : 8 * NT * 1024 * LayerPlanes<T, WK>::w);
   static_assert(most <= 160 * 1024, "LDS of a workgroup");
-  if (allow_lds(&layer_kernel<T, PRO, WK, EPI, NT>, most) != hipSuccess) return FMD_ELAUNCH;
+  if (mx_allow_lds(&layer_kernel<T, PRO, WK, EPI, NT>, most) != hipSuccess) return FMD_ELAUNCH;
   const int64_t tiles = (a.m + 31) / 32, full = 256 * (bytes <= 80 * 1024 ? 2 : 1);
   const int grid = (int)(tiles < full ? tiles : full);
   layer_kernel<T, PRO, WK, EPI, NT><<<dim3(grid, (a.o + 32 * NT - 1) / (32 * NT)), 64 * WAVES, bytes, s>>>(a);

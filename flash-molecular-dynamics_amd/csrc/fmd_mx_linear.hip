@@ -23,9 +23,10 @@ MxEpilogue rows_of(const MxEpilogue& e, int64_t r0, int64_t n, int dtype) {
   return o;
 }
 
-// out[m,n] = epi(A B^T), A = q [m,k] as planes, B already laid out; run = false only counts the workspace
+// out[m,n] = epi(A B^T), A = q [m,k] as planes, B already laid out; codes, scales: where q's 8-bit blocks go, or null; run = false
+// only counts the workspace
 void product_of_rows(MxArena& ar, bool run, MxSource q, int64_t m, int64_t k, const MxOperand& b, int64_t n, int dtype,
-                     const MxEpilogue& e, hipStream_t s) {
+                     const MxEpilogue& e, hipStream_t s, uint8_t* codes = nullptr, uint8_t* scales = nullptr) {
   const int pa = mx_dtype_planes(dtype);
   const int64_t pad = mx_up(k, 64), kt = pad / 64, rows = chunk_rows(m, pa * pad * 2);
   const MxProductPlan plan = mx_product_plan(rows, n, kt, mx_pairs(pa, b.planes).n);
@@ -37,7 +38,8 @@ void product_of_rows(MxArena& ar, bool run, MxSource q, int64_t m, int64_t k, co
     const int64_t c = m - r0 < rows ? m - r0 : rows;
     MxSource part = q;
     part.p = at(q.p, r0 * k, size), part.aux = at(q.aux, r0 * k, aux);
-    mx_planes(part, c, k, false, planes, s);
+    if (codes) mx_planes_keep(part, c, k, planes, codes + r0 * mx_blocks(k) * 32, scales + r0 * mx_blocks(k), s);
+    else mx_planes(part, c, k, false, planes, s);
     const MxOperand a{planes, c * pad * 2, pad * 2, pa, nullptr};
     const MxEpilogue ep = rows_of(e, r0, n, dtype);
     mx_product(a, b, c, n, kt, plan, dtype, ep, parts, s);
@@ -54,7 +56,8 @@ void product_over_rows(MxArena& ar, bool run, MxSource qa, int pa, int64_t k, Mx
   const MxProductPlan plan = mx_product_plan(k, n, pad / 64, mx_pairs(pa, pb).n);
   void* ta = ar.take(pa * k * pad * 2);
   void* tb = ar.take(pb * n * pad * 2);
-  float* parts = chunks * plan.splits > 1 ? (float*)ar.take(chunks * plan.splits * k * n * 4) : nullptr;
+  float* parts = chunks * plan.splits > 1 ? (float*)ar.take(chunks * plan.most * k * n * 4) : nullptr;
+  int64_t count = 0;  // the last chunk is shorter and may have fewer parts
   if (!run) return;
   const int64_t nb = mx_blocks(k);
   const MxEpilogue e{nullptr, out, nullptr, nullptr, nullptr, 0, 0};
@@ -65,10 +68,12 @@ void product_over_rows(MxArena& ar, bool run, MxSource qa, int pa, int64_t k, Mx
     b.p = at(qb.p, r0 * n, mx_dtype_size(qb.dtype));
     mx_planes(a, c, k, true, ta, s);
     mx_planes(b, c, n, true, tb, s);
-    mx_product({ta, k * cpad * 2, cpad * 2, pa, nullptr}, {tb, n * cpad * 2, cpad * 2, pb, nullptr}, k, n, cpad / 64, plan, dtype, e,
-               parts ? parts + i * plan.splits * k * n : nullptr, s);
+    const MxProductPlan here = c == rows ? plan : mx_product_plan(k, n, cpad / 64, mx_pairs(pa, pb).n);
+    mx_product({ta, k * cpad * 2, cpad * 2, pa, nullptr}, {tb, n * cpad * 2, cpad * 2, pb, nullptr}, k, n, cpad / 64, here, dtype, e,
+               parts ? parts + count * k * n : nullptr, s);
+    count += here.splits;
   }
-  if (parts) mx_sum_parts(parts, chunks * plan.splits, k, n, dtype, e, s);
+  if (parts) mx_sum_parts(parts, count, k, n, dtype, e, s);
 }
 
 void sum_over_rows(MxArena& ar, bool run, const MxSource& q, int64_t m, int64_t n, int dtype, void* out, hipStream_t s) {
@@ -79,7 +84,7 @@ void sum_over_rows(MxArena& ar, bool run, const MxSource& q, int64_t m, int64_t 
   float* p = (float*)ar.take(parts * n * 4);
   if (!run) return;
   mx_column_sums(q, m, n, parts, p, s);
-  mx_sum_parts(p, parts, 1, n, dtype, MxEpilogue{nullptr, out, nullptr, nullptr, nullptr, 0, 0}, s);
+  mx_column_totals(p, parts, n, dtype, out, s);
 }
 
 // ---- y = f(x^ W^T + b), W in 4-bit blocks -----------------------------------------------------------------------------
@@ -108,8 +113,8 @@ int64_t fp4_forward(const Fp4Linear& c, void* base, bool run, hipStream_t s) {
     const int64_t kt = (nb + 7) / 8;
     const MxProductPlan plan = mx_product_plan(c.m, c.n, kt, 1);
     void* xc = ar.take(c.m * nb * 16);
-    void* xs = ar.take(c.m * kt * 8);
-    void* ws = ar.take(c.n * kt * 8);
+    void* xs = ar.take(mx_up(c.m, 4) * kt * 8);
+    void* ws = ar.take(mx_up(c.n, 4) * kt * 8);
     float* parts = plan.splits > 1 ? (float*)ar.take(plan.splits * c.m * c.n * 4) : nullptr;
     if (run) {
       mx_quantize4_for_product(c.x, c.dtype, c.m, c.k, xc, xs, s);
@@ -176,12 +181,9 @@ int64_t kept_forward(const Kept& c, void* base, bool run, hipStream_t s) {
   const int p = mx_dtype_planes(c.dtype);
   const int64_t pad = mx_up(c.k, 64);
   void* w = ar.take(p * c.n * pad * 2);
-  if (run) {
-    mx_planes({MX_SRC_DENSE, c.dtype, c.w, nullptr}, c.k, c.n, true, w, s);
-    if (c.codes) fmd_mxint8_quantize(c.x, c.dtype, c.m, c.k, c.codes, c.scales, s);
-  }
+  if (run) mx_planes({MX_SRC_DENSE, c.dtype, c.w, nullptr}, c.k, c.n, true, w, s);
   product_of_rows(ar, run, {c.tanh ? MX_SRC_TANH : MX_SRC_DENSE, c.dtype, c.x, nullptr}, c.m, c.k,
-                  {w, c.n * pad * 2, pad * 2, p, nullptr}, c.n, c.dtype, c.e, s);
+                  {w, c.n * pad * 2, pad * 2, p, nullptr}, c.n, c.dtype, c.e, s, c.codes, c.scales);
   return ar.used;
 }
 

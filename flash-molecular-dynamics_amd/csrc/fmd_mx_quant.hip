@@ -27,13 +27,13 @@ __device__ __forceinline__ void load8(const T* __restrict__ row, int64_t c0, int
 
 struct QuantArgs {
   int64_t m, k, nb;
-  int vec, lay8;
+  int vec, for_product;
   uint32_t* codes;
   uint8_t* scales;
 };
 
-// lay8: where the scale byte of (row, block) goes.  0: [row][blocks].  1: [block/8][row][8], the order in which the product
-// kernel reads them.  The four lanes of a block are always active together
+// for_product: where the scale byte of (row, block) goes.  0: [row][blocks].  1: [block/8][block&1][row][4] with
+// the rows rounded up to 4, as the product kernel reads them.  The four lanes of a block are always active together
 template <int BITS>
 __device__ __forceinline__ void quantize8(const QuantArgs& a, int64_t row, int64_t q, const float (&v)[8]) {
   const int64_t t = row * a.nb * 4 + q;
@@ -51,10 +51,15 @@ __device__ __forceinline__ void quantize8(const QuantArgs& a, int64_t row, int64
   }
   if ((q & 3) == 0) {
     const int64_t b = q >> 2;
-    uint8_t* to = a.scales + (a.lay8 ? ((b >> 3) * a.m + row) * 8 + (b & 7) : row * a.nb + b);
-    *to = (uint8_t)byte;
-    if (a.lay8 && b == a.nb - 1)
-      for (int i = 1; i < 8 - (int)(b & 7); ++i) to[i] = 0;
+    if (a.for_product) {
+      const int64_t pad = (a.m + 3) & ~(int64_t)3;
+      auto at = [&](int64_t i) { return a.scales + (((i >> 3) * 2 + (i & 1)) * pad + row) * 4 + (i >> 1 & 3); };
+      *at(b) = (uint8_t)byte;
+      if (b == a.nb - 1)
+        for (int64_t i = b + 1; i & 7; ++i) *at(i) = 0;
+    } else {
+      a.scales[row * a.nb + b] = (uint8_t)byte;
+    }
   }
 }
 
@@ -189,11 +194,11 @@ void run_dequantize(QuantArgs a, T* out, hipStream_t s) {
 }
 
 template <int BITS>
-int quantize(const void* x, int dtype, int64_t m, int64_t k, void* codes, void* scales, int lay8, hipStream_t s) {
+int quantize(const void* x, int dtype, int64_t m, int64_t k, void* codes, void* scales, int for_product, hipStream_t s) {
   if (m < 0 || k < 1 || dtype < 0 || dtype > 2) return FMD_EINVAL;
   if (m == 0) return FMD_OK;
   if (!x || !codes || !scales || ((uintptr_t)x & 15) || ((uintptr_t)codes & 15)) return FMD_EINVAL;
-  const QuantArgs a{m, k, mx_blocks(k), 0, lay8, (uint32_t*)codes, (uint8_t*)scales};
+  const QuantArgs a{m, k, mx_blocks(k), 0, for_product, (uint32_t*)codes, (uint8_t*)scales};
   if (dtype == FMD_F32) run_quantize<float, BITS>((const float*)x, a, s);
   else if (dtype == FMD_F16) run_quantize<_Float16, BITS>((const _Float16*)x, a, s);
   else run_quantize<mx_bf16, BITS>((const mx_bf16*)x, a, s);
