@@ -312,9 +312,12 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_kernel(const GemmArgs g) {
       for (int b = 0; b < TN; ++b) fb[s & 1][b] = *(const u32x4*)(lb + (b >> 1) * 256 + (b & 1 ? odd : at));
     };
     read(0);
-#define MX_STEP(s)                                                                                                          \
+    // the compiler keeps this order: the next step's fragments on their way before a step's matrix instructions, no two of which in a
+    // row add to the same sums; the next tile's loads amid the first step
+#define MX_STEP(s, BETWEEN)                                                                                                 \
   {                                                                                                                         \
     if (s < 3) read(s + 1);                                                                                                 \
+    __builtin_amdgcn_sched_barrier(0);                                                                                      \
     _Pragma("unroll") for (int a = 0; a < TM; ++a) _Pragma("unroll") for (int b = 0; b < TN; ++b) {                         \
       const u32x4 ua = fa[s & 1][a], ub = fb[s & 1][b];                                                                     \
       if constexpr (FP4) {                                                                                                  \
@@ -325,27 +328,16 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_kernel(const GemmArgs g) {
         acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, ua), __builtin_bit_cast(bf16x8, ub), \
                                                             acc[a][b], 0, 0, 0);                                            \
       }                                                                                                                     \
+      if (a == TM / 2 - 1 && b == TN - 1) {                                                                                 \
+        __builtin_amdgcn_sched_barrier(0);                                                                                  \
+        BETWEEN;                                                                                                            \
+        __builtin_amdgcn_sched_barrier(0);                                                                                  \
+      }                                                                                                                     \
     }                                                                                                                       \
+    __builtin_amdgcn_sched_barrier(0);                                                                                      \
   }
-    // the order: after the first fragments a matrix instruction, a fragment of the next step, a direct load of the next tile, and so on;
-    // all direct loads in the first step, so that they have the other three to land
-    MX_STEP(0)
-    between();
-    MX_STEP(1) MX_STEP(2) MX_STEP(3)
-    __builtin_amdgcn_sched_group_barrier(0x100, TM + TN, 0);
-#pragma unroll
-    for (int i = 0; i < TM * TN; ++i) {
-      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-      if (i < TM + TN) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-      __builtin_amdgcn_sched_group_barrier(0x020, LOADS / (TM * TN), 0);
-    }
-#pragma unroll
-    for (int s = 1; s < 4; ++s)
-#pragma unroll
-      for (int i = 0; i < TM * TN; ++i) {
-        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-        if (s < 3 && i < TM + TN) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-      }
+    MX_STEP(0, between())
+    MX_STEP(1, ) MX_STEP(2, ) MX_STEP(3, )
 #undef MX_STEP
   };
 
