@@ -1,6 +1,6 @@
 // Weight and bias gradients: gw[k,n] = sum over rows p(x8)[.,k] g[.,n], gb[n] = sum g[.,n], x8 in 8-bit blocks.
 //
-// gradient_kernel, for narrow layers (k and n at most 128) over many rows.  The contraction runs over the rows, so a matrix fragment wants 8 rows of one column in a lane.  Lane i of a half wave takes
+// gradient_kernel, for narrow layers (k and n at most 256, in parts of 128 x 128) over many rows.  The contraction runs over the rows, so a matrix fragment wants 8 rows of one column in a lane.  Lane i of a half wave takes
 // columns NT*i .. NT*i+NT-1 of g (one 16-byte load a row) and KT*i .. of the checkpoint; over 8 rows that is one fragment for each
 // of its columns, with no transposition through LDS: which matrix column a lane stands for is free, and the result is stored
 // back in the same order.  A wave holds all of gw in its accumulators (up to 128 x 128: 256 of a lane's 512 registers, one wave a
@@ -25,7 +25,8 @@ struct GradArgs {
   const uint8_t *codes, *scales;
   float* part;  // [slice][32 KT + 1][32 NT]; the last row: bias
   int64_t m;
-  int k, n, nb, vec;
+  int k, n, nb, vec;  // of gw's part that a launch makes (nb: of all columns)
+  int ld, n0, block0;  // columns of g; the part's first column and block of the checkpoint
 };
 
 __device__ __forceinline__ Rows rows_of(const void* p, int64_t row0, int64_t m, int row_bytes) {
@@ -48,14 +49,15 @@ __global__ __launch_bounds__(64 * WAVES, (PER_CU<T, KT>)) void gradient_kernel(c
 
   uint32_t g_raw[8][W], s_raw[8];
   uint32_t c_raw[8];
-  const bool kept = a.codes && k0 < a.nb * 32;  // the bias's gradient alone needs no checkpoint
-  const uint32_t c_off = kept ? (uint32_t)(8 * h * a.nb * 32 + k0) : NOWHERE;
-  const uint32_t s_off = kept ? (uint32_t)(8 * h * a.nb + (k0 >> 5)) : NOWHERE;
+  const int block = a.block0 + (k0 >> 5);
+  const bool kept = a.codes && k0 < a.k && block < a.nb;  // the bias's gradient alone needs no checkpoint
+  const uint32_t c_off = kept ? (uint32_t)((8 * h * a.nb + a.block0) * 32 + k0) : NOWHERE;
+  const uint32_t s_off = kept ? (uint32_t)(8 * h * a.nb + block) : NOWHERE;
   auto fetch = [&](int step) {
     const int64_t row0 = (int64_t)step * 16;
-    const Rows g = rows_of(a.g, row0, a.m, a.n * S), c = rows_of(a.codes, row0, a.m, a.nb * 32), s = rows_of(a.scales, row0, a.m, a.nb);
-    const int gs = mx_here(a.n * S), nbs = mx_here(a.nb);
-    const uint32_t at = (uint32_t)(8 * h * a.n + n0) * S;
+    const Rows g = rows_of(a.g, row0, a.m, a.ld * S), c = rows_of(a.codes, row0, a.m, a.nb * 32), s = rows_of(a.scales, row0, a.m, a.nb);
+    const int gs = mx_here(a.ld * S), nbs = mx_here(a.nb);
+    const uint32_t at = (uint32_t)(8 * h * a.ld + a.n0 + n0) * S;
     if (a.vec) {
       const uint32_t off = n0 < a.n ? at : NOWHERE;
 #pragma unroll
@@ -256,7 +258,7 @@ __global__ __launch_bounds__(64 * TILE_WAVES) void gradient_tile_kernel(const Gr
 
 // gw and gb from the slices: 16 outputs a workgroup, 16 groups of slices each, added in a fixed order
 template <class T>
-__global__ __launch_bounds__(256) void gradient_sum_kernel(const float* __restrict__ part, int slices, int rows, int pitch, int k, int n,
+__global__ __launch_bounds__(256) void gradient_sum_kernel(const float* __restrict__ part, int slices, int rows, int pitch, int k, int n, int ld,
                                                            T* __restrict__ gw, T* __restrict__ gb) {
   __shared__ float lds[16][17];
   const int at = blockIdx.x * 16 + (threadIdx.x & 15), q = threadIdx.x >> 4;
@@ -276,7 +278,7 @@ __global__ __launch_bounds__(256) void gradient_sum_kernel(const float* __restri
     v = 0.f;
 #pragma unroll
     for (int i = 0; i < 16; ++i) v += lds[i][threadIdx.x];
-    if (row < k) gw[(int64_t)row * n + col] = MxType<T>::from(v);
+    if (row < k) gw[(int64_t)row * ld + col] = MxType<T>::from(v);
     else gb[col] = MxType<T>::from(v);
   }
 }
@@ -296,25 +298,34 @@ int by_width(const GradArgs& a, int slices, hipStream_t s) {
   return a.n <= 64 ? launch<T, TANH, 4, 2>(a, slices, s) : launch<T, TANH, 4, 4>(a, slices, s);
 }
 
+// part by part of at most 128 x 128, one after the other in the same workspace
 template <class T>
 int run(GradArgs a, bool tanh, int slices, void* gw, void* gb, hipStream_t s) {
-  const int nt = a.n <= 64 ? 2 : 4, rows = a.k <= 64 ? 64 : 128;
-  a.vec = ((uintptr_t)a.g & 15) == 0 && a.n % nt == 0;
-  const int rc = tanh ? by_width<T, true>(a, slices, s) : by_width<T, false>(a, slices, s);
-  if (rc != FMD_OK) return rc;
-  gradient_sum_kernel<T><<<((a.k + 1) * a.n + 15) / 16, 256, 0, s>>>(a.part, slices, rows, 32 * nt, a.k, a.n, (T*)gw, (T*)gb);
-  return hipGetLastError() == hipSuccess ? FMD_OK : FMD_ELAUNCH;
+  const int k = a.k, n = a.n;
+  for (int k0 = 0; k0 < k; k0 += 128)
+    for (int n0 = 0; n0 < n; n0 += 128) {
+      a.k = k - k0 < 128 ? k - k0 : 128, a.n = n - n0 < 128 ? n - n0 : 128, a.n0 = n0, a.block0 = k0 / 32;
+      const int nt = a.n <= 64 ? 2 : 4, rows = a.k <= 64 ? 64 : 128;
+      a.vec = ((uintptr_t)a.g & 15) == 0 && a.n % nt == 0 && n % nt == 0;
+      const int rc = tanh ? by_width<T, true>(a, slices, s) : by_width<T, false>(a, slices, s);
+      if (rc != FMD_OK) return rc;
+      gradient_sum_kernel<T><<<((a.k + 1) * a.n + 15) / 16, 256, 0, s>>>(a.part, slices, rows, 32 * nt, a.k, a.n, n,
+                                                                         gw ? (T*)gw + (int64_t)k0 * n + n0 : nullptr,
+                                                                         gb && k0 == 0 ? (T*)gb + n0 : nullptr);
+      if (hipGetLastError() != hipSuccess) return FMD_ELAUNCH;
+    }
+  return FMD_OK;
 }
 
 // workgroups along the rows: one step of 16 rows for each wave at least, what fits the chip at once at most
 int slices_for(int dtype, int64_t m, int64_t k) {
-  const int64_t s = (m + 16 * WAVES - 1) / (16 * WAVES), most = k <= 64 && dtype != FMD_F32 ? 512 : 256;
+  const int64_t s = (m + 16 * WAVES - 1) / (16 * WAVES), most = k <= 64 && dtype != FMD_F32 ? 512 : 256;  // of the first part, the largest
   return (int)(s < most ? s : most);
 }
 
 // Which kernel: a tile at a time while the rows are few.  (Both measured at 128 x 128, fp32, tanh: see FEW.)
 constexpr int64_t FEW = 65536, FEW_WIDE = 256;
-bool by_tiles(int64_t m, int64_t n, int64_t k) { return m <= (k <= 128 && n <= 128 ? FEW : FEW_WIDE); }
+bool by_tiles(int64_t m, int64_t n, int64_t k) { return m <= (k <= 256 && n <= 256 ? FEW : FEW_WIDE); }
 int tile_slices(int64_t m, int64_t n, int64_t k) {
   const int64_t tiles = ((k + 31) / 32) * ((n + 31) / 32), s = (m + 32 * TILE_WAVES - 1) / (32 * TILE_WAVES), most = (512 + tiles - 1) / tiles;
   return (int)(m <= 1024 ? 1 : s < most ? s : most);  // two steps for each wave at least
@@ -327,13 +338,13 @@ int run_tiles(GradArgs a, bool tanh, void* gw, void* gb, hipStream_t s) {
   const dim3 grid((a.k + 31) / 32, (a.n + 31) / 32, slices);
   if (tanh) gradient_tile_kernel<T, true><<<grid, 64 * TILE_WAVES, 0, s>>>(a, (T*)gw, (T*)gb);
   else gradient_tile_kernel<T, false><<<grid, 64 * TILE_WAVES, 0, s>>>(a, (T*)gw, (T*)gb);
-  if (slices > 1) gradient_sum_kernel<T><<<((a.k + 1) * a.n + 15) / 16, 256, 0, s>>>(a.part, slices, a.k, a.n, a.k, a.n, (T*)gw, (T*)gb);
+  if (slices > 1) gradient_sum_kernel<T><<<((a.k + 1) * a.n + 15) / 16, 256, 0, s>>>(a.part, slices, a.k, a.n, a.k, a.n, a.n, (T*)gw, (T*)gb);
   return hipGetLastError() == hipSuccess ? FMD_OK : FMD_ELAUNCH;
 }
 
 }  // namespace
 
-bool mx_gradient_fits(int64_t m, int64_t n, int64_t k) { return (k <= 128 && n <= 128) || by_tiles(m, n, k); }
+bool mx_gradient_fits(int64_t m, int64_t n, int64_t k) { return (k <= 256 && n <= 256) || by_tiles(m, n, k); }
 
 int64_t mx_gradient_bytes(int dtype, int64_t m, int64_t n, int64_t k) {
   if (by_tiles(m, n, k)) return tile_slices(m, n, k) > 1 ? (int64_t)tile_slices(m, n, k) * (k + 1) * n * 4 : 0;
@@ -342,7 +353,7 @@ int64_t mx_gradient_bytes(int dtype, int64_t m, int64_t n, int64_t k) {
 
 int mx_gradient(const void* g, const uint8_t* codes, const uint8_t* scales, bool tanh, int dtype, int64_t m, int64_t n, int64_t k,
                 void* gw, void* gb, void* workspace, hipStream_t s) {
-  const GradArgs a{g, codes, scales, (float*)workspace, m, (int)k, (int)n, (int)mx_blocks(k), 0};
+  const GradArgs a{g, codes, scales, (float*)workspace, m, (int)k, (int)n, (int)mx_blocks(k), 0, (int)n, 0, 0};
   if (by_tiles(m, n, k)) {
     if (dtype == FMD_F32) return run_tiles<float>(a, tanh, gw, gb, s);
     if (dtype == FMD_F16) return run_tiles<_Float16>(a, tanh, gw, gb, s);

@@ -1,4 +1,4 @@
-// Narrow layers over many rows: out[m,o] = epi(pro(in)[m,c] V[c,o] (+ bias)), c and o at most 128.  One pass over the rows.
+// Narrow layers over many rows: out[m,o] = epi(pro(in)[m,c] V[c,o] (+ bias)), c and o at most 256.  One pass over the rows.
 //
 // These layers are bound by memory (a row of 128 + 128 fp32 is 1 KB against 32 K multiply-adds), so everything a row needs
 // happens between its one read and its one write: the activation or the gradient's factor, the cut into planes, the 4- or
@@ -282,7 +282,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void layer_kernel(const LayerArgs a)
   __syncthreads();
 
   f32x16 acc[NT];
-  float sums[2] = {};  // columns lane and 64 + lane
+  float sums[4] = {};  // columns lane, 64 + lane, ..
   while (tile < tiles) {
     const int64_t row0 = (int64_t)tile * 32;
     if (ch == 0)
@@ -301,8 +301,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void layer_kernel(const LayerArgs a)
       }
       if (WK == W_FP4_ACROSS && a.sums) {
         const float v = Pass<typename std::conditional<AUX, float, T>::type>::column(own, lane);
-        sums[0] += ch ? 0.f : v;
-        sums[1] += ch ? v : 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sums[i] += i == ch ? v : 0.f;
       }
       const int next_tile = ch + 1 < chunks ? tile : tile + stride, next_ch = ch + 1 < chunks ? ch + 1 : 0;
       if (next_tile < tiles) fetch(next_tile, next_ch);
@@ -445,13 +445,13 @@ __global__ __launch_bounds__(64 * WAVES, 2) void layer_kernel(const LayerArgs a)
     if (a.sums && blockIdx.y == 0) {  // the waves' sums, in order
       __syncthreads();
       float* all = (float*)lds;
-      all[wave * 128 + lane] = sums[0];
-      all[wave * 128 + 64 + lane] = sums[1];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) all[wave * 256 + 64 * i + lane] = sums[i];
       __syncthreads();
       if ((int)threadIdx.x < a.c) {
         float v = 0.f;
 #pragma unroll
-        for (int w = 0; w < WAVES; ++w) v += all[w * 128 + threadIdx.x];
+        for (int w = 0; w < WAVES; ++w) v += all[w * 256 + threadIdx.x];
         a.sums[(int64_t)blockIdx.x * a.c + threadIdx.x] = v;
       }
     }
@@ -467,7 +467,7 @@ __global__ __launch_bounds__(256) void column_totals_kernel(const float* __restr
   if (col < c) {
     const int s1 = count * (q + 1) / 64;
 #pragma unroll 8
-    for (int s = count * q / 64; s < s1; ++s) v += sums[s * c + col];  // at most 512 x 128
+    for (int s = count * q / 64; s < s1; ++s) v += sums[s * c + col];  // at most 512 x 256
   }
   lds[q][threadIdx.x & 3] = v;
   __syncthreads();
@@ -479,15 +479,19 @@ __global__ __launch_bounds__(256) void column_totals_kernel(const float* __restr
   }
 }
 
+template <class T, int PRO, int WK, int NT>
+int lds_bytes(int c) {
+  const int chunks = (c + 63) >> 6;
+  return WAVES * pass_bytes<T, PRO>() + (WK == W_FP4_BOTH ? chunks * NT * 64 * 20 : chunks * 4 * NT * 1024 * LayerPlanes<T, WK>::w);
+}
+constexpr int LDS = 160 * 1024;
+
 template <class T, int PRO, int WK, int EPI, int NT>
 int launch(const LayerArgs& a, hipStream_t s) {
-  const int chunks = (a.c + 63) >> 6;
-  const int wbytes = WK == W_FP4_BOTH ? chunks * NT * 64 * 20 : chunks * 4 * NT * 1024 * LayerPlanes<T, WK>::w;
-  const int bytes = WAVES * pass_bytes<T, PRO>() + wbytes;
-  constexpr int most = WAVES * pass_bytes<T, PRO>() + (WK == W_FP4_BOTH ? 2 * NT * 64 * 20 : 8 * NT * 1024 * LayerPlanes<T, WK>::w);
-  static_assert(most <= 160 * 1024, "LDS of a workgroup");
-  if (mx_allow_lds(&layer_kernel<T, PRO, WK, EPI, NT>, most) != hipSuccess) return FMD_ELAUNCH;
-  const int64_t tiles = (a.m + 31) / 32, full = 256 * (bytes <= 80 * 1024 ? 2 : 1);
+  const int bytes = lds_bytes<T, PRO, WK, NT>(a.c);
+  if (bytes > LDS) return FMD_EINVAL;
+  if (mx_allow_lds(&layer_kernel<T, PRO, WK, EPI, NT>, LDS) != hipSuccess) return FMD_ELAUNCH;
+  const int64_t tiles = (a.m + 31) / 32, full = 256 * (bytes <= LDS / 2 ? 2 : 1);
   const int grid = (int)(tiles < full ? tiles : full);
   layer_kernel<T, PRO, WK, EPI, NT><<<dim3(grid, (a.o + 32 * NT - 1) / (32 * NT)), 64 * WAVES, bytes, s>>>(a);
   if (WK == W_FP4_ACROSS && a.sums) column_totals_kernel<T><<<(a.c + 3) / 4, 256, 0, s>>>(a.sums, grid, a.c, (T*)a.totals);
@@ -499,7 +503,8 @@ int by_width(const LayerArgs& a, hipStream_t s) {
   // A tile of rows is 10 us from one end to the other: up to 64 of them, every 32 outputs get workgroups of their own (269 rows,
   // 128 x 128, fp32: 11.1 us against 18.2); from there on the rows fill the chip (34432 rows: 43 against 25)
   if ((a.m + 31) / 32 <= 64) return launch<T, PRO, WK, EPI, 1>(a, s);
-  return a.o <= 64 ? launch<T, PRO, WK, EPI, 2>(a, s) : launch<T, PRO, WK, EPI, 4>(a, s);
+  // 128 outputs a workgroup, which read the rows once for each 128, where their weight fits LDS (fp32 beyond 128 columns: 64)
+  return a.o <= 64 || lds_bytes<T, PRO, WK, 4>(a.c) > LDS ? launch<T, PRO, WK, EPI, 2>(a, s) : launch<T, PRO, WK, EPI, 4>(a, s);
 }
 
 template <class T>
@@ -522,7 +527,7 @@ int by_kind(LayerArgs a, const MxLayer& l, hipStream_t s) {
 }  // namespace
 
 int64_t mx_layer_sums_bytes(int64_t m, int64_t c) { return (m < 512 * 32 ? (m + 31) / 32 : 512) * c * 4; }
-bool mx_layer_fits(int64_t c, int64_t o) { return c <= 128 && o <= 128; }
+bool mx_layer_fits(int64_t c, int64_t o) { return c <= 256 && o <= 256; }
 
 int mx_layer(const MxLayer& l, int dtype, int64_t m, int64_t c, int64_t o, hipStream_t s) {
   LayerArgs a{};

@@ -94,8 +94,8 @@ def test_workspaces_do_not_grow_with_the_rows():
     from flashmd_amd import _ffi
 
     lib = _ffi.lib()
-    one = lib.fmd_linear_ckpt8_workspace_bytes(0, 1 << 20, 256, 256)
-    assert 0 < one < 1 << 29 and lib.fmd_linear_ckpt8_workspace_bytes(0, 1 << 26, 256, 256) <= one + (1 << 20)
+    one = lib.fmd_linear_ckpt8_workspace_bytes(0, 1 << 20, 300, 300)
+    assert 0 < one < 1 << 29 and lib.fmd_linear_ckpt8_workspace_bytes(0, 1 << 26, 300, 300) <= one + (1 << 20)
 
 
 def _model(activation=None):

@@ -100,7 +100,7 @@ def test_quantize_empty_and_views(K):
 
 # ---------------------------------------------------------------------------------------- 4-bit layers
 LAYERS = [(1, 1, 1), (1, 50, 128), (2, 33, 7), (3, 128, 64), (17, 64, 1), (32, 300, 130), (33, 31, 128), (64, 128, 128), (100, 129, 33),
-          (269, 50, 128), (269, 128, 64), (300, 256, 257), (1000, 128, 128), (65, 1000, 300)]
+          (269, 50, 128), (269, 128, 64), (300, 256, 257), (1000, 128, 128), (65, 1000, 300), (2100, 200, 256), (2200, 256, 129)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -160,7 +160,7 @@ def test_mxfp4_linear_non_finite(K):
 # ---------------------------------------------------------------------------------------- 8-bit checkpoints
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("tanh", [False, True])
-@pytest.mark.parametrize("m,k,n", LAYERS + [(2000, 130, 140), (5000, 50, 128)])
+@pytest.mark.parametrize("m,k,n", LAYERS + [(2000, 130, 140), (5000, 50, 128), (2100, 256, 200), (2500, 170, 256)])
 def test_linear_ckpt8(K, m, k, n, tanh, dtype):
     x = uneven(m, k, dtype, seed=m + k)
     w = rand(k, n, seed=n, scale=(2.0 / (k + n)) ** 0.5, dtype=dtype)
@@ -281,7 +281,7 @@ def test_rows_behind_the_last_are_left_alone(K):
     from flashmd_amd._ffi import call, ptr, stream
 
     lib = _ffi.lib()
-    for m, k, n in ((1, 50, 33), (33, 128, 128), (37, 64, 20), (45, 40, 64), (20, 300, 70), (100, 300, 131), (300, 130, 64)):
+    for m, k, n in ((1, 50, 33), (33, 128, 128), (37, 64, 20), (45, 40, 64), (20, 300, 70), (100, 300, 131), (300, 130, 64), (70, 200, 250), (3001, 257, 70)):
         x, w, g = rand(m, k, seed=1).to(DEV), rand(k, n, seed=2).to(DEV), rand(m, n, seed=3).to(DEV)
         nb, nbn = (k + 31) // 32, (n + 31) // 32
         wc, wsc = K.mxfp4_quantize(w.t().contiguous())
@@ -407,7 +407,7 @@ def test_offsets_beyond_32_bits(K):
     near(K.mxfp4_linear(x.detach(), wc.to(DEV), wsc.to(DEV))[-70:], mo.linear(tail, wv), k)
 
 
-@pytest.mark.parametrize("m,k,n", [(70000, 128, 128), (70001, 50, 128), (66000, 100, 30), (300_000, 130, 40), (70016, 64, 64)])
+@pytest.mark.parametrize("m,k,n", [(70000, 128, 128), (70001, 50, 128), (66000, 100, 30), (300_000, 130, 40), (70016, 64, 64), (70003, 200, 150), (66001, 256, 256), (80000, 300, 40)])
 def test_many_rows(K, m, k, n):
     """Where the weight gradient sums over slices of the rows, and the wide path goes in chunks; small whole numbers, so that every
     product and sum is exact and the result has to be equal to the last bit."""
