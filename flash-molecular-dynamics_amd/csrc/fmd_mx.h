@@ -9,7 +9,9 @@
 // Planes: an fp32 value is the exact sum of three bf16 (truncation keeps 8 significant bits at a time), an fp16 value of
 // two, a bf16 value and every 4- or 8-bit block value is one.  A product of plane sums keeps the plane pairs (i, j) with
 // i + j < max(planes): what is dropped is below the last kept plane's last bit.  bf16 has fp32's range, so no operand
-// needs a scale of its own.
+// needs a scale of its own.  Where every operand is fp16 or a function of fp16 values that stays in its range (a wide layer's
+// training products), one fp16 plane does the work of two bf16 ones: tanh is rounded to 2^-12, and an 8-bit value below 2^-17 to a
+// multiple of fp16's smallest, 2^-24, as its fp16 input was.
 #pragma once
 #include "fmd_common.h"
 
@@ -143,12 +145,20 @@ __device__ __forceinline__ void mx_split2(float x, float y, uint32_t (&out)[P]) 
     }
   }
 }
+// P = 0: one plane of fp16
 template <int P>
-__device__ __forceinline__ void mx_split8(const float (&v)[8], u32x4 (&out)[P]) {
+__device__ __forceinline__ void mx_split8(const float (&v)[8], u32x4 (&out)[P ? P : 1]) {
+  if constexpr (P == 0) {
+    f16x8 o;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i] = (_Float16)v[i];
+    out[0] = __builtin_bit_cast(u32x4, o);
+    return;
+  }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    uint32_t o[P];
-    mx_split2<P>(v[2 * i], v[2 * i + 1], o);
+    uint32_t o[P ? P : 1];
+    mx_split2<P ? P : 1>(v[2 * i], v[2 * i + 1], o);
 #pragma unroll
     for (int p = 0; p < P; ++p) out[p][i] = o[p];
   }

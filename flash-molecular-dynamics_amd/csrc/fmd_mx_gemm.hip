@@ -106,10 +106,11 @@ __global__ __launch_bounds__(256) void planes_kernel(S src, int64_t rows, int64_
     const int64_t row = t / per, c0 = (t - row * per) * 8;
     float v[8];
     src.load(row, c0, v);
-    u32x4 o[P];
+    constexpr int N = P ? P : 1;
+    u32x4 o[N];
     mx_split8<P>(v, o);
 #pragma unroll
-    for (int p = 0; p < P; ++p) *(u32x4*)(out + (int64_t)p * rows * pad + row * pad + c0) = o[p];
+    for (int p = 0; p < N; ++p) *(u32x4*)(out + (int64_t)p * rows * pad + row * pad + c0) = o[p];
   }
 }
 
@@ -136,10 +137,11 @@ __global__ __launch_bounds__(256) void planes_keep_kernel(SrcDense<T, false> src
     if constexpr (TANH)
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] = mx_tanh(v[i]);
-    u32x4 o[P];
+    constexpr int N = P ? P : 1;
+    u32x4 o[N];
     mx_split8<P>(v, o);
 #pragma unroll
-    for (int p = 0; p < P; ++p) *(u32x4*)(out + (int64_t)p * rows * pad + row * pad + q * 8) = o[p];
+    for (int p = 0; p < N; ++p) *(u32x4*)(out + (int64_t)p * rows * pad + row * pad + q * 8) = o[p];
   }
 }
 
@@ -147,7 +149,8 @@ __global__ __launch_bounds__(256) void planes_keep_kernel(SrcDense<T, false> src
 // through LDS, rows 66 halves apart so that neither side meets a bank twice more than it has to
 template <class S, int P>
 __global__ __launch_bounds__(256) void planes_t_kernel(S src, int64_t rows, int64_t cols, int64_t pad, uint16_t* __restrict__ out) {
-  __shared__ uint32_t tile[P][64][33];
+  constexpr int N = P ? P : 1;
+  __shared__ uint32_t tile[N][64][33];
   const int64_t r0 = (int64_t)blockIdx.x * 64, c0 = (int64_t)blockIdx.y * 64;
   const int t = threadIdx.x;
 #pragma unroll
@@ -160,10 +163,10 @@ __global__ __launch_bounds__(256) void planes_t_kernel(S src, int64_t rows, int6
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] = 0.f;
     }
-    u32x4 o[P];
+    u32x4 o[N];
     mx_split8<P>(v, o);
 #pragma unroll
-    for (int p = 0; p < P; ++p)
+    for (int p = 0; p < N; ++p)
 #pragma unroll
       for (int j = 0; j < 4; ++j) tile[p][r][(c >> 1) + j] = o[p][j];
   }
@@ -173,7 +176,7 @@ __global__ __launch_bounds__(256) void planes_t_kernel(S src, int64_t rows, int6
     const int c = (t >> 3) + 32 * i, r = (t & 7) * 8;
     if (c0 + c >= cols) continue;
 #pragma unroll
-    for (int p = 0; p < P; ++p) {
+    for (int p = 0; p < N; ++p) {
       u32x4 o;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -231,8 +234,11 @@ __device__ __forceinline__ void finish_one(const MxEpilogue& e, int64_t row, int
   ((T*)e.out)[row * ld + col] = MxType<T>::from(v);
 }
 
-template <class T, bool FP4, int WM, int WN, int TM, int TN>
+enum { FMT_BF16, FMT_FP4, FMT_F16 };
+
+template <class T, int FMT, int WM, int WN, int TM, int TN>
 __global__ __launch_bounds__(64 * WM * WN) void gemm_kernel(const GemmArgs g) {
+  constexpr bool FP4 = FMT == FMT_FP4;
   static_assert(TM % 2 == 0 && TN % 2 == 0, "two rows of a line belong to one lane");
   constexpr int BM = 32 * WM * TM, BN = 32 * WN * TN, NW = WM * WN, SLOTS = (BM + BN) * 8, LOADS = SLOTS / (64 * NW);
   __shared__ __attribute__((aligned(16))) char lds[2 * (BM + BN) * 128];
@@ -324,6 +330,9 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_kernel(const GemmArgs g) {
         const i32x8 xa = {(int)ua[0], (int)ua[1], (int)ua[2], (int)ua[3], 0, 0, 0, 0};                                      \
         const i32x8 xb = {(int)ub[0], (int)ub[1], (int)ub[2], (int)ub[3], 0, 0, 0, 0};                                      \
         acc[a][b] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(xa, xb, acc[a][b], 4, 4, s, (int)sa[a], s, (int)sb[b]); \
+      } else if constexpr (FMT == FMT_F16) {                                                                                \
+        acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, ua), __builtin_bit_cast(f16x8, ub),    \
+                                                           acc[a][b], 0, 0, 0);                                             \
       } else {                                                                                                              \
         acc[a][b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, ua), __builtin_bit_cast(bf16x8, ub), \
                                                             acc[a][b], 0, 0, 0);                                            \
@@ -555,9 +564,11 @@ void mx_planes(const MxSource& q, int64_t rows, int64_t cols, bool transposed, v
       MX_RUN(SrcI8<true>, P, {(const uint8_t*)q.p, (const uint8_t*)q.aux, cols, mx_blocks(cols)});                       \
   } while (0)
 #define MX_ARG(...) __VA_ARGS__
-  if (q.kind == MX_SRC_I8) MX_RUN(SrcI8<false>, 1, {(const uint8_t*)q.p, (const uint8_t*)q.aux, cols, mx_blocks(cols)});
+  if (q.kind == MX_SRC_I8 && q.half) MX_RUN(SrcI8<false>, 0, {(const uint8_t*)q.p, (const uint8_t*)q.aux, cols, mx_blocks(cols)});
+  else if (q.kind == MX_SRC_I8) MX_RUN(SrcI8<false>, 1, {(const uint8_t*)q.p, (const uint8_t*)q.aux, cols, mx_blocks(cols)});
   else if (q.kind == MX_SRC_FP4) MX_RUN(SrcFp4, 1, {(const uint8_t*)q.p, (const uint8_t*)q.aux, cols, mx_blocks(cols)});
   else if (q.dtype == FMD_F32) MX_TYPED(float, 3);
+  else if (q.half) MX_TYPED(_Float16, 0);
   else if (q.dtype == FMD_F16) MX_TYPED(_Float16, 2);
   else MX_TYPED(mx_bf16, 1);
 #undef MX_RUN
@@ -575,7 +586,7 @@ void mx_planes_keep(const MxSource& q, int64_t rows, int64_t cols, void* out, ui
     else planes_keep_kernel<T, false, P><<<grid, 256, 0, s>>>(src, rows, pad, (uint16_t*)out, nb, codes, scales);                 \
   } while (0)
   if (q.dtype == FMD_F32) MX_TYPED(float, 3);
-  else if (q.dtype == FMD_F16) MX_TYPED(_Float16, 2);
+  else if (q.dtype == FMD_F16) MX_TYPED(_Float16, 0);
   else MX_TYPED(mx_bf16, 1);
 #undef MX_TYPED
 }
@@ -599,11 +610,11 @@ MxProductPlan mx_product_plan(int64_t m, int64_t n, int64_t kt, int npairs) {
   return p;
 }
 
-template <class T, bool FP4>
+template <class T, int FMT>
 static void launch_gemm(const GemmArgs& g, bool big, hipStream_t s) {
   const dim3 grid((unsigned)(g.tiles_m * g.tiles_n), (unsigned)g.splits);
-  if (big) gemm_kernel<T, FP4, 2, 4, 4, 2><<<grid, 512, 0, s>>>(g);
-  else gemm_kernel<T, FP4, 2, 2, 2, 2><<<grid, 256, 0, s>>>(g);
+  if (big) gemm_kernel<T, FMT, 2, 4, 4, 2><<<grid, 512, 0, s>>>(g);
+  else gemm_kernel<T, FMT, 2, 2, 2, 2><<<grid, 256, 0, s>>>(g);
 }
 
 void mx_product(const MxOperand& a, const MxOperand& b, int64_t m, int64_t n, int64_t kt, const MxProductPlan& plan, int dtype,
@@ -620,10 +631,19 @@ void mx_product(const MxOperand& a, const MxOperand& b, int64_t m, int64_t n, in
   for (int i = 0; i < pairs.n; ++i) g.pa |= (uint32_t)pairs.a[i] << 2 * i, g.pb |= (uint32_t)pairs.b[i] << 2 * i;
   g.e = e;
   g.partial = parts;
-  const bool fp4 = a.scales != nullptr;
-  if (parts || dtype == FMD_F32) fp4 ? launch_gemm<float, true>(g, plan.big, s) : launch_gemm<float, false>(g, plan.big, s);
-  else if (dtype == FMD_F16) fp4 ? launch_gemm<_Float16, true>(g, plan.big, s) : launch_gemm<_Float16, false>(g, plan.big, s);
-  else fp4 ? launch_gemm<mx_bf16, true>(g, plan.big, s) : launch_gemm<mx_bf16, false>(g, plan.big, s);
+  const bool f32 = parts || dtype == FMD_F32;
+  if (a.scales) {
+    if (f32) launch_gemm<float, FMT_FP4>(g, plan.big, s);
+    else if (dtype == FMD_F16) launch_gemm<_Float16, FMT_FP4>(g, plan.big, s);
+    else launch_gemm<mx_bf16, FMT_FP4>(g, plan.big, s);
+  } else if (a.half) {
+    if (f32) launch_gemm<float, FMT_F16>(g, plan.big, s);
+    else launch_gemm<_Float16, FMT_F16>(g, plan.big, s);
+  } else {
+    if (f32) launch_gemm<float, FMT_BF16>(g, plan.big, s);
+    else if (dtype == FMD_F16) launch_gemm<_Float16, FMT_BF16>(g, plan.big, s);
+    else launch_gemm<mx_bf16, FMT_BF16>(g, plan.big, s);
+  }
 }
 
 void mx_sum_parts(const float* parts, int64_t count, int64_t m, int64_t n, int dtype, const MxEpilogue& e, hipStream_t s) {

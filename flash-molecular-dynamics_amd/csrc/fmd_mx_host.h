@@ -15,6 +15,7 @@ enum { MX_SRC_DENSE, MX_SRC_TANH, MX_SRC_GRAD_Y, MX_SRC_GRAD_D, MX_SRC_I8, MX_SR
 struct MxSource {
   int kind, dtype;      // dtype: of p where it is dense, of the planes for 8 bits under tanh
   const void *p, *aux;  // aux: y or its derivative, or the scales
+  bool half;            // one plane of fp16 instead of bf16 planes
 };
 
 struct MxOperand {  // K-contiguous rows
@@ -22,6 +23,7 @@ struct MxOperand {  // K-contiguous rows
   int64_t plane, pitch;  // bytes
   int planes;
   const void* scales;  // 4-bit operand: [tile of 8 blocks][half][row][4], else null
+  bool half;           // the plane is fp16
 };
 
 struct MxProductPlan {
@@ -86,6 +88,9 @@ hipError_t mx_allow_lds(K kernel, int bytes) {
 }
 
 static inline int mx_dtype_size(int dtype) { return dtype == FMD_F32 ? 4 : 2; }
+// products of 16-bit operands alone: one plane of their own type
+static inline bool mx_half(int dtype) { return dtype == FMD_F16; }
+static inline int mx_own_planes(int dtype) { return dtype == FMD_F32 ? 3 : 1; }
 static inline int mx_dtype_planes(int dtype) { return dtype == FMD_F32 ? 3 : dtype == FMD_F16 ? 2 : 1; }
 
 // workspace laid out by the same code that uses it: with a null base it only counts

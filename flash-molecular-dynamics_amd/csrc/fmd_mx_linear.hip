@@ -27,7 +27,7 @@ MxEpilogue rows_of(const MxEpilogue& e, int64_t r0, int64_t n, int dtype) {
 // only counts the workspace
 void product_of_rows(MxArena& ar, bool run, MxSource q, int64_t m, int64_t k, const MxOperand& b, int64_t n, int dtype,
                      const MxEpilogue& e, hipStream_t s, uint8_t* codes = nullptr, uint8_t* scales = nullptr) {
-  const int pa = mx_dtype_planes(dtype);
+  const int pa = q.half ? 1 : mx_dtype_planes(dtype);
   const int64_t pad = mx_up(k, 64), kt = pad / 64, rows = chunk_rows(m, pa * pad * 2);
   const MxProductPlan plan = mx_product_plan(rows, n, kt, mx_pairs(pa, b.planes).n);
   void* planes = ar.take(pa * rows * pad * 2);
@@ -40,7 +40,7 @@ void product_of_rows(MxArena& ar, bool run, MxSource q, int64_t m, int64_t k, co
     part.p = at(q.p, r0 * k, size), part.aux = at(q.aux, r0 * k, aux);
     if (codes) mx_planes_keep(part, c, k, planes, codes + r0 * mx_blocks(k) * 32, scales + r0 * mx_blocks(k), s);
     else mx_planes(part, c, k, false, planes, s);
-    const MxOperand a{planes, c * pad * 2, pad * 2, pa, nullptr};
+    const MxOperand a{planes, c * pad * 2, pad * 2, pa, nullptr, q.half};
     const MxEpilogue ep = rows_of(e, r0, n, dtype);
     mx_product(a, b, c, n, kt, plan, dtype, ep, parts, s);
     if (parts) mx_sum_parts(parts, plan.splits, c, n, dtype, ep, s);
@@ -50,7 +50,8 @@ void product_of_rows(MxArena& ar, bool run, MxSource q, int64_t m, int64_t k, co
 // out[k,n] = A^T B summed over the rows of A = qa [m,k] and B = qb [m,n], chunk by chunk in the order of the rows
 void product_over_rows(MxArena& ar, bool run, MxSource qa, int pa, int64_t k, MxSource qb, int64_t n, int64_t m, int dtype, void* out,
                        hipStream_t s) {
-  const int pb = mx_dtype_planes(dtype);
+  const int pb = mx_own_planes(dtype);
+  const bool half = mx_half(dtype);
   const int64_t rows = chunk_rows(m, 2 * (pa * k + pb * n));
   const int64_t pad = mx_up(rows, 64), chunks = (m + rows - 1) / rows;
   const MxProductPlan plan = mx_product_plan(k, n, pad / 64, mx_pairs(pa, pb).n);
@@ -69,7 +70,7 @@ void product_over_rows(MxArena& ar, bool run, MxSource qa, int pa, int64_t k, Mx
     mx_planes(a, c, k, true, ta, s);
     mx_planes(b, c, n, true, tb, s);
     const MxProductPlan here = c == rows ? plan : mx_product_plan(k, n, cpad / 64, mx_pairs(pa, pb).n);
-    mx_product({ta, k * cpad * 2, cpad * 2, pa, nullptr}, {tb, n * cpad * 2, cpad * 2, pb, nullptr}, k, n, cpad / 64, here, dtype, e,
+    mx_product({ta, k * cpad * 2, cpad * 2, pa, nullptr, half}, {tb, n * cpad * 2, cpad * 2, pb, nullptr, half}, k, n, cpad / 64, here, dtype, e,
                parts ? parts + count * k * n : nullptr, s);
     count += here.splits;
   }
@@ -119,14 +120,14 @@ int64_t fp4_forward(const Fp4Linear& c, void* base, bool run, hipStream_t s) {
     if (run) {
       mx_quantize4_for_product(c.x, c.dtype, c.m, c.k, xc, xs, s);
       mx_scale_tiles(c.scales, c.n, nb, ws, s);
-      mx_product({xc, 0, nb * 16, 1, xs}, {c.codes, 0, nb * 16, 1, ws}, c.m, c.n, kt, plan, c.dtype, c.e, parts, s);
+      mx_product({xc, 0, nb * 16, 1, xs, false}, {c.codes, 0, nb * 16, 1, ws, false}, c.m, c.n, kt, plan, c.dtype, c.e, parts, s);
       if (parts) mx_sum_parts(parts, plan.splits, c.m, c.n, c.dtype, c.e, s);
     }
   } else {
     const int64_t pad = mx_up(c.k, 64);
     void* w = ar.take(c.n * pad * 2);
-    if (run) mx_planes({MX_SRC_FP4, FMD_BF16, c.codes, c.scales}, c.n, c.k, false, w, s);
-    product_of_rows(ar, run, {MX_SRC_DENSE, c.dtype, c.x, nullptr}, c.m, c.k, {w, c.n * pad * 2, pad * 2, 1, nullptr}, c.n, c.dtype,
+    if (run) mx_planes({MX_SRC_FP4, FMD_BF16, c.codes, c.scales, false}, c.n, c.k, false, w, s);
+    product_of_rows(ar, run, {MX_SRC_DENSE, c.dtype, c.x, nullptr, false}, c.m, c.k, {w, c.n * pad * 2, pad * 2, 1, nullptr, false}, c.n, c.dtype,
                     c.e, s);
   }
   return ar.used;
@@ -141,7 +142,7 @@ struct Fp4Backward {
 
 int64_t fp4_backward(const Fp4Backward& c, void* base, bool run, bool want_gx, bool want_gb, hipStream_t s) {
   MxArena ar{(char*)base, 0};
-  const MxSource g{c.kind, c.dtype, c.g, c.aux};
+  const MxSource g{c.kind, c.dtype, c.g, c.aux, false};
   const MxEpilogue to_gx{nullptr, c.gx, nullptr, nullptr, nullptr, 0, 0};
   if (want_gx && mx_layer_fits(c.n, c.k)) {
     float* sums = want_gb ? (float*)ar.take(mx_layer_sums_bytes(c.m, c.n)) : nullptr;
@@ -152,8 +153,8 @@ int64_t fp4_backward(const Fp4Backward& c, void* base, bool run, bool want_gx, b
   } else if (want_gx) {
     const int64_t pad = mx_up(c.n, 64);
     void* w = ar.take(c.k * pad * 2);
-    if (run) mx_planes({MX_SRC_FP4, FMD_BF16, c.codes, c.scales}, c.n, c.k, true, w, s);
-    product_of_rows(ar, run, g, c.m, c.n, {w, c.k * pad * 2, pad * 2, 1, nullptr}, c.k, c.dtype, to_gx, s);
+    if (run) mx_planes({MX_SRC_FP4, FMD_BF16, c.codes, c.scales, false}, c.n, c.k, true, w, s);
+    product_of_rows(ar, run, g, c.m, c.n, {w, c.k * pad * 2, pad * 2, 1, nullptr, false}, c.k, c.dtype, to_gx, s);
   }
   if (want_gb) sum_over_rows(ar, run, g, c.m, c.n, c.dtype, c.gb, s);
   return ar.used;
@@ -178,19 +179,21 @@ int64_t kept_forward(const Kept& c, void* base, bool run, hipStream_t s) {
                c.dtype, c.m, c.k, c.n, s);
     return 0;
   }
-  const int p = mx_dtype_planes(c.dtype);
+  const int p = mx_own_planes(c.dtype);
+  const bool half = mx_half(c.dtype);
   const int64_t pad = mx_up(c.k, 64);
   void* w = ar.take(p * c.n * pad * 2);
-  if (run) mx_planes({MX_SRC_DENSE, c.dtype, c.w, nullptr}, c.k, c.n, true, w, s);
-  product_of_rows(ar, run, {c.tanh ? MX_SRC_TANH : MX_SRC_DENSE, c.dtype, c.x, nullptr}, c.m, c.k,
-                  {w, c.n * pad * 2, pad * 2, p, nullptr}, c.n, c.dtype, c.e, s, c.codes, c.scales);
+  if (run) mx_planes({MX_SRC_DENSE, c.dtype, c.w, nullptr, half}, c.k, c.n, true, w, s);
+  product_of_rows(ar, run, {c.tanh ? MX_SRC_TANH : MX_SRC_DENSE, c.dtype, c.x, nullptr, half}, c.m, c.k,
+                  {w, c.n * pad * 2, pad * 2, p, nullptr, half}, c.n, c.dtype, c.e, s, c.codes, c.scales);
   return ar.used;
 }
 
 int64_t kept_backward(const Kept& c, void* base, bool run, bool want_gx, bool want_gw, bool want_gb, hipStream_t s) {
   MxArena ar{(char*)base, 0};
-  const int p = mx_dtype_planes(c.dtype);
-  const MxSource g{MX_SRC_DENSE, c.dtype, c.g, nullptr};
+  const int p = mx_own_planes(c.dtype);
+  const bool half = mx_half(c.dtype);
+  const MxSource g{MX_SRC_DENSE, c.dtype, c.g, nullptr, half};
   const bool narrow = mx_layer_fits(c.n, c.k);
   if (want_gx && narrow) {
     if (run)
@@ -199,10 +202,10 @@ int64_t kept_backward(const Kept& c, void* base, bool run, bool want_gx, bool wa
   } else if (want_gx) {
     const int64_t pad = mx_up(c.n, 64);
     void* w = ar.take(p * c.k * pad * 2);
-    if (run) mx_planes({MX_SRC_DENSE, c.dtype, c.w, nullptr}, c.k, c.n, false, w, s);
+    if (run) mx_planes({MX_SRC_DENSE, c.dtype, c.w, nullptr, half}, c.k, c.n, false, w, s);
     MxEpilogue e{nullptr, c.gx, nullptr, nullptr, nullptr, 0, 0};
     if (c.tanh) e.codes8 = c.codes, e.scales8 = c.scales, e.nb8 = mx_blocks(c.k);
-    product_of_rows(ar, run, g, c.m, c.n, {w, c.k * pad * 2, pad * 2, p, nullptr}, c.k, c.dtype, e, s);
+    product_of_rows(ar, run, g, c.m, c.n, {w, c.k * pad * 2, pad * 2, p, nullptr, half}, c.k, c.dtype, e, s);
   }
   if ((want_gw || want_gb) && mx_gradient_fits(c.m, c.n, c.k)) {  // the bias's sums come along
     const int64_t bytes = mx_gradient_bytes(c.dtype, c.m, c.n, c.k);
@@ -211,7 +214,7 @@ int64_t kept_backward(const Kept& c, void* base, bool run, bool want_gx, bool wa
     return ar.used;
   }
   if (want_gw)
-    product_over_rows(ar, run, {c.tanh ? MX_SRC_I8_TANH : MX_SRC_I8, c.dtype, c.codes, c.scales}, c.tanh ? p : 1, c.k, g, c.n, c.m,
+    product_over_rows(ar, run, {c.tanh ? MX_SRC_I8_TANH : MX_SRC_I8, c.dtype, c.codes, c.scales, half}, c.tanh ? p : 1, c.k, g, c.n, c.m,
                       c.dtype, c.gw, s);
   if (want_gb) sum_over_rows(ar, run, g, c.m, c.n, c.dtype, c.gb, s);
   return ar.used;
