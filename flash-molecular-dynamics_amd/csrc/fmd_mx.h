@@ -114,6 +114,15 @@ __device__ __forceinline__ float mx_tanh(float x) {
   return a < 0.25f ? p : t;  // a NaN takes the second and stays one
 }
 
+// v times tanh' of an 8-bit value.  The product is rounded to fp32 before anything else is made of it (the compiler would form
+// it and round it to 16 bits in one instruction here and two there), so that every kernel gives the same bits.
+__device__ __forceinline__ float mx_times_dtanh(float v, int code, uint32_t byte) {
+  const float y = mx_tanh(mx_value8(code, byte));
+  float r = v * __builtin_fmaf(-y, y, 1.f);
+  asm("" : "+v"(r));
+  return r;
+}
+
 // a wave-uniform value that the compiler takes for a new one: what is computed from it stays where it is used, in scalar
 // registers, instead of becoming dozens of loop-invariant vector registers
 __device__ __forceinline__ int mx_here(int v) {

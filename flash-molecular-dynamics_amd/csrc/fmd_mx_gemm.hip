@@ -227,10 +227,7 @@ __device__ __forceinline__ void finish_one(const MxEpilogue& e, int64_t row, int
   if (e.bias) v += MxType<T>::to(((const T*)e.bias)[col]);
   if (e.tanh) v = mx_tanh(v);
   if (e.dact) ((_Float16*)e.dact)[row * ld + col] = (_Float16)(1.f - v * v);
-  if (e.codes8) {
-    const float t = mx_tanh(mx_value8((int)(int8_t)e.codes8[row * e.nb8 * 32 + col], e.scales8[row * e.nb8 + (col >> 5)]));
-    v *= 1.f - t * t;
-  }
+  if (e.codes8) v = mx_times_dtanh(v, (int)(int8_t)e.codes8[row * e.nb8 * 32 + col], e.scales8[row * e.nb8 + (col >> 5)]);
   ((T*)e.out)[row * ld + col] = MxType<T>::from(v);
 }
 
@@ -425,10 +422,7 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_kernel(const GemmArgs g) {
           if (!INSIDE && (row_of(a, r) >= g.m || col >= g.n)) continue;
           float v[TN];
 #pragma unroll
-          for (int b = 0; b < TN; ++b) {
-            const float x = mx_tanh(mx_value8((int)(int8_t)(code[r] >> 8 * b), byte[r]));
-            v[b] = acc[a][b][r] * (1.f - x * x);
-          }
+          for (int b = 0; b < TN; ++b) v[b] = mx_times_dtanh(acc[a][b][r], (int)(int8_t)(code[r] >> 8 * b), byte[r]);
           write((T*)g.e.out + row_of(a, r) * ld + col, v);
         }
       }

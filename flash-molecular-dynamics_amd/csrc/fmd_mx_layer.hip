@@ -416,10 +416,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void layer_kernel(const LayerArgs a)
         const uint32_t byte = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(scales, sat + row * nbs, 0, 0);
         float v[NT];
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          const float y = mx_tanh(mx_value8((int)(int8_t)(q >> 8 * t), byte));
-          v[t] = acc[t][r] * (1.f - y * y);
-        }
+        for (int t = 0; t < NT; ++t) v[t] = mx_times_dtanh(acc[t][r], (int)(int8_t)(q >> 8 * t), byte);
         write(T{}, out, r, v);
       }
     } else {

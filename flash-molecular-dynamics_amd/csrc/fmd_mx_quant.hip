@@ -21,20 +21,24 @@ __device__ __forceinline__ void load8(const T* __restrict__ row, int64_t c0, int
     for (int i = 0; i < 8; ++i) v[i] = MxType<T>::to(t[i]);
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = c0 + i < k ? MxType<T>::to(row[c0 + i]) : 0.f;
+    for (int i = 0; i < 8; ++i) {
+      const bool there = c0 + i < k;  // the load itself is unconditional, of a value that exists
+      const float x = MxType<T>::to(row[there ? c0 + i : 0]);
+      v[i] = there ? x : 0.f;
+    }
   }
 }
 
 struct QuantArgs {
   int64_t m, k, nb;
-  int vec, for_product;
+  int vec;
   uint32_t* codes;
   uint8_t* scales;
 };
 
-// for_product: where the scale byte of (row, block) goes.  0: [row][blocks].  1: [block/8][block&1][row][4] with
+// PRODUCT: where the scale byte of (row, block) goes.  false: [row][blocks].  true: [block/8][block&1][row][4] with
 // the rows rounded up to 4, as the product kernel reads them.  The four lanes of a block are always active together
-template <int BITS>
+template <int BITS, bool PRODUCT>
 __device__ __forceinline__ void quantize8(const QuantArgs& a, int64_t row, int64_t q, const float (&v)[8]) {
   const int64_t t = row * a.nb * 4 + q;
   uint32_t top = 0;
@@ -51,7 +55,7 @@ __device__ __forceinline__ void quantize8(const QuantArgs& a, int64_t row, int64
   }
   if ((q & 3) == 0) {
     const int64_t b = q >> 2;
-    if (a.for_product) {
+    if constexpr (PRODUCT) {
       const int64_t pad = (a.m + 3) & ~(int64_t)3;
       auto at = [&](int64_t i) { return a.scales + (((i >> 3) * 2 + (i & 1)) * pad + row) * 4 + (i >> 1 & 3); };
       *at(b) = (uint8_t)byte;
@@ -63,18 +67,18 @@ __device__ __forceinline__ void quantize8(const QuantArgs& a, int64_t row, int64
   }
 }
 
-template <class T, int BITS>
+template <class T, int BITS, bool PRODUCT>
 __global__ __launch_bounds__(256) void quantize_kernel(const T* __restrict__ x, const QuantArgs a) {
   const int64_t total = a.m * a.nb * 4;
   for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < total; t += (int64_t)gridDim.x * 256) {
     const int64_t row = t / (a.nb * 4), q = t - row * (a.nb * 4);
     float v[8];
     load8<T>(x + row * a.k, q * 8, a.k, a.vec != 0, v);
-    quantize8<BITS>(a, row, q, v);
+    quantize8<BITS, PRODUCT>(a, row, q, v);
   }
 }
 
-template <class T, int BITS>
+template <class T, int BITS, bool PRODUCT>
 __global__ __launch_bounds__(256) void quantize_staged_kernel(const T* __restrict__ x, const QuantArgs a) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int k = (int)a.k, q4 = (int)a.nb * 4;
@@ -93,7 +97,7 @@ __global__ __launch_bounds__(256) void quantize_staged_kernel(const T* __restric
       const int row = t / q4, q = t - row * q4;
       float v[8];
       load8<T>((const T*)lds + row * k, q * 8, k, false, v);
-      quantize8<BITS>(a, row0 + row, q, v);
+      quantize8<BITS, PRODUCT>(a, row0 + row, q, v);
     }
     __syncthreads();
   }
@@ -171,14 +175,14 @@ int grid_for(int64_t threads) {
   return (int)(g < 256 * 16 ? g : 256 * 16);
 }
 
-template <class T, int BITS>
+template <class T, int BITS, bool PRODUCT>
 void run_quantize(const T* x, QuantArgs a, hipStream_t s) {
   a.vec = a.k * sizeof(T) % 16 == 0;
   if (!a.vec && a.k * (int64_t)sizeof(T) * ROWS <= STAGE) {
     const int64_t groups = (a.m + ROWS - 1) / ROWS;
-    quantize_staged_kernel<T, BITS><<<(int)(groups < 8192 ? groups : 8192), 256, (int)mx_up(a.k * sizeof(T) * ROWS, 16), s>>>(x, a);
+    quantize_staged_kernel<T, BITS, PRODUCT><<<(int)(groups < 8192 ? groups : 8192), 256, (int)mx_up(a.k * sizeof(T) * ROWS, 16), s>>>(x, a);
   } else {
-    quantize_kernel<T, BITS><<<grid_for(a.m * a.nb * 4), 256, 0, s>>>(x, a);
+    quantize_kernel<T, BITS, PRODUCT><<<grid_for(a.m * a.nb * 4), 256, 0, s>>>(x, a);
   }
 }
 
@@ -193,15 +197,15 @@ void run_dequantize(QuantArgs a, T* out, hipStream_t s) {
   }
 }
 
-template <int BITS>
-int quantize(const void* x, int dtype, int64_t m, int64_t k, void* codes, void* scales, int for_product, hipStream_t s) {
+template <int BITS, bool PRODUCT = false>
+int quantize(const void* x, int dtype, int64_t m, int64_t k, void* codes, void* scales, hipStream_t s) {
   if (m < 0 || k < 1 || dtype < 0 || dtype > 2) return FMD_EINVAL;
   if (m == 0) return FMD_OK;
   if (!x || !codes || !scales || ((uintptr_t)x & 15) || ((uintptr_t)codes & 15)) return FMD_EINVAL;
-  const QuantArgs a{m, k, mx_blocks(k), 0, for_product, (uint32_t*)codes, (uint8_t*)scales};
-  if (dtype == FMD_F32) run_quantize<float, BITS>((const float*)x, a, s);
-  else if (dtype == FMD_F16) run_quantize<_Float16, BITS>((const _Float16*)x, a, s);
-  else run_quantize<mx_bf16, BITS>((const mx_bf16*)x, a, s);
+  const QuantArgs a{m, k, mx_blocks(k), 0, (uint32_t*)codes, (uint8_t*)scales};
+  if (dtype == FMD_F32) run_quantize<float, BITS, PRODUCT>((const float*)x, a, s);
+  else if (dtype == FMD_F16) run_quantize<_Float16, BITS, PRODUCT>((const _Float16*)x, a, s);
+  else run_quantize<mx_bf16, BITS, PRODUCT>((const mx_bf16*)x, a, s);
   FMD_CHECK_LAUNCH();
   return FMD_OK;
 }
@@ -211,7 +215,7 @@ int dequantize(const void* codes, const void* scales, int64_t m, int64_t k, void
   if (m < 0 || k < 1 || dtype < 0 || dtype > 2) return FMD_EINVAL;
   if (m == 0) return FMD_OK;
   if (!out || !codes || !scales || ((uintptr_t)out & 15) || ((uintptr_t)codes & 15)) return FMD_EINVAL;
-  const QuantArgs a{m, k, mx_blocks(k), 0, 0, (uint32_t*)codes, (uint8_t*)scales};
+  const QuantArgs a{m, k, mx_blocks(k), 0, (uint32_t*)codes, (uint8_t*)scales};
   if (dtype == FMD_F32) run_dequantize<float, BITS>(a, (float*)out, s);
   else if (dtype == FMD_F16) run_dequantize<_Float16, BITS>(a, (_Float16*)out, s);
   else run_dequantize<mx_bf16, BITS>(a, (mx_bf16*)out, s);
@@ -222,18 +226,18 @@ int dequantize(const void* codes, const void* scales, int64_t m, int64_t k, void
 }  // namespace
 
 int mx_quantize4_for_product(const void* x, int dtype, int64_t m, int64_t k, void* codes, void* scales, hipStream_t s) {
-  return quantize<4>(x, dtype, m, k, codes, scales, 1, s);
+  return quantize<4, true>(x, dtype, m, k, codes, scales, s);
 }
 
 extern "C" int fmd_mxfp4_quantize(const void* x, int dtype, int64_t m, int64_t k, void* codes, void* scales, void* stream) {
-  return quantize<4>(x, dtype, m, k, codes, scales, 0, fmd_stream(stream));
+  return quantize<4>(x, dtype, m, k, codes, scales, fmd_stream(stream));
 }
 extern "C" int fmd_mxfp4_dequantize(const void* codes, const void* scales, int64_t m, int64_t k, void* out, int dtype,
                                     void* stream) {
   return dequantize<4>(codes, scales, m, k, out, dtype, fmd_stream(stream));
 }
 extern "C" int fmd_mxint8_quantize(const void* x, int dtype, int64_t m, int64_t k, void* codes, void* scales, void* stream) {
-  return quantize<8>(x, dtype, m, k, codes, scales, 0, fmd_stream(stream));
+  return quantize<8>(x, dtype, m, k, codes, scales, fmd_stream(stream));
 }
 extern "C" int fmd_mxint8_dequantize(const void* codes, const void* scales, int64_t m, int64_t k, void* out, int dtype,
                                      void* stream) {

@@ -407,7 +407,7 @@ def test_offsets_beyond_32_bits(K):
     near(K.mxfp4_linear(x.detach(), wc.to(DEV), wsc.to(DEV))[-70:], mo.linear(tail, wv), k)
 
 
-@pytest.mark.parametrize("m,k,n", [(70000, 128, 128), (70001, 50, 128), (66000, 100, 30), (300_000, 130, 40), (70016, 64, 64), (70003, 200, 150), (66001, 256, 256), (80000, 300, 40)])
+@pytest.mark.parametrize("m,k,n", [(70000, 128, 128), (70001, 50, 128), (66000, 100, 30), (300_000, 130, 40), (70016, 64, 64), (70003, 200, 150), (70005, 64, 33), (65600, 33, 128), (66001, 256, 256), (80000, 300, 40)])
 def test_many_rows(K, m, k, n):
     """Where the weight gradient sums over slices of the rows, and the wide path goes in chunks; small whole numbers, so that every
     product and sum is exact and the result has to be equal to the last bit."""
@@ -522,3 +522,33 @@ def test_training_step_with_activation_checkpoints():
     assert any(v > 1e-4 for v in off.values())               # the checkpoints were used
     e1, again = step()
     assert torch.equal(e1, e0) and all(rel(a, b) < 1e-5 for a, b in zip(again, exact))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("k,n", [(50, 128), (64, 64), (33, 127), (7, 30)])
+@pytest.mark.parametrize("tanh", [False, True])
+def test_both_gradients_of_many_rows(K, k, n, tanh, dtype):
+    """Many rows of a narrow layer, against 64 bits on the GPU; gx is bit for bit the same when it is asked for alone.  In fp16 a few of the uneven values are beyond its range: what
+    comes of them is not finite where the reference is not, and everything else is as near as ever."""
+    m = 66_005
+    g = rand(m, n, seed=1, scale=1e-2, dtype=dtype).to(DEV)
+    x, w, b = uneven(m, k, dtype, seed=2).to(DEV), rand(k, n, seed=3, scale=0.2, dtype=dtype).to(DEV), rand(n, seed=4, dtype=dtype).to(DEV)
+    op = K.fused_tanh_linear_ckpt8_autograd if tanh else K.linear_ckpt8_autograd
+    leaves = [t.clone().requires_grad_() for t in (x, w, b)]
+    y = op(*leaves)
+    gx, gw, gb = torch.autograd.grad(y, leaves, g)
+    kept = K.mxint8_dequantize(*K.mxint8_quantize(x), k).double()
+    G, W = g.double(), w.double()
+    p = torch.tanh if tanh else (lambda t: t)
+
+    def finite_near(got, want, terms):
+        fine = torch.isfinite(want)
+        assert torch.equal(torch.isfinite(got), fine)
+        near(got[fine], want[fine], terms)
+
+    finite_near(y, p(x.double()) @ W + b.double(), k)
+    finite_near(gx, (G @ W.t().contiguous()) * ((1 - torch.tanh(kept) ** 2) if tanh else 1.0), n)
+    finite_near(gw, p(kept).t().contiguous() @ G, m)
+    finite_near(gb, G.sum(0), m)
+    (alone,) = torch.autograd.grad(op(leaves[0], w, b), leaves[:1], g)
+    assert torch.equal(torch.nan_to_num(alone), torch.nan_to_num(gx))
