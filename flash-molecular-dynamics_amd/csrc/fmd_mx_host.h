@@ -45,7 +45,7 @@ void mx_sum_parts(const float* parts, int64_t count, int64_t m, int64_t n, int d
 void mx_column_totals(const float* parts, int64_t count, int64_t cols, int dtype, void* out, hipStream_t s);
 void mx_column_sums(const MxSource& q, int64_t rows, int64_t cols, int64_t parts, float* out, hipStream_t s);
 
-// a layer of at most 128 x 128 in one pass over the rows (fmd_mx_layer.hip)
+// a layer of at most 256 x 256 in one pass over the rows (fmd_mx_layer.hip)
 enum { MX_WEIGHT_DENSE, MX_WEIGHT_FP4, MX_WEIGHT_FP4_BOTH, MX_WEIGHT_FP4_ACROSS };
 struct MxLayer {
   const void *in, *aux;

@@ -88,6 +88,8 @@ void sum_over_rows(MxArena& ar, bool run, const MxSource& q, int64_t m, int64_t 
   mx_column_totals(p, parts, n, dtype, out, s);
 }
 
+// The four calls below return the bytes of their workspace, or below zero the error of a launch that asked for it (which takes it
+// from the runtime: what is not handed on is lost).
 // ---- y = f(x^ W^T + b), W in 4-bit blocks -----------------------------------------------------------------------------
 struct Fp4Linear {
   const void *x, *codes, *scales;
@@ -101,13 +103,12 @@ int64_t fp4_forward(const Fp4Linear& c, void* base, bool run, hipStream_t s) {
   MxArena ar{(char*)base, 0};
   if (mx_layer_fits(c.k, c.n)) {
     if (run)
-      mx_layer({c.x, nullptr, MX_SRC_DENSE, c.codes, c.scales, c.both ? MX_WEIGHT_FP4_BOTH : MX_WEIGHT_FP4, 0, 0, nullptr, nullptr, false, c.e, nullptr, nullptr},
-               c.dtype, c.m, c.k, c.n, s);
+      return mx_layer({c.x, nullptr, MX_SRC_DENSE, c.codes, c.scales, c.both ? MX_WEIGHT_FP4_BOTH : MX_WEIGHT_FP4, 0, 0, nullptr, nullptr, false,
+                       c.e, nullptr, nullptr}, c.dtype, c.m, c.k, c.n, s);
     return 0;
   }
   if (mx_rows_fits(c.m)) {
-    if (run) mx_rows(c.x, c.dtype, c.codes, c.scales, c.both, c.m, c.n, c.k, c.e, s);
-    return 0;
+    return run ? mx_rows(c.x, c.dtype, c.codes, c.scales, c.both, c.m, c.n, c.k, c.e, s) : 0;
   }
   const int64_t nb = mx_blocks(c.k);
   if (c.both) {
@@ -118,7 +119,7 @@ int64_t fp4_forward(const Fp4Linear& c, void* base, bool run, hipStream_t s) {
     void* ws = ar.take(mx_up(c.n, 4) * kt * 8);
     float* parts = plan.splits > 1 ? (float*)ar.take(plan.splits * c.m * c.n * 4) : nullptr;
     if (run) {
-      mx_quantize4_for_product(c.x, c.dtype, c.m, c.k, xc, xs, s);
+      if (const int rc = mx_quantize4_for_product(c.x, c.dtype, c.m, c.k, xc, xs, s)) return rc;
       mx_scale_tiles(c.scales, c.n, nb, ws, s);
       mx_product({xc, 0, nb * 16, 1, xs, false}, {c.codes, 0, nb * 16, 1, ws, false}, c.m, c.n, kt, plan, c.dtype, c.e, parts, s);
       if (parts) mx_sum_parts(parts, plan.splits, c.m, c.n, c.dtype, c.e, s);
@@ -147,7 +148,7 @@ int64_t fp4_backward(const Fp4Backward& c, void* base, bool run, bool want_gx, b
   if (want_gx && mx_layer_fits(c.n, c.k)) {
     float* sums = want_gb ? (float*)ar.take(mx_layer_sums_bytes(c.m, c.n)) : nullptr;
     if (run)
-      mx_layer({c.g, c.aux, c.kind, c.codes, c.scales, MX_WEIGHT_FP4_ACROSS, 0, 0, nullptr, nullptr, false, to_gx, sums, c.gb}, c.dtype, c.m,
+      return mx_layer({c.g, c.aux, c.kind, c.codes, c.scales, MX_WEIGHT_FP4_ACROSS, 0, 0, nullptr, nullptr, false, to_gx, sums, c.gb}, c.dtype, c.m,
                c.n, c.k, s);
     return ar.used;
   } else if (want_gx) {
@@ -175,7 +176,7 @@ int64_t kept_forward(const Kept& c, void* base, bool run, hipStream_t s) {
   MxArena ar{(char*)base, 0};
   if (mx_layer_fits(c.k, c.n)) {
     if (run)
-      mx_layer({c.x, nullptr, c.tanh ? MX_SRC_TANH : MX_SRC_DENSE, c.w, nullptr, MX_WEIGHT_DENSE, c.n, 1, c.codes, c.scales, false, c.e, nullptr, nullptr},
+      return mx_layer({c.x, nullptr, c.tanh ? MX_SRC_TANH : MX_SRC_DENSE, c.w, nullptr, MX_WEIGHT_DENSE, c.n, 1, c.codes, c.scales, false, c.e, nullptr, nullptr},
                c.dtype, c.m, c.k, c.n, s);
     return 0;
   }
@@ -196,9 +197,12 @@ int64_t kept_backward(const Kept& c, void* base, bool run, bool want_gx, bool wa
   const MxSource g{MX_SRC_DENSE, c.dtype, c.g, nullptr, half};
   const bool narrow = mx_layer_fits(c.n, c.k);
   if (want_gx && narrow) {
-    if (run)
-      mx_layer({c.g, nullptr, MX_SRC_DENSE, c.w, nullptr, MX_WEIGHT_DENSE, 1, c.n, c.tanh ? c.codes : nullptr, c.tanh ? c.scales : nullptr, c.tanh,
-                {nullptr, c.gx, nullptr, nullptr, nullptr, 0, 0}, nullptr, nullptr}, c.dtype, c.m, c.n, c.k, s);
+    if (run) {
+      const int rc = mx_layer({c.g, nullptr, MX_SRC_DENSE, c.w, nullptr, MX_WEIGHT_DENSE, 1, c.n, c.tanh ? c.codes : nullptr,
+                               c.tanh ? c.scales : nullptr, c.tanh, {nullptr, c.gx, nullptr, nullptr, nullptr, 0, 0}, nullptr, nullptr},
+                              c.dtype, c.m, c.n, c.k, s);
+      if (rc) return rc;
+    }
   } else if (want_gx) {
     const int64_t pad = mx_up(c.n, 64);
     void* w = ar.take(p * c.k * pad * 2);
@@ -210,7 +214,7 @@ int64_t kept_backward(const Kept& c, void* base, bool run, bool want_gx, bool wa
   if ((want_gw || want_gb) && mx_gradient_fits(c.m, c.n, c.k)) {  // the bias's sums come along
     const int64_t bytes = mx_gradient_bytes(c.dtype, c.m, c.n, c.k);
     void* part = bytes ? ar.take(bytes) : nullptr;
-    if (run) mx_gradient(c.g, c.codes, c.scales, c.tanh, c.dtype, c.m, c.n, c.k, c.gw, c.gb, part, s);
+    if (run) return mx_gradient(c.g, c.codes, c.scales, c.tanh, c.dtype, c.m, c.n, c.k, c.gw, c.gb, part, s);
     return ar.used;
   }
   if (want_gw)
@@ -242,7 +246,7 @@ extern "C" int fmd_mxfp4_linear(const void* x, int dtype, const void* codes, con
   if (!x || !codes || !scales || !y || off16(x) || off16(codes) || off16(y) || off16(workspace) || (dact && !tanh)) return FMD_EINVAL;
   const Fp4Linear c{x, codes, scales, dtype, m, n, k, quantize_input != 0, {bias, y, dact, nullptr, nullptr, 0, tanh}};
   if (!workspace && fp4_forward(c, nullptr, false, nullptr)) return FMD_EINVAL;
-  fp4_forward(c, workspace, true, fmd_stream(stream));
+  if (const int64_t rc = fp4_forward(c, workspace, true, fmd_stream(stream)); rc < 0) return (int)rc;
   FMD_CHECK_LAUNCH();
   return FMD_OK;
 }
@@ -264,7 +268,7 @@ extern "C" int fmd_mxfp4_linear_bwd(const void* g, int dtype, const void* aux, i
   const int kind = aux_kind == FMD_AUX_Y ? MX_SRC_GRAD_Y : aux_kind == FMD_AUX_DACT ? MX_SRC_GRAD_D : MX_SRC_DENSE;
   const Fp4Backward c{g, aux, codes, scales, gx, gbias, dtype, kind, m, n, k};
   if (!workspace && fp4_backward(c, nullptr, false, gx && m, gbias, nullptr)) return FMD_EINVAL;
-  fp4_backward(c, workspace, true, gx && m, gbias, fmd_stream(stream));
+  if (const int64_t rc = fp4_backward(c, workspace, true, gx && m, gbias, fmd_stream(stream)); rc < 0) return (int)rc;
   FMD_CHECK_LAUNCH();
   return FMD_OK;
 }
@@ -286,7 +290,7 @@ extern "C" int fmd_linear_ckpt8(const void* x, int dtype, const void* w, const v
   c.x = x, c.w = w, c.codes = (uint8_t*)codes, c.scales = (uint8_t*)scales, c.dtype = dtype, c.m = m, c.n = n, c.k = k, c.tanh = tanh != 0;
   c.e = {bias, y, nullptr, nullptr, nullptr, 0, 0};
   if (!workspace && kept_forward(c, nullptr, false, nullptr)) return FMD_EINVAL;
-  kept_forward(c, workspace, true, fmd_stream(stream));
+  if (const int64_t rc = kept_forward(c, workspace, true, fmd_stream(stream)); rc < 0) return (int)rc;
   FMD_CHECK_LAUNCH();
   return FMD_OK;
 }
@@ -311,7 +315,7 @@ extern "C" int fmd_linear_ckpt8_bwd(const void* g, int dtype, const void* codes,
   c.g = g, c.w = w, c.codes = (uint8_t*)codes, c.scales = (uint8_t*)scales, c.gx = gx, c.gw = gw, c.gb = gbias;
   c.dtype = dtype, c.m = m, c.n = n, c.k = k, c.tanh = tanh != 0;
   if (!workspace && kept_backward(c, nullptr, false, gx, gw, gbias, nullptr)) return FMD_EINVAL;
-  kept_backward(c, workspace, true, gx, gw, gbias, fmd_stream(stream));
+  if (const int64_t rc = kept_backward(c, workspace, true, gx, gw, gbias, fmd_stream(stream)); rc < 0) return (int)rc;
   FMD_CHECK_LAUNCH();
   return FMD_OK;
 }

@@ -89,6 +89,28 @@ def test_c_entries_refuse_bad_arguments():
     assert lib.fmd_linear_ckpt8_bwd_workspace_bytes(0, 4, 8, -2, 0, 1, 1, 1) == BAD
 
 
+@pytest.mark.skipif(torch.cuda.is_available(), reason="the addresses are not a GPU's: only where every launch fails")
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+def test_a_failed_launch_is_reported(dtype):
+    """Where no kernel can be launched, no path of an entry point may answer that it went well."""
+    from flashmd_amd import _ffi
+
+    lib, p, FAILED = _ffi.lib(), ctypes.c_void_p(1 << 20), -2
+    for m, n, k in ((40, 64, 64), (40, 300, 300), (5000, 64, 64), (100000, 64, 64), (500, 300, 300), (5000, 300, 300)):
+        for both in (0, 1):
+            assert lib.fmd_mxfp4_linear(p, dtype, p, p, p, p, None, m, n, k, 0, both, p, None) == FAILED
+        for gx, gb in ((p, None), (None, p), (p, p)):
+            assert lib.fmd_mxfp4_linear_bwd(p, dtype, None, 0, p, p, gx, gb, m, n, k, p, None) == FAILED
+        for tanh in (0, 1):
+            assert lib.fmd_linear_ckpt8(p, dtype, p, p, p, p, p, m, n, k, tanh, p, None) == FAILED
+            for gx, gw, gb in ((p, None, None), (None, p, None), (None, None, p), (p, p, p)):
+                assert lib.fmd_linear_ckpt8_bwd(p, dtype, p, p, p, gx, gw, gb, m, n, k, tanh, p, None) == FAILED
+    for f in (lib.fmd_mxfp4_quantize, lib.fmd_mxint8_quantize):
+        assert f(p, dtype, 4, 40, p, p, None) == FAILED
+    for f in (lib.fmd_mxfp4_dequantize, lib.fmd_mxint8_dequantize):
+        assert f(p, p, 4, 40, p, dtype, None) == FAILED
+
+
 def test_workspaces_do_not_grow_with_the_rows():
     """Large batches go through the wide path in chunks: what the planes of one take, not of all."""
     from flashmd_amd import _ffi
