@@ -17,7 +17,7 @@
 namespace {
 
 constexpr int WAVES = 4;
-constexpr uint32_t NOWHERE = 0x40000000u;  // behind the end of every descriptor: 16 rows of at most 2^24 fp32
+constexpr uint32_t NOWHERE = 0x40000000u;  // behind the end of every descriptor: 16 rows of at most 2^20 fp32 are 2^26 bytes
 typedef __amdgpu_buffer_rsrc_t Rows;
 
 struct GradArgs {

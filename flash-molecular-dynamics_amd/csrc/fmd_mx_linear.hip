@@ -224,16 +224,19 @@ int64_t kept_backward(const Kept& c, void* base, bool run, bool want_gx, bool wa
   return ar.used;
 }
 
-bool bad_sizes(int dtype, int64_t m, int64_t n, int64_t k) {
-  // rows of a product are counted in 32 bits within a chunk, and a weight in all
-  return dtype < 0 || dtype > 2 || m < 0 || n < 1 || k < 1 || m > (int64_t)1 << 34 || n > 1 << 24 || k > 1 << 24;
+// Up to 2^20 a side of a weight (grids of 64 and 32 columns count in 16 bits), 2^34 rows (steps of 16 count in 32) and 2^38 elements
+// a matrix (at most 2^22 + 2^21 tiles of a product: fewer than 2^32 threads); the rows of a 4-bit x go through one product.
+bool bad_sizes(int dtype, int64_t m, int64_t n, int64_t k, bool both = false) {
+  const int64_t side = (int64_t)1 << 20, most = (int64_t)1 << 38;
+  return dtype < 0 || dtype > 2 || m < 0 || n < 1 || k < 1 || m > (int64_t)1 << (both ? 29 : 34) || n > side || k > side ||
+         m * n > most || m * k > most || n * k > most;
 }
 bool off16(const void* p) { return ((uintptr_t)p & 15) != 0; }
 
 }  // namespace
 
 extern "C" int64_t fmd_mxfp4_linear_workspace_bytes(int dtype, int64_t m, int64_t n, int64_t k, int quantize_input) {
-  if (bad_sizes(dtype, m, n, k)) return FMD_EINVAL;
+  if (bad_sizes(dtype, m, n, k, quantize_input != 0)) return FMD_EINVAL;
   if (m == 0) return 0;
   Fp4Linear c{nullptr, nullptr, nullptr, dtype, m, n, k, quantize_input != 0, {}};
   return fp4_forward(c, nullptr, false, nullptr);
@@ -241,7 +244,7 @@ extern "C" int64_t fmd_mxfp4_linear_workspace_bytes(int dtype, int64_t m, int64_
 
 extern "C" int fmd_mxfp4_linear(const void* x, int dtype, const void* codes, const void* scales, const void* bias, void* y, void* dact,
                                 int64_t m, int64_t n, int64_t k, int tanh, int quantize_input, void* workspace, void* stream) {
-  if (bad_sizes(dtype, m, n, k) || (quantize_input && m > INT32_MAX)) return FMD_EINVAL;
+  if (bad_sizes(dtype, m, n, k, quantize_input != 0)) return FMD_EINVAL;
   if (m == 0) return FMD_OK;
   if (!x || !codes || !scales || !y || off16(x) || off16(codes) || off16(y) || off16(workspace) || (dact && !tanh)) return FMD_EINVAL;
   const Fp4Linear c{x, codes, scales, dtype, m, n, k, quantize_input != 0, {bias, y, dact, nullptr, nullptr, 0, tanh}};

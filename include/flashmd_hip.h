@@ -192,6 +192,8 @@ int fmd_matmul_f32_f16_to_f16(const float* a, const void* b, void* c, int64_t m,
  *        8-bit blocks
  *   fmd_linear_ckpt8_bwd  from those: gx = (g W^T) p'(x8), gw[k,n] = p(x8)^T g, gbias = sum g; each may be NULL; m >= 1
  *   *_workspace_bytes     0: none is needed and NULL will do; negative: FMD_EINVAL
+ *   The layers take up to 2^20 inputs and outputs, 2^34 rows (2^29 with quantize_input) and 2^38 elements a matrix, else
+ *   FMD_EINVAL.
  * ------------------------------------------------------------------------------------------- */
 #define FMD_F32 0
 #define FMD_F16 1

@@ -111,6 +111,27 @@ def test_a_failed_launch_is_reported(dtype):
         assert f(p, p, 4, 40, p, dtype, None) == FAILED
 
 
+def test_sizes_beyond_the_grids_are_refused():
+    """A dimension of a weight past 2^20, rows past 2^34, 4-bit rows past 2^29, or a matrix past 2^38 elements: refused before a
+    grid or an index could wrap."""
+    from flashmd_amd import _ffi
+
+    lib, p, BAD, top = _ffi.lib(), ctypes.c_void_p(1 << 20), -1, 1 << 20
+    for m, n, k in ((4, top + 1, 8), (4, 8, top + 1), ((1 << 34) + 1, 8, 8), (1 << 30, 257, 8), (1 << 30, 8, 257), (4, top, (1 << 18) + 1)):
+        assert lib.fmd_mxfp4_linear_workspace_bytes(0, m, n, k, 0) == BAD
+        assert lib.fmd_mxfp4_linear(p, 0, p, p, None, p, None, m, n, k, 0, 0, p, None) == BAD
+        assert lib.fmd_mxfp4_linear_bwd_workspace_bytes(0, m, n, k, 1, 1) == BAD
+        assert lib.fmd_mxfp4_linear_bwd(p, 0, None, 0, p, p, p, p, m, n, k, p, None) == BAD
+        assert lib.fmd_linear_ckpt8_workspace_bytes(0, m, n, k) == BAD
+        assert lib.fmd_linear_ckpt8(p, 0, p, None, p, p, p, m, n, k, 0, p, None) == BAD
+        assert lib.fmd_linear_ckpt8_bwd_workspace_bytes(0, m, n, k, 0, 1, 1, 1) == BAD
+        assert lib.fmd_linear_ckpt8_bwd(p, 0, p, p, p, p, p, p, m, n, k, 0, p, None) == BAD
+    for n, k in ((8, 8), (8, 300)):
+        assert lib.fmd_mxfp4_linear_workspace_bytes(0, (1 << 29) + 1, n, k, 1) == BAD
+        assert lib.fmd_mxfp4_linear(p, 0, p, p, None, p, None, (1 << 29) + 1, n, k, 0, 1, p, None) == BAD
+    assert lib.fmd_mxfp4_linear_workspace_bytes(0, 65, top, 300, 0) > 0 and lib.fmd_mxfp4_linear_workspace_bytes(0, 1 << 29, 8, 300, 1) > 0
+
+
 def test_workspaces_do_not_grow_with_the_rows():
     """Large batches go through the wide path in chunks: what the planes of one take, not of all."""
     from flashmd_amd import _ffi
