@@ -246,7 +246,7 @@ extern "C" int fmd_mxfp4_linear(const void* x, int dtype, const void* codes, con
                                 int64_t m, int64_t n, int64_t k, int tanh, int quantize_input, void* workspace, void* stream) {
   if (bad_sizes(dtype, m, n, k, quantize_input != 0)) return FMD_EINVAL;
   if (m == 0) return FMD_OK;
-  if (!x || !codes || !scales || !y || off16(x) || off16(codes) || off16(y) || off16(workspace) || (dact && !tanh)) return FMD_EINVAL;
+  if (!x || !codes || !scales || !y || off16(x) || off16(codes) || off16(y) || off16(workspace) || off16(dact) || (dact && !tanh)) return FMD_EINVAL;
   const Fp4Linear c{x, codes, scales, dtype, m, n, k, quantize_input != 0, {bias, y, dact, nullptr, nullptr, 0, tanh}};
   if (!workspace && fp4_forward(c, nullptr, false, nullptr)) return FMD_EINVAL;
   if (const int64_t rc = fp4_forward(c, workspace, true, fmd_stream(stream)); rc < 0) return (int)rc;
@@ -312,7 +312,7 @@ extern "C" int fmd_linear_ckpt8_bwd(const void* g, int dtype, const void* codes,
   if (bad_sizes(dtype, m, n, k) || m == 0) return FMD_EINVAL;
   if (!gx && !gw && !gbias) return FMD_OK;
   const bool kept = gw || (gx && tanh);
-  if (!g || off16(g) || off16(workspace) || (gx && (!w || off16(w) || off16(gx))) || (kept && (!codes || !scales || off16(codes))))
+  if (!g || off16(g) || off16(workspace) || off16(gw) || (gx && (!w || off16(w) || off16(gx))) || (kept && (!codes || !scales || off16(codes))))
     return FMD_EINVAL;
   Kept c{};
   c.g = g, c.w = w, c.codes = (uint8_t*)codes, c.scales = (uint8_t*)scales, c.gx = gx, c.gw = gw, c.gb = gbias;

@@ -176,8 +176,8 @@ int fmd_matmul_f32_f16_to_f16(const float* a, const void* b, void* c, int64_t m,
  *   8 bits: codes [m][32 nb] int8 in [-127,127], byte = max(floor(log2 amax), -127) + 127, value = code / 64 * 2^(byte-127);
  *           nearest even
  *   A block that holds an Inf or a NaN has byte 255, codes 0 and stands for NaN.
- * dtype: FMD_F32 | FMD_F16 | FMD_BF16 of every dense tensor of a call.  Device pointers of dense tensors, codes and
- * workspaces are 16-byte aligned, else FMD_EINVAL; m = 0 is a call that does nothing.  Sums are held in fp32.  Results do
+ * dtype: FMD_F32 | FMD_F16 | FMD_BF16 of every dense tensor of a call.  Device pointers of matrices, codes and
+ * workspaces are 16-byte aligned, else FMD_EINVAL (bias, gbias: to their elements); m = 0 is a call that does nothing.  Sums are held in fp32.  Results do
  * not depend on timing (no atomics).  A value that is not finite makes what is computed from it not finite (Inf may
  * become NaN).
  *

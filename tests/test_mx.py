@@ -132,6 +132,15 @@ def test_sizes_beyond_the_grids_are_refused():
     assert lib.fmd_mxfp4_linear_workspace_bytes(0, 65, top, 300, 0) > 0 and lib.fmd_mxfp4_linear_workspace_bytes(0, 1 << 29, 8, 300, 1) > 0
 
 
+def test_misaligned_results_are_refused():
+    from flashmd_amd import _ffi
+
+    lib, p, odd, BAD = _ffi.lib(), ctypes.c_void_p(1 << 20), ctypes.c_void_p((1 << 20) + 2), -1
+    for m, n, k in ((4, 8, 32), (5000, 300, 300)):
+        assert lib.fmd_mxfp4_linear(p, 1, p, p, None, p, odd, m, n, k, 1, 0, p, None) == BAD     # dact
+        assert lib.fmd_linear_ckpt8_bwd(p, 1, p, p, p, None, odd, None, m, n, k, 0, p, None) == BAD  # gw
+
+
 def test_workspaces_do_not_grow_with_the_rows():
     """Large batches go through the wide path in chunks: what the planes of one take, not of all."""
     from flashmd_amd import _ffi
