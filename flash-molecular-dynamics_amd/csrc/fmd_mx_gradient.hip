@@ -1,15 +1,18 @@
 // Weight and bias gradients: gw[k,n] = sum over rows p(x8)[.,k] g[.,n], gb[n] = sum g[.,n], x8 in 8-bit blocks.
 //
-// gradient_kernel, for narrow layers (k and n at most 256, in parts of 128 x 128) over many rows.  The contraction runs over the rows, so a matrix fragment wants 8 rows of one column in a lane.  Lane i of a half wave takes
-// columns NT*i .. NT*i+NT-1 of g (one 16-byte load a row) and KT*i .. of the checkpoint; over 8 rows that is one fragment for each
-// of its columns, with no transposition through LDS: which matrix column a lane stands for is free, and the result is stored
-// back in the same order.  A wave holds all of gw in its accumulators (up to 128 x 128: 256 of a lane's 512 registers, one wave a
-// SIMD) and takes 16 rows a step, the next step's rows already on their way.  The waves of a workgroup add up in LDS, the
-// workgroups in a second kernel, in a fixed order.  Bound by reading g and the checkpoint once.
+// gradient_kernel, for narrow layers (k and n at most 256, in parts of 128 x 128) over many rows.  The contraction runs over the
+// rows, so a matrix fragment wants 8 rows of one column in a lane.  Lane i of a half wave takes columns NT*i .. NT*i+NT-1 of g (one
+// 16-byte load a row) and KT*i .. of the checkpoint; over 8 rows that is one fragment for each of its columns, with no
+// transposition through LDS: which matrix column a lane stands for is free, and the result is stored back in the same order.  A
+// wave holds all of gw in its accumulators (up to 128 x 128: 256 of a lane's 512 registers, one wave a SIMD) and takes 16 rows a
+// step, the next step's rows already on their way.  The waves of a workgroup add up in LDS, the workgroups in a second kernel, in a
+// fixed order.  Bound by reading g and the checkpoint once: 262144 x 128 x 128 fp32 under tanh in 116 us, 1.5 TB/s (the 6 products of
+// a term and the tanh come on top of the bytes), bf16 84 us.
 //
 // gradient_tile_kernel, for few rows and any width.  A workgroup makes one 32 x 32 tile of gw from a slice of the rows; its eight
 // waves take 16 rows each in turn.  g and the checkpoint are read once for every tile beside or below, from the caches, but a
-// few rows spread over many workgroups, and a workgroup has 16 sums a lane to bring together instead of 256.
+// few rows spread over many workgroups, and a workgroup has 16 sums a lane to bring together instead of 256.  Bound by latency while
+// the rows are few (269 x 128 x 128 fp32: 5.8 us), by those reads later.
 #include <type_traits>
 
 #include "fmd_mx_host.h"
@@ -323,12 +326,19 @@ int slices_for(int dtype, int64_t m, int64_t k) {
   return (int)(s < most ? s : most);
 }
 
-// Which kernel: a tile at a time while the rows are few.  (Both measured at 128 x 128, fp32, tanh: see FEW.)
-constexpr int64_t FEW = 65536, FEW_WIDE = 256;
-bool by_tiles(int64_t m, int64_t n, int64_t k) { return m <= (k <= 256 && n <= 256 ? FEW : FEW_WIDE); }
+// Which kernel: a tile at a time while the rows are few; it reads a narrow layer's rows once for each 32 columns of the other side,
+// the parts' kernel once for each 128, and general products write both operands anew.  Tiles against the other, us, tanh, with sums:
+//   narrow: 1000 x 128 x 128 fp32 8.0 / 50, 65536 fp32 49 / 70, 98304 66 / 77 (bf16 54 / 64), 131072 85 / 85 (bf16 70 / 68), 262144
+//           158 / 116; 98304 x 256 x 200 264 / 305, x 64 x 256 64 / 60
+//   wide:   500 x 1000 x 1000 fp32 24 / 41 (bf16 16 / 29), 1000 42 / 48 (28 / 35), 2000 78 / 62 (52 / 40); 64 x 1024 x 4096 bf16 15 / 16,
+//           128 19 / 17, 300 34 / 21; 5000 x 300 x 300 31 / 59
+constexpr int64_t FEW = 98304, FEW_PRODUCTS = (int64_t)1 << 29;
+bool by_tiles(int64_t m, int64_t n, int64_t k) { return k <= 256 && n <= 256 ? m <= FEW : m * n <= FEW_PRODUCTS / k; }
+// Rows in parts: two steps of 16 for each wave at least, and none up to 512 rows, where the sum over parts is a launch too many (400 x
+// 128 x 128 fp32: 7.1 in one, 7.9 in two; 1000: 13.6 in one, 8.0 in four)
 int tile_slices(int64_t m, int64_t n, int64_t k) {
   const int64_t tiles = ((k + 31) / 32) * ((n + 31) / 32), s = (m + 32 * TILE_WAVES - 1) / (32 * TILE_WAVES), most = (512 + tiles - 1) / tiles;
-  return (int)(m <= 1024 ? 1 : s < most ? s : most);  // two steps for each wave at least
+  return (int)(m <= 512 ? 1 : s < most ? s : most);
 }
 
 template <class T>

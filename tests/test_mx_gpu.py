@@ -552,3 +552,43 @@ def test_both_gradients_of_many_rows(K, k, n, tanh, dtype):
     finite_near(gb, G.sum(0), m)
     (alone,) = torch.autograd.grad(op(leaves[0], w, b), leaves[:1], g)
     assert torch.equal(torch.nan_to_num(alone), torch.nan_to_num(gx))
+
+
+def near_where_finite(got, want, terms):
+    """An uneven value may be beyond fp16: its block stands for NaN, and what comes of it is not finite in the reference either."""
+    fine = torch.isfinite(want)
+    assert torch.equal(torch.isfinite(got).cpu(), fine)
+    near(got.cpu()[fine], want[fine], terms)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("tanh", [False, True])
+@pytest.mark.parametrize("m,k,n", [(512, 128, 128), (513, 128, 128), (700, 33, 65), (1000, 64, 50), (1025, 7, 30), (500, 300, 300), (513, 300, 257),
+                                   (900, 1000, 40), (600, 257, 1), (5000, 300, 300), (6000, 301, 299), (12000, 299, 150), (512, 1024, 1024),
+                                   (513, 1024, 1024)])
+def test_gradient_of_middling_rows(K, m, k, n, tanh, dtype):
+    """Both sides of where the weight gradient takes its rows in parts, and of where it leaves the tiles for the general product."""
+    x, w = uneven(m, k, dtype, seed=m + n), rand(k, n, seed=n, scale=(2.0 / (k + n)) ** 0.5, dtype=dtype)
+    bias, g = rand(n, seed=2, dtype=dtype), rand(m, n, seed=3, scale=1e-2, dtype=dtype)
+    _, _, gw_ref, gb_ref = mo.linear_ckpt8(x, w, bias, tanh, g)
+    leaves = [t.to(DEV).requires_grad_() for t in (x, w, bias)]
+    y = (K.fused_tanh_linear_ckpt8_autograd if tanh else K.linear_ckpt8_autograd)(*leaves)
+    gw, gb = torch.autograd.grad(y, leaves[1:], g.to(DEV))
+    near_where_finite(gw, gw_ref, m)
+    near_where_finite(gb, gb_ref, m)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m,k,n", [(98304, 64, 33), (98305, 64, 33), (98305, 50, 128), (98320, 64, 64), (98305, 128, 128), (100001, 33, 127),
+                                   (98311, 200, 150), (98310, 129, 30), (98305, 7, 200), (99000, 256, 256)])
+def test_gradient_of_many_rows(K, m, k, n, dtype):
+    """Both sides of where a narrow layer's weight gradient leaves the tiles; against the oracle, and the same bits twice."""
+    x, w = uneven(m, k, dtype, seed=k), rand(k, n, seed=n, scale=(2.0 / (k + n)) ** 0.5, dtype=dtype)
+    bias, g = rand(n, seed=2, dtype=dtype), rand(m, n, seed=3, scale=1e-2, dtype=dtype)
+    _, _, gw_ref, gb_ref = mo.linear_ckpt8(x, w, bias, True, g)
+    leaves = [t.to(DEV).requires_grad_() for t in (x, w, bias)]
+    first = torch.autograd.grad(K.fused_tanh_linear_ckpt8_autograd(*leaves), leaves[1:], g.to(DEV))
+    near_where_finite(first[0], gw_ref, m)
+    near_where_finite(first[1], gb_ref, m)
+    again = torch.autograd.grad(K.fused_tanh_linear_ckpt8_autograd(*leaves), leaves[1:], g.to(DEV))
+    assert all(torch.equal(torch.nan_to_num(a), torch.nan_to_num(b)) for a, b in zip(first, again))
