@@ -277,7 +277,8 @@ typedef __fp16 hv2 __attribute__((ext_vector_type(2)));
 // younger; plain v_fma_f32 / v_cvt_pkrtz / v_fma_mix / transcendentals overlap within ~15 %).  In the pair kernels
 // the two waves of a SIMD are one producer and one consumer whose VALU phases are meant to run under each other's
 // MFMA bursts, so they use the scalar pair type (FMD_SCALAR_PAIRS, set by their translation units, which are also
-// compiled with -fno-slp-vectorize); the node kernels run one wave per SIMD and keep the packed form.
+// compiled with -fno-slp-vectorize); the node and W16A16 kernels keep pairs as vectors.  The whole library is built without packed
+// fp32 instructions (Makefile), so that both types now come to scalar ones.
 #ifdef FMD_SCALAR_PAIRS
 struct f32x2 {
   float x, y;

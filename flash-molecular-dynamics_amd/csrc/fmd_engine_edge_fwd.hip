@@ -5,7 +5,8 @@
 // This file is compiled twice: as itself it holds the fp32-grade kernels, whose pair arithmetic is SCALAR
 // (FMD_SCALAR_PAIRS, fmd_engine.h: packed fp32 cannot issue beside the partner wave's MFMAs, and these kernels are three
 // MFMAs per product); fmd_engine_edge_fwd_half.hip includes it with FMD_HALF_TU set and holds the W16A16 kernels, one
-// MFMA per product, which are faster with the PACKED pair type (same-box A/B, profiles/r05_ab_packed_half.txt).
+// MFMA per product, with pairs as vectors of two floats (faster as long as packed instructions were allowed: same-box A/B,
+// profiles/r05_ab_packed_half.txt; the library is built without them, see the Makefile).
 #ifndef FMD_HALF_TU
 #define FMD_SCALAR_PAIRS 1
 #endif

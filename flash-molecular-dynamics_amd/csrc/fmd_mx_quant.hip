@@ -1,14 +1,15 @@
 // Block quantisation along the rows and back (formats: fmd_mx.h).
 //
 // A thread holds 8 columns, four neighbouring lanes a block of 32: the block's largest magnitude is an unsigned maximum of
-// the bit patterns over the four lanes.  One pass: read x once, write codes and scales once.  Bound by memory.
+// the bit patterns over the four lanes.  One pass: read x once, write codes and scales once.  Bound by memory:
+// 8192 x 8192 bf16 in 4 bits in 33 us, 5.1 TB/s, back in 29 us, 5.9 TB/s (a large copy runs at 5.0).
 #include "fmd_mx.h"
 
 namespace {
 
 // Rows whose length is no multiple of 16 bytes: a workgroup moves ROWS whole rows, which are (32 rows, any length) a multiple of
 // 16 bytes of memory, in 16-byte pieces through LDS and takes its columns from there.  (1882048 x 50 fp32 in 4 bits, quantising /
-// back to bf16: 121 / 125 us with single values from memory.)
+// back to bf16: 121 / 125 us with single values from memory, 97 / 64 us like this: 4.5 / 4.0 TB/s.)
 constexpr int ROWS = 32, STAGE = 32 * 1024;  // most LDS of a workgroup; it asks for what its rows take
 
 template <class T>
