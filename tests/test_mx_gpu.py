@@ -592,3 +592,10 @@ def test_gradient_of_many_rows(K, m, k, n, dtype):
     near_where_finite(first[1], gb_ref, m)
     again = torch.autograd.grad(K.fused_tanh_linear_ckpt8_autograd(*leaves), leaves[1:], g.to(DEV))
     assert all(torch.equal(torch.nan_to_num(a), torch.nan_to_num(b)) for a, b in zip(first, again))
+
+
+@pytest.mark.parametrize("m,k,n", [(98400, 50, 128), (98400, 130, 64), (700, 300, 300)])
+def test_streams_and_graphs_beside_the_boundaries(K, m, k, n):
+    """The weight gradient over parts of many rows, and the tiles of a wide layer, repeated, on two streams and in a graph."""
+    test_repeats_and_other_streams(K, m, k, n)
+    test_captured_and_replayed(K, m, k, n)
