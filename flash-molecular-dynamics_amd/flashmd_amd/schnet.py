@@ -112,7 +112,7 @@ class MLP(torch.nn.Module):
             init_xavier_uniform(layer)
 
     def forward(self, x, data=None):
-        if self.checkpoint_bits == 8:
+        if self.checkpoint_bits == 8 and self.training:
             # Linear, then (tanh, Linear) pairs: each keeps its input for the backward pass in 8-bit blocks
             for i, linear in enumerate(self.layers[0::2]):
                 op = K.fused_tanh_linear_ckpt8_autograd if i else K.linear_ckpt8_autograd
@@ -210,7 +210,7 @@ class InteractionBlock(torch.nn.Module):
 
     def forward(self, x, edge_index, edge_weight, edge_attr, *args, csr_data: dict = None):
         x = self.conv(x, edge_index, edge_weight, edge_attr, csr_data=csr_data)
-        if self.checkpoint_bits == 8:
+        if self.checkpoint_bits == 8 and self.training:
             return K.fused_tanh_linear_ckpt8_autograd(x.contiguous(), self.lin.weight.t().contiguous(), self.lin.bias)
         if self.use_fused_tanh_linear:  # reference :534-541
             _need_gpu(x, "InteractionBlock")
@@ -339,9 +339,10 @@ def set_activation_checkpoints(model: torch.nn.Module, bits: Optional[int] = 8) 
     """Training with 8-bit activation checkpoints: the MLPs (filter and output networks) and the interaction blocks' output
     layers of ``model`` keep their layers' inputs for the backward pass in 8-bit blocks (33 bytes for 32 values) instead of
     in full; ``bits=None`` goes back.  Forward results are those of the layers without checkpoints up to fp32 rounding; the
-    weights' gradients, and the gradients that pass a tanh, come from the rounded values.  Parameters and their names stay as
-    they are.  Not in the reference.  Works on the operator path; the fused engine, which computes forces and nothing for
-    training, is not concerned.  W16A16 and MXFP4 networks are left alone."""
+    weights' gradients, and the gradients that pass a tanh, come from the rounded values.  A module in ``eval()`` runs its layers
+    as if nothing were set, so that the forces of an evaluation are the exact gradient of its energy on every path.  Parameters
+    and their names stay as they are.  Not in the reference.  Works on the operator path; the fused engine, which computes
+    forces and nothing for training, is not concerned.  W16A16 and MXFP4 networks are left alone."""
     if bits not in (8, None):
         raise ValueError(f"activation checkpoints in {bits} bits are not built: 8 or None")
     found = [m for m in model.modules() if isinstance(m, (MLP, InteractionBlock))]

@@ -179,6 +179,21 @@ def test_activation_checkpoints_setting():
     assert all(m.checkpoint_bits is None for m in other.modules() if isinstance(m, (S.MLP, S.InteractionBlock)))
 
 
+def test_activation_checkpoints_are_for_training_alone():
+    """In eval() the layers run as they are: on the CPU with plain torch, where the checkpointed ones would refuse."""
+    import flashmd_amd.schnet as S
+
+    model, x = _model(), torch.randn(5, 16)
+    nets = (model.output_network, model.interaction_blocks[0].conv.filter_network)
+    want = [net(x if net is model.output_network else x.repeat(1, 2)[:, :20]) for net in nets]
+    S.set_activation_checkpoints(model).eval()
+    got = [net(x if net is model.output_network else x.repeat(1, 2)[:, :20]) for net in nets]
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+    model.train()
+    with pytest.raises(RuntimeError, match="GPU"):
+        model.output_network(x)
+
+
 def test_mxfp4_swap_refusals():
     from flashmd_amd.mxfp4 import MXFP4MLP, apply_mxfp4_to_model
 

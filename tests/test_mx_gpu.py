@@ -599,3 +599,24 @@ def test_streams_and_graphs_beside_the_boundaries(K, m, k, n):
     """The weight gradient over parts of many rows, and the tiles of a wide layer, repeated, on two streams and in a graph."""
     test_repeats_and_other_streams(K, m, k, n)
     test_captured_and_replayed(K, m, k, n)
+
+
+def test_forces_of_an_evaluation_do_not_go_through_checkpoints(monkeypatch):
+    """Operator path, eval(): energies and forces with the setting on are those without it, and the 64-bit model's within the operator
+    path's fp32 budget of 1e-5; through 8-bit values they are off by about 1e-2."""
+    import copy
+
+    import flashmd_amd.schnet as S
+
+    monkeypatch.setattr(S, "USE_FUSED_ENGINE", False)
+    model = _schnet().to(DEV).eval()
+    _, f_ref, _ = _plain_run(copy.deepcopy(model).cpu().double(), S)
+    want = S.GradientsOut(model)(_batch(S)).out["SchNet"]
+    got = S.GradientsOut(S.set_activation_checkpoints(model)).eval()(_batch(S)).out["SchNet"]
+    assert rel(got["forces"], f_ref) < 1e-5
+    assert rel(got["energy"], want["energy"]) < 1e-5 and rel(got["forces"], want["forces"]) < 1e-5
+    model.train()                                             # and in training they do
+    data = _batch(S)
+    data.pos.requires_grad_(True)
+    rounded = -torch.autograd.grad(model(data).out["SchNet"]["energy"].sum(), data.pos)[0]
+    assert rel(rounded, f_ref) > 1e-4
