@@ -99,6 +99,8 @@ class GaussianBasis(torch.nn.Module):
 class MLP(torch.nn.Module):
     """reference models/mlp.py:6-57"""
 
+    checkpoint_bits = None  # set_activation_checkpoints; the class's, so that modules pickled before it existed have it, too
+
     def __init__(self, layer_widths: List[int], activation_func=None, last_bias: bool = True):
         super().__init__()
         activation_func = activation_func or torch.nn.Tanh()
@@ -107,7 +109,6 @@ class MLP(torch.nn.Module):
             layers += [torch.nn.Linear(w_in, w_out, bias=True), activation_func]
         layers.append(torch.nn.Linear(layer_widths[-2], layer_widths[-1], bias=last_bias))
         self.layers = torch.nn.Sequential(*layers)
-        self.checkpoint_bits = None  # set_activation_checkpoints
         for layer in self.layers:
             init_xavier_uniform(layer)
 
@@ -199,13 +200,14 @@ class CFConv(torch.nn.Module):
 class InteractionBlock(torch.nn.Module):
     """reference models/schnet.py:453-548"""
 
+    checkpoint_bits = None  # as in MLP
+
     def __init__(self, cfconv_layer, hidden_channels=128, activation=None):
         super().__init__()
         self.conv = cfconv_layer
         self.activation = activation or torch.nn.Tanh()
         self.lin = torch.nn.Linear(hidden_channels, hidden_channels)
         self.use_fused_tanh_linear = USE_FUSED_TANH_LINEAR and isinstance(self.activation, torch.nn.Tanh)
-        self.checkpoint_bits = None  # set_activation_checkpoints
         init_xavier_uniform(self.lin)
 
     def forward(self, x, edge_index, edge_weight, edge_attr, *args, csr_data: dict = None):

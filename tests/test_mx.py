@@ -194,6 +194,26 @@ def test_activation_checkpoints_are_for_training_alone():
         model.output_network(x)
 
 
+def test_modules_pickled_before_the_setting_existed():
+    """A whole module from an older pickle has no ``checkpoint_bits`` of its own: it runs as it did, and takes the setting."""
+    import io
+
+    import flashmd_amd.schnet as S
+
+    model = _model().eval()
+    for m in model.modules():
+        m.__dict__.pop("checkpoint_bits", None)               # what an older version wrote
+    f = io.BytesIO()
+    torch.save(model, f)
+    f.seek(0)
+    old = torch.load(f, weights_only=False)
+    x = torch.randn(3, 16)
+    assert torch.equal(old.output_network(x), model.output_network(x))
+    S.set_activation_checkpoints(old)
+    assert sum(m.checkpoint_bits == 8 for m in old.modules() if isinstance(m, (S.MLP, S.InteractionBlock))) == 5
+    assert S.MLP.checkpoint_bits is None and S.InteractionBlock.checkpoint_bits is None
+
+
 def test_mxfp4_swap_refusals():
     from flashmd_amd.mxfp4 import MXFP4MLP, apply_mxfp4_to_model
 
