@@ -8,7 +8,8 @@
 
 Not part of the reference's surface (its narrowest format is fp16, reference models/gptq.py); conventions are those of
 ``flashmd_amd.kernels``: contiguous GPU tensors, HIP kernels on torch's current stream, fresh outputs, no CPU fallback.
-Dense tensors are float32, float16 or bfloat16, one type within a call.  The gradients are not differentiable again.
+Dense tensors are float32, float16 or bfloat16, one type within a call.  The gradients are not differentiable again: what tries,
+such as a loss on forces taken with ``create_graph=True``, gets a RuntimeError.
 """
 from __future__ import annotations
 
@@ -16,7 +17,6 @@ import functools
 from typing import Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _ffi
 
@@ -138,6 +138,38 @@ def mxint8_dequantize(codes, scales, num_columns: int, dtype: torch.dtype = torc
     return _dequantize("fmd_mxint8_dequantize", codes, scales, num_columns, dtype, BLOCK, torch.int8)
 
 
+class _NotTwice(torch.autograd.Function):
+    """Stands between a layer's gradients and everything they depend on, and raises when they are to be differentiated."""
+
+    @staticmethod
+    def forward(ctx, anchor, grad_output, *gradients):
+        return gradients
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError("flashmd_amd: the gradients of block-scaled layers cannot be differentiated again, so a loss on forces "
+                           "cannot be trained through them; use a loss on energies, or the layers they stand for "
+                           "(set_activation_checkpoints(model, bits=None))")
+
+
+def _once(backward):
+    """For a layer whose forward returns (y, anchor) and saves the anchor, an empty output, last.  Under ``create_graph`` the kernels'
+    results would be constants to autograd, and whatever is derived from them would lack their part without a word.  The anchor
+    leads to the layer's inputs without keeping them."""
+
+    @functools.wraps(backward)
+    def wrapper(ctx, grad_output, _):
+        if not torch.is_grad_enabled():
+            return backward(ctx, grad_output)
+        with torch.no_grad():
+            out = backward(ctx, grad_output)
+        there = [i for i, g in enumerate(out) if g is not None]
+        found = _NotTwice.apply(ctx.saved_tensors[-1], grad_output, *(out[i] for i in there))
+        return tuple(found[there.index(i)] if i in there else None for i in range(len(out)))
+
+    return wrapper
+
+
 # ==================================================================================================
 # y = f(x W^T + b), W in 4-bit blocks
 # ==================================================================================================
@@ -185,13 +217,15 @@ class MXFP4LinearFunction(torch.autograd.Function):
         y, dact = _linear(x, codes, scales, bias, DTYPES[x.dtype], tanh, quantize_input, tanh and need and not wide)
         ctx.aux_kind = AUX_NONE if not tanh else AUX_Y if wide else AUX_DACT
         ctx.k = x.shape[1]
-        ctx.save_for_backward(codes, scales, y if ctx.aux_kind == AUX_Y else dact)
-        return y
+        ctx.set_materialize_grads(False)
+        anchor = x.new_empty(0) if need else None
+        ctx.save_for_backward(codes, scales, y if ctx.aux_kind == AUX_Y else dact, anchor)
+        return y, anchor
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, grad_output):
-        codes, scales, aux = ctx.saved_tensors
+        codes, scales, aux, _ = ctx.saved_tensors
         want_x, want_b = ctx.needs_input_grad[0], ctx.needs_input_grad[3]
         g = _aligned(grad_output.contiguous())
         m, n = g.shape
@@ -211,7 +245,7 @@ def mxfp4_linear_autograd(x, codes, scales, bias=None, activation: Optional[str]
     """``mxfp4_linear`` with gradients of x and bias.  Without ``quantize_input`` the gradient of x is the derivative of what
     was computed, so forces taken through such layers are those of their energy."""
     _check_linear(x, codes, scales, bias, activation)
-    return MXFP4LinearFunction.apply(x, codes, scales, bias, activation == "tanh", bool(quantize_input))
+    return MXFP4LinearFunction.apply(x, codes, scales, bias, activation == "tanh", bool(quantize_input))[0]
 
 
 # ==================================================================================================
@@ -238,14 +272,16 @@ class LinearCkpt8Function(torch.autograd.Function):
             ws = _workspace(x, "fmd_linear_ckpt8_workspace_bytes", kind, m, n, k)
             _launch(x.device, "fmd_linear_ckpt8", _at(x), kind, _at(w), _at(bias), _at(y), _at(codes), _at(scales), m, n, k, tanh,
                     _at(ws))
-        ctx.save_for_backward(codes, scales, weight)
+        ctx.set_materialize_grads(False)
+        anchor = x.new_empty(0) if any(ctx.needs_input_grad) else None
+        ctx.save_for_backward(codes, scales, weight, anchor)
         ctx.tanh = tanh
-        return y
+        return y, anchor
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, grad_output):
-        codes, scales, weight = ctx.saved_tensors
+        codes, scales, weight, _ = ctx.saved_tensors
         want_x, want_w, want_b = ctx.needs_input_grad[:3]
         g = _aligned(grad_output.contiguous())
         (m, n), k = g.shape, weight.shape[0]
@@ -268,7 +304,7 @@ def _ckpt8(x, weight, bias, tanh: bool) -> torch.Tensor:
     assert x.shape[1] == weight.shape[0], f"Dimension mismatch: x has {x.shape[1]} columns but weight has {weight.shape[0]} rows"
     assert weight.shape[0] >= 1 and weight.shape[1] >= 1, "an empty weight"
     _vector(bias, weight.shape[1], x)
-    return LinearCkpt8Function.apply(x, weight, bias, tanh)
+    return LinearCkpt8Function.apply(x, weight, bias, tanh)[0]
 
 
 def linear_ckpt8_autograd(x, weight, bias=None) -> torch.Tensor:

@@ -344,7 +344,9 @@ def set_activation_checkpoints(model: torch.nn.Module, bits: Optional[int] = 8) 
     weights' gradients, and the gradients that pass a tanh, come from the rounded values.  A module in ``eval()`` runs its layers
     as if nothing were set, so that the forces of an evaluation are the exact gradient of its energy on every path.  Parameters
     and their names stay as they are.  Not in the reference.  Works on the operator path; the fused engine, which computes
-    forces and nothing for training, is not concerned.  W16A16 and MXFP4 networks are left alone."""
+    forces and nothing for training, is not concerned.  For a loss on energies: the checkpointed layers' gradients cannot be
+    differentiated again, and a loss on forces taken with ``create_graph=True`` raises a RuntimeError in its backward pass.
+    W16A16 and MXFP4 networks are left alone."""
     if bits not in (8, None):
         raise ValueError(f"activation checkpoints in {bits} bits are not built: 8 or None")
     found = [m for m in model.modules() if isinstance(m, (MLP, InteractionBlock))]

@@ -150,6 +150,38 @@ def test_workspaces_do_not_grow_with_the_rows():
     assert 0 < one < 1 << 29 and lib.fmd_linear_ckpt8_workspace_bytes(0, 1 << 26, 300, 300) <= one + (1 << 20)
 
 
+@pytest.mark.parametrize("op", ["linear_ckpt8_autograd", "fused_tanh_linear_ckpt8_autograd", "mxfp4_linear_autograd", "mxfp4_tanh"])
+def test_gradients_are_not_differentiated_again(op, monkeypatch):
+    """create_graph=True with a gradient that is a constant (energies summed for forces): a loss of the result may not come back
+    without the layer's part, whichever of the layer's inputs, or of what is before them, it is differentiated for.  The graph
+    alone is looked at: the kernels are left out."""
+    import flashmd_amd.kernels as K
+    from flashmd_amd import _ffi, mx
+
+    monkeypatch.setattr(_ffi, "require_gpu", lambda *t: None)
+    monkeypatch.setattr(mx, "_launch", lambda *a: None)
+    before, x0 = torch.randn(8, 40, requires_grad=True), torch.randn(5, 8, requires_grad=True)
+    b = torch.randn(6, requires_grad=True)
+    if op.startswith("mxfp4"):
+        codes, scales = torch.zeros(6, 32, dtype=FP4), torch.zeros(6, 2, dtype=torch.uint8)
+        leaves = [before, x0, b]
+        f = lambda x: K.mxfp4_linear_autograd(x, codes, scales, b, "tanh" if op == "mxfp4_tanh" else None)
+    else:
+        w = torch.randn(40, 6, requires_grad=True)
+        leaves = [before, x0, b, w]
+        f = lambda x: getattr(K, op)(x, w, b)
+    for factor in (1.0, torch.ones(1, requires_grad=True)):
+        y = f(x0 @ before)
+        forces = torch.autograd.grad((y * factor).sum(), x0, create_graph=True)[0]
+        for leaf in leaves:
+            with pytest.raises(RuntimeError, match="differentiated again"):
+                torch.autograd.grad((forces * forces).sum(), leaf, retain_graph=True)
+        with pytest.raises(RuntimeError, match="differentiated again"):
+            ((forces * forces).sum() + y.sum()).backward(retain_graph=True)
+        # a loss of the outputs beside them is no second derivative
+        assert all(g.shape == t.shape for g, t in zip(torch.autograd.grad(y.sum(), leaves), leaves))
+
+
 def _model(activation=None):
     import flashmd_amd.schnet as S
 

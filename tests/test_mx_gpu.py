@@ -620,3 +620,24 @@ def test_forces_of_an_evaluation_do_not_go_through_checkpoints(monkeypatch):
     data.pos.requires_grad_(True)
     rounded = -torch.autograd.grad(model(data).out["SchNet"]["energy"].sum(), data.pos)[0]
     assert rel(rounded, f_ref) > 1e-4
+
+
+def test_a_loss_on_forces_is_refused_with_checkpoints(monkeypatch):
+    """GradientsOut in training keeps the graph of the forces.  A loss on energies beside them has the gradients of the bare model's; one
+    on forces, which the PyTorch path can differentiate, raises instead of leaving the layers' part out."""
+    import flashmd_amd.schnet as S
+
+    for gate, off in (("USE_TRITON_MESSAGE_PASSING", False), ("USE_FUSED_RBF", "0"), ("USE_FUSED_TANH_LINEAR", False), ("USE_CSR", False),
+                      ("USE_SRC_CSR_GRAD_X", False), ("USE_FUSED_ENGINE", False)):
+        monkeypatch.setattr(S, gate, off)
+    model = _schnet().to(DEV).train()
+    (S.GradientsOut(model).train()(_batch(S)).out["SchNet"]["forces"] ** 2).sum().backward()
+    S.set_activation_checkpoints(model)
+    params = list(model.parameters())
+    e = model(_batch(S)).out["SchNet"]["energy"]
+    want = torch.autograd.grad((e * e).sum(), params)
+    out = S.GradientsOut(model).train()(_batch(S)).out["SchNet"]
+    with pytest.raises(RuntimeError, match="differentiated again"):
+        (out["forces"] ** 2).sum().backward(retain_graph=True)
+    got = torch.autograd.grad((out["energy"] ** 2).sum(), params)
+    assert all(rel(a, b) < 1e-5 for a, b in zip(got, want))
