@@ -472,6 +472,15 @@ __global__ __launch_bounds__(256) void sum_parts_kernel(const float* __restrict_
   }
 }
 
+// parts[0] = sum over parts, in the parts' order
+__global__ __launch_bounds__(256) void fold_parts_kernel(float* parts, int64_t count, int64_t elements) {
+  for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < elements; t += (int64_t)gridDim.x * 256) {
+    float v = 0.f;
+    for (int64_t s = 0; s < count; ++s) v += parts[s * elements + t];
+    parts[t] = v;
+  }
+}
+
 // column sums of a gradient: part [blockIdx.y] of 64 columns
 template <class S>
 __global__ __launch_bounds__(256) void column_sums_kernel(S src, int64_t rows, int64_t cols, int64_t rows_per_part,
@@ -651,6 +660,10 @@ void mx_sum_parts(const float* parts, int64_t count, int64_t m, int64_t n, int d
   if (dtype == FMD_F32) sum_parts_kernel<float><<<grid_for(m * n), 256, 0, s>>>(parts, count, m, n, e);
   else if (dtype == FMD_F16) sum_parts_kernel<_Float16><<<grid_for(m * n), 256, 0, s>>>(parts, count, m, n, e);
   else sum_parts_kernel<mx_bf16><<<grid_for(m * n), 256, 0, s>>>(parts, count, m, n, e);
+}
+
+void mx_fold_parts(float* parts, int64_t count, int64_t elements, hipStream_t s) {
+  fold_parts_kernel<<<grid_for(elements), 256, 0, s>>>(parts, count, elements);
 }
 
 void mx_column_sums(const MxSource& q, int64_t rows, int64_t cols, int64_t parts, float* out, hipStream_t s) {

@@ -42,6 +42,7 @@ MxProductPlan mx_product_plan(int64_t m, int64_t n, int64_t kt, int npairs);
 void mx_product(const MxOperand& a, const MxOperand& b, int64_t m, int64_t n, int64_t kt, const MxProductPlan& plan, int dtype,
                 const MxEpilogue& e, float* parts, hipStream_t s);
 void mx_sum_parts(const float* parts, int64_t count, int64_t m, int64_t n, int dtype, const MxEpilogue& e, hipStream_t s);
+void mx_fold_parts(float* parts, int64_t count, int64_t elements, hipStream_t s);
 void mx_column_totals(const float* parts, int64_t count, int64_t cols, int dtype, void* out, hipStream_t s);
 void mx_column_sums(const MxSource& q, int64_t rows, int64_t cols, int64_t parts, float* out, hipStream_t s);
 

@@ -150,6 +150,23 @@ def test_workspaces_do_not_grow_with_the_rows():
     assert 0 < one < 1 << 29 and lib.fmd_linear_ckpt8_workspace_bytes(0, 1 << 26, 300, 300) <= one + (1 << 20)
 
 
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+@pytest.mark.parametrize("k,n", [(300, 300), (2000, 1000), (8192, 8192), (16384, 16384), (20000, 300)])
+def test_workspaces_of_gradients_do_not_grow_with_the_rows(k, n, dtype):
+    """The weight gradient's sums over chunks of rows: one chunk's planes (128 MiB, or 1024 rows), four [k, n] matrices in fp32 or 128 MiB
+    of smaller ones, and what the weight and the sums of the bias take, whatever the rows."""
+    from flashmd_amd import _ffi
+
+    lib, mib = _ffi.lib(), 1 << 20
+    for tanh in (0, 1):
+        at = [lib.fmd_linear_ckpt8_bwd_workspace_bytes(dtype, m, n, k, tanh, 1, 1, 1) for m in (1 << 16, 1 << 18, 1 << 20, 1 << 23)]
+        planes = max(128 * mib, 1024 * 6 * (k + n + 64))
+        assert max(at) <= 2 * planes + max(128 * mib, 4 * 4 * k * n) + 6 * (n + 64) * k + 64 * mib, (tanh, at)
+        assert at[3] - at[2] <= mib
+    at = [lib.fmd_mxfp4_linear_bwd_workspace_bytes(dtype, m, n, k, 1, 1) for m in (1 << 18, 1 << 20, 1 << 23)]
+    assert at[2] - at[1] <= mib and at[2] <= 128 * mib + 1024 * 6 * (n + 64) + 2 * (n + 64) * k + 64 * mib
+
+
 @pytest.mark.parametrize("op", ["linear_ckpt8_autograd", "fused_tanh_linear_ckpt8_autograd", "mxfp4_linear_autograd", "mxfp4_tanh"])
 def test_gradients_are_not_differentiated_again(op, monkeypatch):
     """create_graph=True with a gradient that is a constant (energies summed for forces): a loss of the result may not come back

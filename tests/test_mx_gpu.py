@@ -641,3 +641,24 @@ def test_a_loss_on_forces_is_refused_with_checkpoints(monkeypatch):
         (out["forces"] ** 2).sum().backward(retain_graph=True)
     got = torch.autograd.grad((out["energy"] ** 2).sum(), params)
     assert all(rel(a, b) < 1e-5 for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("dtype,m,k,n", [(torch.float32, 60_000, 2000, 1000), (torch.float32, 26_000, 4200, 2100), (torch.bfloat16, 36_003, 6000, 2999),
+                                         (torch.float16, 36_001, 6000, 2999)])
+def test_weight_gradient_over_many_chunks(K, dtype, m, k, n):
+    """More chunks of rows than sums that are held at once, in parts and whole, the last chunk short.  Small whole numbers: sums are exact
+    in fp32 (below 2^24), so every result has to be the exact one rounded once."""
+    gen = torch.Generator(device=DEV).manual_seed(m)
+
+    def whole(low, high, *shape):
+        return torch.randint(low, high, shape, generator=gen, device=DEV).to(dtype)
+
+    x, w, b, g = whole(-2, 3, m, k), whole(-2, 3, k, n), whole(-3, 4, n), whole(-1, 2, m, n)
+    x[:, 0::32] = 64.0                                        # with 64 the largest of its block, whole numbers are kept whole
+    leaves = [t.requires_grad_() for t in (x, w, b)]
+    y = K.linear_ckpt8_autograd(*leaves)
+    gx, gw, gb = torch.autograd.grad(y, leaves, g)
+    with torch.no_grad():
+        X, W, G = x.double(), w.double(), g.double()
+        assert torch.equal(y, (X @ W + b.double()).to(dtype)) and torch.equal(gx, (G @ W.t().contiguous()).to(dtype))
+        assert torch.equal(gw, (X.t().contiguous() @ G).to(dtype)) and torch.equal(gb, G.sum(0).to(dtype))
