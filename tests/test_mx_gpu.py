@@ -662,3 +662,50 @@ def test_weight_gradient_over_many_chunks(K, dtype, m, k, n):
         X, W, G = x.double(), w.double(), g.double()
         assert torch.equal(y, (X @ W + b.double()).to(dtype)) and torch.equal(gx, (G @ W.t().contiguous()).to(dtype))
         assert torch.equal(gw, (X.t().contiguous() @ G).to(dtype)) and torch.equal(gb, G.sum(0).to(dtype))
+
+
+@pytest.mark.parametrize("dtype,wide", [(torch.float32, 20_000), (torch.float16, 60_000), (torch.bfloat16, 60_000)])
+@pytest.mark.parametrize("tanh", [False, True])
+def test_checkpointed_layer_across_a_chunk(K, dtype, wide, tanh):
+    """Chunks of 1024 rows and a short one of 76: the forward pass's planes and checkpoint (many inputs), the gradient of x with tanh' of the
+    checkpoint in its epilogue (many outputs).  The rows behind the first chunk are compared by themselves, too."""
+    m, c = 1100, 1024
+    for k, n in ((wide, 260), (260, wide)):
+        x, w = uneven(m, k, dtype, seed=1), rand(k, n, seed=2, scale=(2.0 / (k + n)) ** 0.5, dtype=dtype)
+        x = torch.where(torch.isfinite(x), x, torch.zeros((), dtype=dtype))
+        bias, g = rand(n, seed=3, dtype=dtype), rand(m, n, seed=4, scale=1e-2, dtype=dtype)
+        leaves = [t.to(DEV).requires_grad_() for t in (x, w, bias)]
+        y = (K.fused_tanh_linear_ckpt8_autograd if tanh else K.linear_ckpt8_autograd)(*leaves)
+        gx, gw, gb = torch.autograd.grad(y, leaves, g.to(DEV))
+        kept = K.mxint8_dequantize(*K.mxint8_quantize(x.to(DEV)), k)
+        X, W, G, B = (t.to(DEV).double() for t in (x, w, g, bias))
+        p = torch.tanh if tanh else (lambda t: t)
+        y_ref, gx_ref = p(X) @ W + B, G @ W.t().contiguous()
+        if tanh:
+            gx_ref = gx_ref / torch.cosh(kept.double()) ** 2
+        for rows in (slice(0, m), slice(c, m)):
+            near(y[rows], y_ref[rows], k, "y")
+            near(gx[rows], gx_ref[rows], n, "gx")
+        near(gw, p(kept.double()).t().contiguous() @ G, m, "gw")
+        near(gb, G.sum(0), m, "gb")
+
+
+@pytest.mark.parametrize("dtype,wide", [(torch.float32, 20_000), (torch.float16, 30_000), (torch.bfloat16, 60_000)])
+@pytest.mark.parametrize("tanh", [False, True])
+def test_four_bit_layer_across_a_chunk(K, dtype, wide, tanh):
+    """The same for 4-bit weights: y and the kept derivative of its tanh (many inputs), the gradient through it (many outputs)."""
+    m, c = 1100, 1024
+    for k, n in ((wide, 260), (260, wide)):
+        x, bias, g = rand(m, k, seed=1, dtype=dtype), rand(n, seed=3, dtype=dtype), rand(m, n, seed=4, scale=1e-2, dtype=dtype)
+        codes, scales = K.mxfp4_quantize(rand(n, k, seed=2, scale=(1.0 / k) ** 0.5).to(DEV))
+        W = K.mxfp4_dequantize(codes, scales, k).double()
+        xg, bg = x.to(DEV).requires_grad_(), bias.to(DEV).requires_grad_()
+        y = K.mxfp4_linear_autograd(xg, codes, scales, bg, "tanh" if tanh else None)
+        gx, gb = torch.autograd.grad(y, (xg, bg), g.to(DEV))
+        z = x.to(DEV).double() @ W.t().contiguous() + bias.to(DEV).double()
+        G = g.to(DEV).double() / torch.cosh(z) ** 2 if tanh else g.to(DEV).double()
+        y_ref, gx_ref = torch.tanh(z) if tanh else z, G @ W
+        for rows in (slice(0, m), slice(c, m)):
+            near(y[rows], y_ref[rows], k, "y")
+            near(gx[rows], gx_ref[rows], n + (k if tanh else 0), "gx")
+        near(gb, G.sum(0), m + (k if tanh else 0), "gb")
