@@ -83,6 +83,16 @@ struct Raw {
   }
 };
 
+// What a lane writes there in one type, others read in another: words that the compiler takes for any type's
+typedef uint16_t any16 __attribute__((may_alias));
+typedef uint32_t any32 __attribute__((may_alias));
+typedef u32x4 any128 __attribute__((may_alias));
+// A wave's accesses of LDS are done in their order; the compiler, which sees one lane's addresses, keeps that order across this
+__device__ __forceinline__ void between_lanes() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
+  __builtin_amdgcn_wave_barrier();
+}
+
 // LDS of a wave, 32 rows x 64 values: row r's piece q of 16 bytes at position q ^ s(r), so that neither the rows' writes nor
 // the lanes' reads (a row each) meet a bank twice
 template <class T>
@@ -95,14 +105,14 @@ struct Pass {
 #pragma unroll
       for (int i = 0; i < R::PIECES; ++i) {
         const int r = i * (64 / R::PER_ROW) + lane / R::PER_ROW, q = lane % R::PER_ROW;
-        *(u32x4*)(lds + r * ROW + (q ^ swz(r)) * 16) = raw.v[i];
+        *(any128*)(lds + r * ROW + (q ^ swz(r)) * 16) = raw.v[i];
       }
     } else {
 #pragma unroll
       for (int i = 0; i < 32; ++i) {
         char* to = lds + i * ROW + ((lane / PER) ^ swz(i)) * 16 + (lane % PER) * S;
-        if constexpr (S == 4) *(uint32_t*)to = raw.v[i >> 2][i & 3];
-        else *(uint16_t*)to = (uint16_t)raw.v[i >> 2][i & 3];
+        if constexpr (S == 4) *(any32*)to = raw.v[i >> 2][i & 3];
+        else *(any16*)to = (uint16_t)raw.v[i >> 2][i & 3];
       }
     }
   }
@@ -113,8 +123,8 @@ struct Pass {
     for (int r = 0; r < 32; ++r) {
       const char* at = lds + r * ROW + ((col / PER) ^ swz(r)) * 16 + col % PER * S;
       T v;
-      if constexpr (S == 4) v = __builtin_bit_cast(T, *(const uint32_t*)at);
-      else v = __builtin_bit_cast(T, *(const uint16_t*)at);
+      if constexpr (S == 4) v = __builtin_bit_cast(T, (uint32_t) * (const any32*)at);
+      else v = __builtin_bit_cast(T, (uint16_t) * (const any16*)at);
       s[r & 3] += MxType<T>::to(v);
     }
     return (s[0] + s[1]) + (s[2] + s[3]);
@@ -124,7 +134,7 @@ struct Pass {
     constexpr int N = ROW / 32;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const u32x4 u = *(const u32x4*)(lds + row * ROW + ((h * N + i) ^ swz(row)) * 16);
+      const u32x4 u = *(const any128*)(lds + row * ROW + ((h * N + i) ^ swz(row)) * 16);
       T t[PER];
       *(u32x4*)t = u;
 #pragma unroll
@@ -153,14 +163,14 @@ __device__ __forceinline__ void put_product(char* lds, const Raw<T>& g, const Ra
         f32x4 o;
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[e] = MxType<T>::to(gv[4 * k + e]) * factor(MxType<A>::to(av[4 * k + e]));
-        *(f32x4*)(lds + r * 256 + ((q * (R::PER / 4) + k) ^ Pass<float>::swz(r)) * 16) = o;
+        *(any128*)(lds + r * 256 + ((q * (R::PER / 4) + k) ^ Pass<float>::swz(r)) * 16) = __builtin_bit_cast(u32x4, o);
       }
     }
   } else {
 #pragma unroll
     for (int i = 0; i < 32; ++i)
-      *(float*)(lds + i * 256 + ((lane >> 2) ^ Pass<float>::swz(i)) * 16 + (lane & 3) * 4) =
-          Raw<T>::value(g.v[i >> 2][i & 3]) * factor(Raw<A>::value(aux.v[i >> 2][i & 3]));
+      *(any32*)(lds + i * 256 + ((lane >> 2) ^ Pass<float>::swz(i)) * 16 + (lane & 3) * 4) =
+          __builtin_bit_cast(uint32_t, Raw<T>::value(g.v[i >> 2][i & 3]) * factor(Raw<A>::value(aux.v[i >> 2][i & 3])));
   }
 }
 
@@ -300,9 +310,11 @@ __global__ __launch_bounds__(64 * WAVES, 2) void layer_kernel(const LayerArgs a)
       float x[32];
       if constexpr (AUX) {
         put_product<T>(own, raw, raw_aux, vec, lane);
+        between_lanes();
         Pass<float>::get(own, j, h, x);
       } else {
         Pass<T>::put(own, raw, vec, lane);
+        between_lanes();
         Pass<T>::get(own, j, h, x);
       }
       if (WK == W_FP4_ACROSS && a.sums) {
@@ -310,6 +322,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void layer_kernel(const LayerArgs a)
 #pragma unroll
         for (int i = 0; i < 4; ++i) sums[i] += i == ch ? v : 0.f;
       }
+      between_lanes();
       const int next_tile = ch + 1 < chunks ? tile : tile + stride, next_ch = ch + 1 < chunks ? ch + 1 : 0;
       if (next_tile < tiles) fetch(next_tile, next_ch);
       if (EPI == EPI_ACT && WK == W_DENSE && a.codes8 && blockIdx.y == 0) {

@@ -709,3 +709,19 @@ def test_four_bit_layer_across_a_chunk(K, dtype, wide, tanh):
             near(y[rows], y_ref[rows], k, "y")
             near(gx[rows], gx_ref[rows], n + (k if tanh else 0), "gx")
         near(gb, G.sum(0), m + (k if tanh else 0), "gb")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m,k,n", [(5000, 64, 33), (34_432, 20, 7), (2100, 100, 255), (40, 33, 50), (9000, 128, 129)])
+def test_products_with_the_derivative_between_lanes(K, dtype, m, k, n):
+    """g f' of rows that no 16-byte piece divides goes through LDS word by word, and is read back by other lanes as rows and as columns.
+    With x = 0 and no bias f' is 1: whole numbers give exact gradients, rounded once."""
+    gen = torch.Generator().manual_seed(n)
+    w, g = torch.randint(-3, 4, (n, k), generator=gen).float(), torch.randint(-2, 3, (m, n), generator=gen).to(dtype)
+    w[:, 0::32] = 4.0                                         # blocks whose whole numbers up to 4 are kept whole
+    codes, scales, values = mo.mxfp4(w)
+    assert torch.equal(values, w.double())
+    x, b = torch.zeros(m, k, dtype=dtype, device=DEV).requires_grad_(), torch.zeros(n, dtype=dtype, device=DEV).requires_grad_()
+    y = K.mxfp4_linear_autograd(x, codes.to(DEV), scales.to(DEV), b, "tanh")
+    gx, gb = torch.autograd.grad(y, (x, b), g.to(DEV))
+    assert torch.equal(gx.cpu(), (g.double() @ values).to(dtype)) and torch.equal(gb.cpu(), g.double().sum(0).to(dtype))
