@@ -725,3 +725,33 @@ def test_products_with_the_derivative_between_lanes(K, dtype, m, k, n):
     y = K.mxfp4_linear_autograd(x, codes.to(DEV), scales.to(DEV), b, "tanh")
     gx, gb = torch.autograd.grad(y, (x, b), g.to(DEV))
     assert torch.equal(gx.cpu(), (g.double() @ values).to(dtype)) and torch.equal(gb.cpu(), g.double().sum(0).to(dtype))
+
+
+def saturated(m, k, dtype, top):
+    """values of both signs up to `top`, the larger ones dense"""
+    gen = torch.Generator().manual_seed(m)
+    x = top * torch.rand(m, k, generator=gen) ** 0.5 * torch.randint(0, 2, (m, k), generator=gen).mul(2).sub(1)
+    return x.to(dtype)
+
+
+def each_near(got, want, top, scale=1.0):
+    """Element by element.  tanh' = 4 t (1 - t), t = 1 / (e^{2|x|} + 1): 2|x| log2(e) and its constant are rounded (1.5 units in the last
+    place of it each way, at most 3 |x| of the result's), the exponential, the reciprocal and three operations by a unit or so each:
+    2^-24 (5 |x| + 16); then the type's own half a step, relative or of its smallest number."""
+    t = torch.finfo(got.dtype)
+    off = (got.double().cpu() - want).abs()
+    tol = (2.0 ** -24 * (5 * top + 16) + (t.eps / 2 if got.dtype != torch.float32 else 0.0)) * want.abs() + t.smallest_normal * t.eps / 2
+    worst = float((off / tol).max())
+    assert worst <= 1.0, worst
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m,k", [(40, 64), (40, 50), (3000, 64), (100, 300), (300, 1030)])
+def test_derivative_of_a_saturated_checkpoint(K, dtype, m, k):
+    """tanh' of kept values up to 14, element by element: through an identity weight the gradient of x is g tanh'(x8) and nothing else."""
+    top = 14.0
+    x, w = saturated(m, k, dtype, top), torch.eye(k, dtype=dtype)
+    leaf = x.to(DEV).requires_grad_()
+    y = K.fused_tanh_linear_ckpt8_autograd(leaf, w.to(DEV))
+    (gx,) = torch.autograd.grad(y, leaf, torch.full((m, k), 1024.0, dtype=dtype, device=DEV))
+    each_near(gx, 1024.0 / torch.cosh(mo.mxint8(x)[2]) ** 2, top)
