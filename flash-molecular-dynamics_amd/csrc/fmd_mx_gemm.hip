@@ -41,7 +41,7 @@ struct SrcDense {
       for (int i = 0; i < 8; ++i) v[i] = mx_tanh(v[i]);  // tanh(0) = 0: padding stays zero
   }
 };
-// a gradient times the derivative of the activation behind it.  AUX 1: aux = y in fp32, factor 1 - y^2; 2: aux = the factor in fp16
+// a gradient times the derivative of the activation behind it.  AUX 1: aux = y in fp32, factor 1 - y^2; 2: aux = the factor as mx_dact
 template <class T, int AUX>
 struct SrcGrad {
   const T* p;
@@ -57,7 +57,7 @@ struct SrcGrad {
       for (int i = 0; i < 8; ++i) v[i] *= 1.f - y[i] * y[i];
     } else if constexpr (AUX == 2) {
       float d[8];
-      SrcDense<_Float16, false>{(const _Float16*)aux, cols, vec}.load(row, c0, d);
+      SrcDense<mx_dact, false>{(const mx_dact*)aux, cols, vec}.load(row, c0, d);
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] *= d[i];
     }
@@ -229,8 +229,11 @@ struct GemmArgs {
 template <class T>
 __device__ __forceinline__ void finish_one(const MxEpilogue& e, int64_t row, int64_t col, int64_t ld, float v) {
   if (e.bias) v += MxType<T>::to(((const T*)e.bias)[col]);
-  if (e.tanh) v = mx_tanh(v);
-  if (e.dact) ((_Float16*)e.dact)[row * ld + col] = (_Float16)(1.f - v * v);
+  if (e.tanh) {
+    const float t = mx_sigma(v);
+    if (e.dact) ((mx_dact*)e.dact)[row * ld + col] = MxType<mx_dact>::from(mx_keep_dtanh_of(t));
+    v = mx_tanh(v, t);
+  }
   if (e.codes8) v = mx_times_dtanh(v, (int)(int8_t)e.codes8[row * e.nb8 * 32 + col], e.scales8[row * e.nb8 + (col >> 5)]);
   ((T*)e.out)[row * ld + col] = MxType<T>::from(v);
 }
@@ -438,13 +441,17 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_kernel(const GemmArgs g) {
           if (INSIDE || col + b < g.n) bias[b] = MxType<T>::to(((const T*)g.e.bias)[col + b]);
       if (g.e.tanh) {
         each([&](int64_t at, float (&v)[TN]) {
+          float t[TN];
 #pragma unroll
-          for (int b = 0; b < TN; ++b) v[b] = mx_tanh(v[b] + bias[b]);
+          for (int b = 0; b < TN; ++b) {
+            t[b] = mx_sigma(v[b] + bias[b]);
+            v[b] = mx_tanh(v[b] + bias[b], t[b]);
+          }
           write((T*)g.e.out + at, v);
           if (g.e.dact) {
 #pragma unroll
-            for (int b = 0; b < TN; ++b) v[b] = 1.f - v[b] * v[b];
-            write((_Float16*)g.e.dact + at, v);
+            for (int b = 0; b < TN; ++b) t[b] = mx_keep_dtanh_of(t[b]);
+            write((mx_dact*)g.e.dact + at, t);
           }
         });
       } else {

@@ -5,7 +5,7 @@
 struct MxEpilogue {            // v = acc (+ bias) (tanh) (* tanh'(8-bit value)) -> out
   const void* bias;            // in out's type, or null
   void* out;
-  void* dact;                  // fp16 1 - tanh^2, or null
+  void* dact;                  // tanh' as mx_dact, or null
   const uint8_t *codes8, *scales8;  // [row][32 nb8], [row][nb8], or null
   int64_t nb8;
   int tanh;

@@ -78,8 +78,7 @@ struct Raw {
   }
   static __device__ __forceinline__ float value(uint32_t u) {
     if constexpr (S == 4) return __builtin_bit_cast(float, u);
-    else if constexpr (std::is_same<T, mx_bf16>::value) return __builtin_bit_cast(float, u << 16);
-    else return (float)__builtin_bit_cast(_Float16, (uint16_t)u);
+    else return MxType<T>::to(__builtin_bit_cast(T, (uint16_t)u));
   }
 };
 
@@ -143,11 +142,11 @@ struct Pass {
   }
 };
 
-// a gradient and its factor, multiplied in fp32 on the way into LDS.  T = float: aux = y, factor 1 - y^2; else aux = the factor in fp16
+// a gradient and its factor, multiplied in fp32 on the way into LDS.  T = float: aux = y, factor 1 - y^2; else aux = the factor
 template <class T>
-__device__ __forceinline__ void put_product(char* lds, const Raw<T>& g, const Raw<typename std::conditional<sizeof(T) == 4, float, _Float16>::type>& aux,
+__device__ __forceinline__ void put_product(char* lds, const Raw<T>& g, const Raw<typename std::conditional<sizeof(T) == 4, float, mx_dact>::type>& aux,
                                             bool vec, int lane) {
-  using A = typename std::conditional<sizeof(T) == 4, float, _Float16>::type;
+  using A = typename std::conditional<sizeof(T) == 4, float, mx_dact>::type;
   using R = Raw<T>;
   auto factor = [](float v) { return sizeof(T) == 4 ? 1.f - v * v : v; };
   if (vec) {
@@ -269,7 +268,7 @@ constexpr int pass_bytes() {  // LDS of a wave on the way from rows to lanes
 template <class T, int PRO, int WK, int EPI, int NT>
 __global__ __launch_bounds__(64 * WAVES, 2) void layer_kernel(const LayerArgs a) {
   constexpr int PA = LayerPlanes<T, WK>::in, PB = LayerPlanes<T, WK>::w, TOP = PA > PB ? PA : PB;
-  using AuxT = typename std::conditional<sizeof(T) == 4, float, _Float16>::type;
+  using AuxT = typename std::conditional<sizeof(T) == 4, float, mx_dact>::type;
   constexpr bool AUX = PRO == PRO_GRAD_Y || PRO == PRO_GRAD_D;
   constexpr int S = sizeof(T);
   extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -308,6 +307,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void layer_kernel(const LayerArgs a)
         for (int r = 0; r < 16; ++r) acc[t][r] = 0.f;
     {
       float x[32];
+      between_lanes();
       if constexpr (AUX) {
         put_product<T>(own, raw, raw_aux, vec, lane);
         between_lanes();
@@ -322,7 +322,6 @@ __global__ __launch_bounds__(64 * WAVES, 2) void layer_kernel(const LayerArgs a)
 #pragma unroll
         for (int i = 0; i < 4; ++i) sums[i] += i == ch ? v : 0.f;
       }
-      between_lanes();
       const int next_tile = ch + 1 < chunks ? tile : tile + stride, next_ch = ch + 1 < chunks ? ch + 1 : 0;
       if (next_tile < tiles) fetch(next_tile, next_ch);
       if (EPI == EPI_ACT && WK == W_DENSE && a.codes8 && blockIdx.y == 0) {
@@ -397,7 +396,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void layer_kernel(const LayerArgs a)
     tile += stride;
     const int col = o0 + NT * j, os = mx_here(a.o), nbs = mx_here(a.nb8);
     const bool whole = a.o % NT == 0;
-    // v of one row into out (U = T) or dact (U = fp16); a lane's columns in one store where every row starts on a multiple of NT
+    // v of one row into out (U = T) or dact (U = mx_dact); a lane's columns in one store where every row starts on a multiple of NT
     auto write = [&](auto zero, Rows rows, int r, const float (&v)[NT]) {
       using U = decltype(zero);
       constexpr int SU = sizeof(U);
@@ -445,15 +444,20 @@ __global__ __launch_bounds__(64 * WAVES, 2) void layer_kernel(const LayerArgs a)
         float v[NT];
 #pragma unroll
         for (int t = 0; t < NT; ++t) v[t] = acc[t][r] + bias[t];
-        if (a.tanh)
+        if ((WK == W_FP4 || WK == W_FP4_BOTH) && a.tanh) {  // the others have none
+          float u[NT];
 #pragma unroll
-          for (int t = 0; t < NT; ++t) v[t] = mx_tanh(v[t]);
-        write(T{}, out, r, v);
-        if (a.dact) {
+          for (int t = 0; t < NT; ++t) {
+            u[t] = mx_sigma(v[t]);
+            v[t] = mx_tanh(v[t], u[t]);
+          }
+          if (a.dact) {
 #pragma unroll
-          for (int t = 0; t < NT; ++t) v[t] = 1.f - v[t] * v[t];
-          write(_Float16{}, dact, r, v);
+            for (int t = 0; t < NT; ++t) u[t] = mx_keep_dtanh_of(u[t]);
+            write(mx_dact{}, dact, r, u);
+          }
         }
+        write(T{}, out, r, v);
       }
     }
   }

@@ -143,10 +143,13 @@ __global__ __launch_bounds__(64 * WAVES) void rows_kernel(const RowsArgs a) {
     for (int w = 0; w < WAVES; ++w) v += ((const float*)&lds[w][t][((c >> 2) << 4) + ((o >> 4) & 15)])[c & 3];
     if (m >= a.m || n >= a.n) continue;
     if (a.e.bias) v += MxType<T>::to(((const T*)a.e.bias)[n]);
-    if (a.e.tanh) v = mx_tanh(v);
     const int64_t at = (int64_t)m * a.n + n;
+    if (a.e.tanh) {
+      const float t = mx_sigma(v);
+      if (a.e.dact) ((mx_dact*)a.e.dact)[at] = MxType<mx_dact>::from(mx_keep_dtanh_of(t));
+      v = mx_tanh(v, t);
+    }
     ((T*)a.e.out)[at] = MxType<T>::from(v);
-    if (a.e.dact) ((_Float16*)a.e.dact)[at] = (_Float16)(1.f - v * v);
   }
 }
 

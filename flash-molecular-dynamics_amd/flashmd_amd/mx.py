@@ -189,7 +189,7 @@ def _linear(x, codes, scales, bias, kind: int, tanh: bool, quantize_input: bool,
     n = codes.shape[0]
     x, codes = _aligned(x), _aligned(codes)
     y = torch.empty((m, n), dtype=x.dtype, device=x.device)
-    dact = torch.empty((m, n), dtype=torch.float16, device=x.device) if want_dact else None
+    dact = torch.empty((m, n), dtype=torch.int16, device=x.device) if want_dact else None
     if m:
         ws = _workspace(x, "fmd_mxfp4_linear_workspace_bytes", kind, m, n, k, quantize_input)
         _launch(x.device, "fmd_mxfp4_linear", _at(x), kind, _at(codes), _at(scales), _at(bias), _at(y), _at(dact), m, n, k, tanh,
@@ -207,8 +207,9 @@ def mxfp4_linear(x, codes, scales, bias=None, activation: Optional[str] = None, 
 
 class MXFP4LinearFunction(torch.autograd.Function):
     """gx = (g f') W, gb = sum g f'.  The codes have no gradient; with ``quantize_input`` the quantisation of x passes the
-    gradient on as if it were the identity.  f' = 1 - y^2 comes from y in float32 and, in 16 bits, where 1 - y^2 of the
-    rounded y would lose its leading digits near saturation, from a float16 copy made before y is rounded."""
+    gradient on as if it were the identity.  f' comes from y in float32, as 1 - y^2 (off by up to 2^-23, as y is rounded: digits
+    are lost near saturation, as everywhere in torch).  In 16 bits 1 - y^2 of the rounded y would be far worse: f' itself is
+    kept in 16 bits, computed before y is rounded, within 2^-13 of itself or 2^-27."""
 
     @staticmethod
     def forward(ctx, x, codes, scales, bias, tanh, quantize_input):

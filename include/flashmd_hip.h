@@ -183,11 +183,11 @@ int fmd_matmul_f32_f16_to_f16(const float* a, const void* b, void* c, int64_t m,
  *
  *   fmd_mxfp4_quantize / _dequantize, fmd_mxint8_quantize / _dequantize: x [m,k] <-> codes, scales
  *   fmd_mxfp4_linear      y[m,n] = f(x^ W^T + bias): W [n,k] as codes, scales; f the identity or (tanh != 0) tanh;
- *        x^ = x, or with quantize_input x's own 4-bit blocks.  dact (fp16 [m,n], or NULL): 1 - y^2 before y is rounded, for the
- *        backward pass of a 16-bit layer
+ *        x^ = x, or with quantize_input x's own 4-bit blocks.  dact (16 bits a value, [m,n], or NULL): f' of the sum before anything
+ *        is rounded, within 2^-13 of itself or 2^-27, for the backward pass of a 16-bit layer, which alone reads it
  *   fmd_mxfp4_linear_bwd  gx = (g f') W^, gbias = sum over rows of g f'; f' from aux: FMD_AUX_NONE (f' = 1), FMD_AUX_Y (fp32
- *        only: aux = y, f' = 1 - y^2), FMD_AUX_DACT (16 bits only: aux = dact).  gx / gbias may be NULL.  With quantize_input
- *        this is the gradient that passes the quantisation unchanged
+ *        only: aux = y, f' = 1 - y^2, off by up to 2^-23 as y is rounded), FMD_AUX_DACT (16 bits only: aux = dact).  gx / gbias
+ *        may be NULL.  With quantize_input this is the gradient that passes the quantisation unchanged
  *   fmd_linear_ckpt8      y = p(x) W + bias, W [k,n], p the identity or tanh; codes, scales (both or neither NULL): x in
  *        8-bit blocks
  *   fmd_linear_ckpt8_bwd  from those: gx = (g W^T) p'(x8), gw[k,n] = p(x8)^T g, gbias = sum g; each may be NULL; m >= 1

@@ -734,13 +734,14 @@ def saturated(m, k, dtype, top):
     return x.to(dtype)
 
 
-def each_near(got, want, top, scale=1.0):
+def each_near(got, want, top, more=0.0, least=0.0):
     """Element by element.  tanh' = 4 t (1 - t), t = 1 / (e^{2|x|} + 1): 2|x| log2(e) and its constant are rounded (1.5 units in the last
     place of it each way, at most 3 |x| of the result's), the exponential, the reciprocal and three operations by a unit or so each:
-    2^-24 (5 |x| + 16); then the type's own half a step, relative or of its smallest number."""
+    2^-24 (5 |x| + 16); then the type's own half a step, relative or of its smallest number, and what is given as `more` (relative)
+    and `least`."""
     t = torch.finfo(got.dtype)
-    off = (got.double().cpu() - want).abs()
-    tol = (2.0 ** -24 * (5 * top + 16) + (t.eps / 2 if got.dtype != torch.float32 else 0.0)) * want.abs() + t.smallest_normal * t.eps / 2
+    off = (got.detach().double().cpu() - want).abs()
+    tol = (2.0 ** -24 * (5 * top + 16) + more + (t.eps / 2 if got.dtype != torch.float32 else 0.0)) * want.abs() + t.smallest_normal * t.eps / 2 + least
     worst = float((off / tol).max())
     assert worst <= 1.0, worst
 
@@ -755,3 +756,42 @@ def test_derivative_of_a_saturated_checkpoint(K, dtype, m, k):
     y = K.fused_tanh_linear_ckpt8_autograd(leaf, w.to(DEV))
     (gx,) = torch.autograd.grad(y, leaf, torch.full((m, k), 1024.0, dtype=dtype, device=DEV))
     each_near(gx, 1024.0 / torch.cosh(mo.mxint8(x)[2]) ** 2, top)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("m,k", [(40, 64), (40, 50), (5, 255), (3000, 64), (40, 300), (100, 300), (300, 1030), (6000, 2100)])
+def test_derivative_of_a_saturated_four_bit_layer(K, dtype, m, k):
+    """f' of sums up to 14 in 16 bits, element by element: through an identity the gradient of x is g f' and nothing else, in every kernel
+    that keeps f' (few rows, narrow, wide, the contraction in parts) and in those that read it.  f' is kept within 2^-13 of itself or 2^-27; in
+    fp16 the product g f' is cut to two planes of 8 bits, 2^-15 of it at most."""
+    top = 14.0
+    x = saturated(m, k, dtype, top)
+    codes, scales = K.mxfp4_quantize(torch.eye(k, device=DEV))
+    leaf, b = x.to(DEV).requires_grad_(), torch.zeros(k, dtype=dtype, device=DEV).requires_grad_()
+    y = K.mxfp4_linear_autograd(leaf, codes, scales, b, "tanh")
+    gx, gb = torch.autograd.grad(y, (leaf, b), torch.full((m, k), 1024.0, dtype=dtype, device=DEV))
+    want = 1024.0 / torch.cosh(x.double()) ** 2
+    each_near(y, torch.tanh(x.double()), top)
+    planes = 2.0 ** -15 if dtype == torch.float16 else 0.0
+    small = want < 1024.0 * 2.0 ** -14
+    each_near(gx[~small], want[~small], top, planes + 2.0 ** -13)
+    each_near(gx[small], want[small], top, planes, 1024.0 * 2.0 ** -27)
+    near(gb, want.sum(0), m)
+
+
+def test_kept_derivatives_that_are_exact_or_not_numbers(K):
+    """f' of 0 is 1 and of an Inf 0, exactly; of a NaN it is one, in every kernel that keeps or reads it."""
+    for dtype in (torch.float16, torch.bfloat16):
+        for m, k in ((40, 64), (40, 50), (40, 300), (100, 300), (300, 1030)):
+            x = torch.zeros(m, k, dtype=dtype)
+            codes, scales = K.mxfp4_quantize(torch.eye(k, device=DEV))
+            bias = torch.zeros(k, dtype=dtype)
+            bias[1], bias[3], bias[k - 1] = float("inf"), float("nan"), -float("inf")
+            leaf, b = x.to(DEV).requires_grad_(), bias.to(DEV).requires_grad_()
+            y = K.mxfp4_linear_autograd(leaf, codes, scales, b, "tanh")
+            gb, = torch.autograd.grad(y, b, torch.full((m, k), 3.0, dtype=dtype, device=DEV), retain_graph=True)
+            want = torch.full((k,), 3.0 * m, dtype=torch.float64)
+            want[1], want[3], want[k - 1] = 0.0, float("nan"), 0.0
+            assert torch.equal(torch.nan_to_num(gb.double().cpu(), nan=-1.0), torch.nan_to_num(want.to(dtype).double(), nan=-1.0))
+            gx, = torch.autograd.grad(y, leaf, torch.full((m, k), 3.0, dtype=dtype, device=DEV))
+            assert bool(torch.isnan(gx).all())                # every product has the NaN among its terms, times the identity's zeros
