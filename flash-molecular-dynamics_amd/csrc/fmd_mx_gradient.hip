@@ -41,9 +41,13 @@ __device__ __forceinline__ Rows rows_of(const void* p, int64_t row0, int64_t m, 
 // workgroups a CU: two where half the registers are enough
 template <class T, int KT> constexpr int PER_CU = sizeof(T) == 2 && KT == 2 ? 2 : 1;
 
+// planes of p(x8): one holds the 8 bits themselves, their tanh is not rounded to bf16 first (193688 x 128 x 128 bf16 168 us a call either
+// way, 500 x 1000 x 1000 87 against 89)
+template <class T, bool TANH> constexpr int KEPT_PLANES = !TANH ? 1 : MxType<T>::planes < 2 ? 2 : MxType<T>::planes;
+
 template <class T, bool TANH, int KT, int NT>
 __global__ __launch_bounds__(64 * WAVES, (PER_CU<T, KT>)) void gradient_kernel(const GradArgs a) {
-  constexpr int PA = TANH ? MxType<T>::planes : 1, PB = MxType<T>::planes, TOP = PA > PB ? PA : PB, S = sizeof(T);
+  constexpr int PA = KEPT_PLANES<T, TANH>, PB = MxType<T>::planes, TOP = PA > PB ? PA : PB, S = sizeof(T);
   constexpr int W = NT * S / 4;                    // dwords of a lane's columns in a row of g
   extern __shared__ __attribute__((aligned(16))) float lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), j = lane & 31, h = lane >> 5;
@@ -182,7 +186,7 @@ constexpr int TILE_WAVES = 8;
 
 template <class T, bool TANH>
 __global__ __launch_bounds__(64 * TILE_WAVES) void gradient_tile_kernel(const GradArgs a, T* __restrict__ gw, T* __restrict__ gb) {
-  constexpr int PA = TANH ? MxType<T>::planes : 1, PB = MxType<T>::planes, TOP = PA > PB ? PA : PB, S = sizeof(T);
+  constexpr int PA = KEPT_PLANES<T, TANH>, PB = MxType<T>::planes, TOP = PA > PB ? PA : PB, S = sizeof(T);
   __shared__ float lds[TILE_WAVES][17][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), j = lane & 31, h = lane >> 5;
   const int block = blockIdx.x, k = block * 32 + j, n = blockIdx.y * 32 + j;  // 32 columns of the checkpoint: one block

@@ -39,8 +39,10 @@ struct LayerArgs {
   int c, o, vec, wvec, tanh, nb8;
 };
 
-template <class T, int WK> struct LayerPlanes {
-  static constexpr int in = WK == W_FP4_BOTH ? 1 : MxType<T>::planes;
+// an operand that is computed here has a second plane in bf16: one would round it to the layer's type before the product does
+// (193688 x 128 x 128 bf16 under tanh, us a call: forward 56 against 53, backward of a 4-bit layer 79 against 81)
+template <class T, int WK, int PRO = PRO_ID> struct LayerPlanes {
+  static constexpr int in = WK == W_FP4_BOTH ? 1 : PRO != PRO_ID && MxType<T>::planes == 1 ? 2 : MxType<T>::planes;
   static constexpr int w = WK == W_DENSE ? MxType<T>::planes : 1;
 };
 
@@ -267,7 +269,7 @@ constexpr int pass_bytes() {  // LDS of a wave on the way from rows to lanes
 
 template <class T, int PRO, int WK, int EPI, int NT>
 __global__ __launch_bounds__(64 * WAVES, 2) void layer_kernel(const LayerArgs a) {
-  constexpr int PA = LayerPlanes<T, WK>::in, PB = LayerPlanes<T, WK>::w, TOP = PA > PB ? PA : PB;
+  constexpr int PA = LayerPlanes<T, WK, PRO>::in, PB = LayerPlanes<T, WK>::w, TOP = PA > PB ? PA : PB;
   using AuxT = typename std::conditional<sizeof(T) == 4, float, mx_dact>::type;
   constexpr bool AUX = PRO == PRO_GRAD_Y || PRO == PRO_GRAD_D;
   constexpr int S = sizeof(T);

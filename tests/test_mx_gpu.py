@@ -795,3 +795,31 @@ def test_kept_derivatives_that_are_exact_or_not_numbers(K):
             assert torch.equal(torch.nan_to_num(gb.double().cpu(), nan=-1.0), torch.nan_to_num(want.to(dtype).double(), nan=-1.0))
             gx, = torch.autograd.grad(y, leaf, torch.full((m, k), 3.0, dtype=dtype, device=DEV))
             assert bool(torch.isnan(gx).all())                # every product has the NaN among its terms, times the identity's zeros
+
+
+@pytest.mark.parametrize("m,k,n", [(269, 128, 128), (3000, 50, 128), (66_005, 57, 131), (99_000, 128, 100), (400, 300, 300), (5, 7, 200)])
+def test_computed_operands_of_narrow_bf16_layers_are_not_rounded(K, m, k, n):
+    """tanh(x), tanh(x8) and g f' enter their products in two planes, within 2^-15 of themselves (g f' within 2^-13, as f' is kept), so that
+    nearly every result is the exact one rounded once.  A result that is off by e of the results' root mean square R before it is rounded
+    rounds otherwise with a chance of about 2^7.5 e R / |v|, for normal v 0.8 r (1 + ln 1/r) on average, r = 2^7.5 e: 4 % for e = 2^-14.3
+    (2^-13 in the root mean square), but 50 % for operands rounded to bf16 (e = 2^-9.3)."""
+    def otherwise(got, want):
+        return float((got.detach() != want.to(torch.bfloat16)).double().mean())
+
+    x, w = rand(m, k, seed=1), rand(k, n, seed=2, scale=(2.0 / (k + n)) ** 0.5, dtype=torch.bfloat16)
+    x, g = x.bfloat16(), rand(m, n, seed=3, scale=1e-2, dtype=torch.bfloat16)
+    most = 0.12
+    leaves = [t.to(DEV).requires_grad_() for t in (x, w)]
+    y = K.fused_tanh_linear_ckpt8_autograd(*leaves)
+    gw = torch.autograd.grad(y, leaves[1], g.to(DEV))[0]
+    X, W, G = x.to(DEV).double(), w.to(DEV).double(), g.to(DEV).double()
+    kept = K.mxint8_dequantize(*K.mxint8_quantize(x.to(DEV)), k).double()
+    if max(k, n) <= 256:
+        assert otherwise(y, torch.tanh(X) @ W) <= most
+    assert otherwise(gw, torch.tanh(kept).t().contiguous() @ G) <= most
+    codes, scales = K.mxfp4_quantize(w.t().contiguous().to(DEV))
+    V = K.mxfp4_dequantize(codes, scales, k).double()
+    y = K.mxfp4_linear_autograd(leaves[0], codes, scales, None, "tanh")
+    gx = torch.autograd.grad(y, leaves[0], g.to(DEV))[0]
+    if max(k, n) <= 256:
+        assert otherwise(gx, (G / torch.cosh(X @ V.t().contiguous()) ** 2) @ V) <= most
