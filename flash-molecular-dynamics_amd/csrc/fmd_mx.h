@@ -10,8 +10,14 @@
 // two, a bf16 value and every 4- or 8-bit block value is one.  A product of plane sums keeps the plane pairs (i, j) with
 // i + j < max(planes): what is dropped is below the last kept plane's last bit.  bf16 has fp32's range, so no operand
 // needs a scale of its own.  Where every operand is fp16 or a function of fp16 values that stays in its range (a wide layer's
-// training products), one fp16 plane does the work of two bf16 ones: tanh is rounded to 2^-12, and an 8-bit value below 2^-17 to a
-// multiple of fp16's smallest, 2^-24, as its fp16 input was.
+// training products), one fp16 plane does the work of two bf16 ones; the 8-bit value of an fp16 number is one itself.
+//
+// Operands that are computed (tanh(x), tanh of an 8-bit value, a gradient times tanh') are no such sums.  fp32 has its three planes for
+// them, a narrow 16-bit layer two: 2^-15 of the value.  A wide 16-bit layer has one plane of its type for them, two bf16 ones for an fp16
+// gradient times tanh': they are rounded to the type once more, as a layer of separate 16-bit operations would, because a second
+// plane doubles the products.  8192 x 4096 -> 1024 bf16 under tanh, us a call: forward 128, with two planes 228; backward 290, 418; 2.2e-3
+// from the exact result, 1.7e-3.  4096 x 4096 -> 4096 with 4-bit weights backward 192, 303.  1294 x 6196 -> 2319 fp16, a training step
+// with two bf16 planes of everything 573, with one fp16 plane 277; 2.9e-4 and 2.1e-4.
 #pragma once
 #include "fmd_common.h"
 

@@ -89,7 +89,7 @@ hipError_t mx_allow_lds(K kernel, int bytes) {
 }
 
 static inline int mx_dtype_size(int dtype) { return dtype == FMD_F32 ? 4 : 2; }
-// products of 16-bit operands alone: one plane of their own type
+// a wide layer's products of 16-bit operands alone: one plane of their own type, to which computed ones are rounded (fmd_mx.h)
 static inline bool mx_half(int dtype) { return dtype == FMD_F16; }
 static inline int mx_own_planes(int dtype) { return dtype == FMD_F32 ? 3 : 1; }
 static inline int mx_dtype_planes(int dtype) { return dtype == FMD_F32 ? 3 : dtype == FMD_F16 ? 2 : 1; }

@@ -8,7 +8,9 @@
 
 Not part of the reference's surface (its narrowest format is fp16, reference models/gptq.py); conventions are those of
 ``flashmd_amd.kernels``: contiguous GPU tensors, HIP kernels on torch's current stream, fresh outputs, no CPU fallback.
-Dense tensors are float32, float16 or bfloat16, one type within a call.  The gradients are not differentiable again: what tries,
+Dense tensors are float32, float16 or bfloat16, one type within a call.  Sums are held in float32 and results rounded once; a 16-bit
+layer with a side beyond 256 also rounds what it computes for a product (tanh of its input, a gradient times tanh') to 16 bits, as
+torch's own 16-bit operations do.  The gradients are not differentiable again: what tries,
 such as a loss on forces taken with ``create_graph=True``, gets a RuntimeError.
 """
 from __future__ import annotations

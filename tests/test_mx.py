@@ -21,6 +21,19 @@ def test_oracle_blocks_by_hand():
     assert float(values[0, 2]) == 126 / 64 * 4
 
 
+def test_kept_values_of_fp16_inputs_are_fp16_numbers():
+    """What lets a wide fp16 layer hold x8 in one fp16 plane: an fp16 input is a multiple of 2^-24, so that its code is one of 2^-24 / 2^(E-6)
+    where that is more than one, and 127 / 64 2^15 is below fp16's largest.  Every magnitude there is, beside every block exponent."""
+    bits = torch.arange(1, 0x7c00, dtype=torch.int32).to(torch.int16)
+    every = bits.view(torch.float16)                          # ascending: 31743 magnitudes
+    for top in range(-24, 16):                                # the exponent of the block's largest
+        below = every[every.double() < 2.0 ** (top + 1)]
+        below = torch.cat((below, -below, torch.zeros(-2 * below.numel() % 31, dtype=torch.float16))).view(-1, 31)
+        x = torch.cat((torch.full((below.shape[0], 1), 2.0 ** top, dtype=torch.float16), below), dim=1)
+        values = mo.mxint8(x)[2]
+        assert torch.equal(values.half().double(), values)
+
+
 def test_cpu_tensors_are_refused():
     import flashmd_amd.kernels as K
 
