@@ -41,28 +41,37 @@ def _aligned(t: torch.Tensor) -> torch.Tensor:
 def _dense(x: torch.Tensor, what: str = "x") -> int:
     """Checks a dense matrix; its type's number."""
     _ffi.require_gpu(x)
-    assert x.dim() == 2, f"{what} must be a matrix, got {x.dim()} dimensions"
-    assert x.dtype in DTYPES, f"{what} must be float32, float16 or bfloat16, got {x.dtype}"
-    assert x.is_contiguous(), f"{what} must be contiguous"
+    if x.dim() != 2:
+        raise AssertionError(f"{what} must be a matrix, got {x.dim()} dimensions")
+    if x.dtype not in DTYPES:
+        raise AssertionError(f"{what} must be float32, float16 or bfloat16, got {x.dtype}")
+    if not x.is_contiguous():
+        raise AssertionError(f"{what} must be contiguous")
     return DTYPES[x.dtype]
 
 
 def _blocked(codes: torch.Tensor, scales: torch.Tensor, k: int, per_block: int, dtype: torch.dtype):
     _ffi.require_gpu(codes, scales)
-    assert codes.dtype == dtype and scales.dtype == torch.uint8, f"codes must be {dtype} and scales uint8"
-    assert codes.dim() == 2 and scales.dim() == 2 and codes.is_contiguous() and scales.is_contiguous()
-    assert k >= 1 and codes.shape == (scales.shape[0], per_block * blocks(k)) and scales.shape[1] == blocks(k), \
-        f"{k} columns take {blocks(k)} blocks a row: codes {tuple(codes.shape)}, scales {tuple(scales.shape)}"
-    assert codes.device == scales.device
+    if codes.dtype != dtype or scales.dtype != torch.uint8:
+        raise AssertionError(f"codes must be {dtype} and scales uint8")
+    if codes.dim() != 2 or scales.dim() != 2 or not codes.is_contiguous() or not scales.is_contiguous():
+        raise AssertionError("codes and scales must be contiguous matrices")
+    if k < 1 or codes.shape != (scales.shape[0], per_block * blocks(k)) or scales.shape[1] != blocks(k):
+        raise AssertionError(f"{k} columns take {blocks(k)} blocks a row: codes {tuple(codes.shape)}, scales {tuple(scales.shape)}")
+    if codes.device != scales.device:
+        raise AssertionError(f"codes are on {codes.device}, scales on {scales.device}")
 
 
 def _vector(b: Optional[torch.Tensor], n: int, like: torch.Tensor):
     if b is not None:
         _ffi.require_gpu(b)
-        assert b.shape == (n,) and b.dtype == like.dtype and b.is_contiguous() and b.device == like.device, \
-            f"bias must be {n} contiguous {like.dtype} on {like.device}"
+        if b.shape != (n,) or b.dtype != like.dtype or not b.is_contiguous() or b.device != like.device:
+            raise AssertionError(f"bias must be {n} contiguous {like.dtype} on {like.device}")
 
 
+# Arguments that do not fit raise AssertionError, like the package's other operators, but from an ``if``: the kernels trust the sizes,
+# and ``python -O`` drops assert statements.
+#
 # A call's host side costs as much as a small layer's kernels, so it is kept short: the library's functions are looked up once,
 # workspace sizes once a layer shape, pointers go through ctypes as plain integers.
 
@@ -103,7 +112,8 @@ def _launch(device: torch.device, name: str, *args):
 def _quantize(name: str, x, per_block: int, dtype) -> tuple:
     kind = _dense(x)
     m, k = x.shape
-    assert k >= 1, "no columns to quantise"
+    if k < 1:
+        raise AssertionError("no columns to quantise")
     x = _aligned(x.detach())
     codes = torch.empty((m, per_block * blocks(k)), dtype=dtype, device=x.device)
     scales = torch.empty((m, blocks(k)), dtype=torch.uint8, device=x.device)
@@ -113,7 +123,8 @@ def _quantize(name: str, x, per_block: int, dtype) -> tuple:
 
 def _dequantize(name: str, codes, scales, num_columns: int, dtype, per_block: int, code_dtype) -> torch.Tensor:
     _blocked(codes, scales, num_columns, per_block, code_dtype)
-    assert dtype in DTYPES, f"dtype must be float32, float16 or bfloat16, got {dtype}"
+    if dtype not in DTYPES:
+        raise AssertionError(f"dtype must be float32, float16 or bfloat16, got {dtype}")
     codes = _aligned(codes)
     out = torch.empty((codes.shape[0], num_columns), dtype=dtype, device=codes.device)
     _launch(codes.device, name, _at(codes), _at(scales), codes.shape[0], num_columns, _at(out), DTYPES[dtype])
@@ -179,9 +190,11 @@ def _once(backward):
 
 def _check_linear(x, codes, scales, bias, activation) -> int:
     kind = _dense(x)
-    assert activation in (None, "tanh"), f"activation must be None or 'tanh', got {activation!r}"
+    if activation not in (None, "tanh"):
+        raise AssertionError(f"activation must be None or 'tanh', got {activation!r}")
     _blocked(codes, scales, x.shape[1], BLOCK // 2, torch.uint8)
-    assert codes.device == x.device and codes.shape[0] >= 1
+    if codes.device != x.device or codes.shape[0] < 1:
+        raise AssertionError(f"{codes.shape[0]} rows of codes on {codes.device} for x on {x.device}")
     _vector(bias, codes.shape[0], x)
     return kind
 
@@ -303,9 +316,12 @@ class LinearCkpt8Function(torch.autograd.Function):
 def _ckpt8(x, weight, bias, tanh: bool) -> torch.Tensor:
     _dense(x)
     _dense(weight, "weight")
-    assert x.dtype == weight.dtype and x.device == weight.device, "x and weight must have one type and one device"
-    assert x.shape[1] == weight.shape[0], f"Dimension mismatch: x has {x.shape[1]} columns but weight has {weight.shape[0]} rows"
-    assert weight.shape[0] >= 1 and weight.shape[1] >= 1, "an empty weight"
+    if x.dtype != weight.dtype or x.device != weight.device:
+        raise AssertionError("x and weight must have one type and one device")
+    if x.shape[1] != weight.shape[0]:
+        raise AssertionError(f"Dimension mismatch: x has {x.shape[1]} columns but weight has {weight.shape[0]} rows")
+    if weight.shape[0] < 1 or weight.shape[1] < 1:
+        raise AssertionError("an empty weight")
     _vector(bias, weight.shape[1], x)
     return LinearCkpt8Function.apply(x, weight, bias, tanh)[0]
 

@@ -212,6 +212,42 @@ def test_gradients_are_not_differentiated_again(op, monkeypatch):
         assert all(g.shape == t.shape for g, t in zip(torch.autograd.grad(y.sum(), leaves), leaves))
 
 
+def test_sizes_are_checked_under_python_O():
+    """With assert statements dropped: what does not fit is refused before anything is launched (the launch is replaced)."""
+    import os
+    import subprocess
+    import sys
+
+    code = """
+import torch
+import flashmd_amd.kernels as K
+from flashmd_amd import _ffi, mx
+assert False, "assertions are on"
+_ffi.require_gpu = lambda *t: None
+def launched(*a): raise SystemExit("launched " + a[1])
+mx._launch = launched
+x, w, b = torch.zeros(4, 40), torch.zeros(40, 8), torch.zeros(8)
+codes, scales, c8 = torch.zeros(8, 32, dtype=torch.uint8), torch.zeros(8, 2, dtype=torch.uint8), torch.zeros(8, 64, dtype=torch.int8)
+n = 0
+for f in (lambda: K.mxfp4_quantize(x.double()), lambda: K.mxfp4_quantize(x[0]), lambda: K.mxint8_quantize(x.t()), lambda: K.mxfp4_quantize(x[:, :0].contiguous()),
+          lambda: K.mxfp4_dequantize(codes, scales, 65), lambda: K.mxfp4_dequantize(codes[:5], scales, 40), lambda: K.mxint8_dequantize(codes, scales, 40),
+          lambda: K.mxint8_dequantize(c8, scales[:, :1].contiguous(), 40), lambda: K.mxfp4_dequantize(codes, scales, 40, torch.float64),
+          lambda: K.mxfp4_linear(torch.zeros(4, 70), codes, scales), lambda: K.mxfp4_linear(x, codes, scales, b[:7]),
+          lambda: K.mxfp4_linear(x, codes, scales, b.half()), lambda: K.mxfp4_linear(x, codes, scales, activation="relu"),
+          lambda: K.mxfp4_linear_autograd(x, codes[:0], scales[:0]), lambda: K.linear_ckpt8_autograd(x, w[:39]), lambda: K.linear_ckpt8_autograd(x, w.half()),
+          lambda: K.fused_tanh_linear_ckpt8_autograd(x, w, b[:3]), lambda: K.linear_ckpt8_autograd(x, w[:, :0].contiguous())):
+    try:
+        f()
+    except AssertionError as e:
+        n += bool(str(e))
+print("refused", n)
+"""
+    here = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    env = dict(os.environ, PYTHONPATH=os.path.join(here, "flash-molecular-dynamics_amd"))
+    p = subprocess.run([sys.executable, "-O", "-c", code], env=env, capture_output=True, text=True, timeout=110)
+    assert p.stdout.strip() == "refused 18", (p.stdout, p.stderr[-500:])
+
+
 def _model(activation=None):
     import flashmd_amd.schnet as S
 
