@@ -305,11 +305,12 @@ int by_width(const GradArgs& a, int slices, hipStream_t s) {
   return a.n <= 64 ? launch<T, TANH, 4, 2>(a, slices, s) : launch<T, TANH, 4, 4>(a, slices, s);
 }
 
-// part by part of at most 128 x 128, one after the other in the same workspace
+// part by part of at most 128 x 128, one after the other in the same workspace.  The bias's sums come with the first parts along k; for
+// them alone (the same bits as beside gw) the others are left out
 template <class T>
 int run(GradArgs a, bool tanh, int slices, void* gw, void* gb, hipStream_t s) {
   const int k = a.k, n = a.n;
-  for (int k0 = 0; k0 < k; k0 += 128)
+  for (int k0 = 0; k0 < (gw ? k : 1); k0 += 128)
     for (int n0 = 0; n0 < n; n0 += 128) {
       a.k = k - k0 < 128 ? k - k0 : 128, a.n = n - n0 < 128 ? n - n0 : 128, a.n0 = n0, a.block0 = k0 / 32;
       const int nt = a.n <= 64 ? 2 : 4, rows = a.k <= 64 ? 64 : 128;
@@ -349,7 +350,7 @@ template <class T>
 int run_tiles(GradArgs a, bool tanh, void* gw, void* gb, hipStream_t s) {
   const int slices = tile_slices(a.m, a.n, a.k);
   if (slices == 1) a.part = nullptr;
-  const dim3 grid((a.k + 31) / 32, (a.n + 31) / 32, slices);
+  const dim3 grid(gw ? (a.k + 31) / 32 : 1, (a.n + 31) / 32, slices);  // the bias's sums are the first block's
   if (tanh) gradient_tile_kernel<T, true><<<grid, 64 * TILE_WAVES, 0, s>>>(a, (T*)gw, (T*)gb);
   else gradient_tile_kernel<T, false><<<grid, 64 * TILE_WAVES, 0, s>>>(a, (T*)gw, (T*)gb);
   if (slices > 1) gradient_sum_kernel<T><<<((a.k + 1) * a.n + 15) / 16, 256, 0, s>>>(a.part, slices, a.k, a.n, a.k, a.n, a.n, (T*)gw, (T*)gb);

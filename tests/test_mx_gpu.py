@@ -823,3 +823,20 @@ def test_computed_operands_of_narrow_bf16_layers_are_not_rounded(K, m, k, n):
     gx = torch.autograd.grad(y, leaves[0], g.to(DEV))[0]
     if max(k, n) <= 256:
         assert otherwise(gx, (G / torch.cosh(X @ V.t().contiguous()) ** 2) @ V) <= most
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m,k,n", [(1, 40, 33), (300, 128, 128), (1000, 300, 131), (70_000, 50, 128), (99_001, 256, 255)])
+def test_bias_gradient_alone(K, dtype, m, k, n):
+    """Whole numbers: the exact sum rounded once, whatever else is asked for."""
+    gen = torch.Generator().manual_seed(m)
+    g = torch.randint(-2, 3, (m, n), generator=gen).to(dtype).to(DEV)
+    x, w, b = rand(m, k, seed=1, dtype=dtype).to(DEV), rand(k, n, seed=2, dtype=dtype).to(DEV), rand(n, seed=3, dtype=dtype).to(DEV)
+    want = g.double().sum(0).to(dtype)
+    for op in (K.linear_ckpt8_autograd, K.fused_tanh_linear_ckpt8_autograd):
+        leaf, weight = b.clone().requires_grad_(), w.clone().requires_grad_()
+        assert torch.equal(torch.autograd.grad(op(x, w, leaf), leaf, g)[0], want)
+        assert torch.equal(torch.autograd.grad(op(x, weight, leaf), (weight, leaf), g)[1], want)
+        uneven_g = uneven(m, n, torch.float32, seed=4).clamp(-1e3, 1e3).to(dtype).to(DEV)    # and the same bits alone
+        assert torch.equal(torch.autograd.grad(op(x, w, leaf), leaf, uneven_g)[0],
+                           torch.autograd.grad(op(x, weight, leaf), (weight, leaf), uneven_g)[1])
