@@ -840,3 +840,71 @@ def test_bias_gradient_alone(K, dtype, m, k, n):
         uneven_g = uneven(m, n, torch.float32, seed=4).clamp(-1e3, 1e3).to(dtype).to(DEV)    # and the same bits alone
         assert torch.equal(torch.autograd.grad(op(x, w, leaf), leaf, uneven_g)[0],
                            torch.autograd.grad(op(x, weight, leaf), (weight, leaf), uneven_g)[1])
+
+
+class _LayerOnKeptValues(torch.autograd.Function):
+    """p(x) W^T + b in 64 bits whose backward pass has the given kept values of x in its place"""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, kept, tanh):
+        ctx.save_for_backward(weight, kept)
+        ctx.tanh = tanh
+        y = (torch.tanh(x) if tanh else x) @ weight.t()
+        return y if bias is None else y + bias
+
+    @staticmethod
+    def backward(ctx, g):
+        weight, kept = ctx.saved_tensors
+        p = torch.tanh(kept) if ctx.tanh else kept
+        gx = g @ weight
+        return gx / torch.cosh(kept) ** 2 if ctx.tanh else gx, g.t() @ p, g.sum(0) if ctx.needs_input_grad[2] else None, None, None
+
+
+def test_training_step_is_that_of_the_kept_values(monkeypatch):
+    """Every parameter's gradient of a loss of energies against the model in 64 bits that has, layer by layer, the very 8-bit values the GPU
+    kept: what is left is the operator path's fp32 arithmetic, the 1e-4 that the layers without checkpoints are held to."""
+    import copy
+
+    import flashmd_amd.schnet as S
+    from oracle import schnet_oracle as so
+
+    model = S.set_activation_checkpoints(_schnet().to(DEV).train())
+    plain = copy.deepcopy(model).cpu().double()
+    kept = []
+    for name in ("linear_ckpt8_autograd", "fused_tanh_linear_ckpt8_autograd"):
+        def record(x, weight, bias=None, op=getattr(S.K, name)):
+            kept.append((x.detach().cpu().double(), S.K.mxint8_dequantize(*S.K.mxint8_quantize(x), x.shape[1]).cpu().double()))
+            return op(x, weight, bias)
+
+        monkeypatch.setattr(S.K, name, record)
+    e = model(_batch(S)).out["SchNet"]["energy"]
+    got = torch.autograd.grad((e * e).sum(), list(model.parameters()))
+    monkeypatch.undo()
+    assert len(kept) == 2 * 3 + 3
+
+    used = iter(kept)
+
+    def layer(x, linear, tanh):
+        seen, values = next(used)
+        assert rel(seen, x) < 1e-5                            # the same rows in the same order
+        return _LayerOnKeptValues.apply(x, linear.weight, linear.bias, values, tanh)
+
+    def mlp(x, net):
+        for i, linear in enumerate(net.layers[0::2]):
+            x = layer(x, linear, i > 0)
+        return x
+
+    data = _batch(S, "cpu", torch.float64)
+    src, dst = so.radius_graph(data.pos.float(), data.ptr, 5.0)
+    x = plain.embedding_layer(data.atom_types)
+    d = (data.pos[dst] - data.pos[src]).norm(dim=1)
+    rbf = plain.rbf_layer(d)
+    for blk in plain.interaction_blocks:
+        h = blk.conv.lin1(x)
+        wf = mlp(rbf, blk.conv.filter_network) * blk.conv.cutoff(d).view(-1, 1)
+        h = blk.conv.lin2(torch.zeros_like(h).index_add_(0, dst, h[src] * wf))
+        x = x + layer(h, blk.lin, True)
+    energy = torch.zeros(3, dtype=torch.float64).index_add_(0, data.batch, mlp(x, plain.output_network).flatten())
+    want = torch.autograd.grad((energy * energy).sum(), list(plain.parameters()))
+    off = {n: rel(g, w) for (n, _), g, w in zip(model.named_parameters(), got, want)}
+    assert rel(e, energy) < 1e-5 and max(off.values()) < 1e-4, off
