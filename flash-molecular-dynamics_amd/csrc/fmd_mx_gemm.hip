@@ -7,9 +7,9 @@
 //
 // The transforms (tanh, the gradient's tanh', dequantisation) happen in step 1, once per element, or in the epilogue.
 //
-// Bound by the matrix pipe and the reads of LDS that feed it: 8192 x 8192 x 4096 in 151 us from 4-bit operands (3.6 PF); bf16 8192 x 1024 x
-// 4096, with the small tile, in 113 us (0.61 PF); bf16 4096 x 4096 x 4096 against 4-bit weights in 128 us (1.08 PF), the planes' kernels
-// included.
+// 8192 x 8192 x 4096 in 150 us from 4-bit operands (3.7 PF), matrix pipe busy 48 % of the time, no bank conflicts, waves waiting 45 % of
+// theirs: the barrier of each tile, where its loads have to have landed, bounds it.  bf16 8192 x 1024 x 4096, with the small tile, in 101 us
+// (0.68 PF, matrix pipe 51 %); bf16 4096 x 4096 x 4096 against 4-bit weights in 126 us (1.09 PF), the planes' kernels included.
 #include <type_traits>
 
 #include "fmd_mx_host.h"
@@ -612,8 +612,8 @@ void mx_scale_tiles(const void* scales, int64_t rows, int64_t nb, void* out, hip
 
 // The large tile reads each operand half as often and is worth it once its workgroups fill three quarters of the chip; else the small
 // tile, and the contraction in parts.  Calls with 4096 columns of x, us, bf16 planes / both in 4 bits, large against small:
-//   2560 x 4096 (160 large tiles) 133 / 81 against 126 / 48;  2816 x 4352 (187) 153 / 82 against 141 / 55;
-//   8192 x 1536 (192) 120 / 51 against 135 / 57;  3840 x 4096 (240) 124 / 49 against 148 / 56;  4096 x 4096 (256) 128 / 51 against 149 / 57
+//   2560 x 4096 (160 large tiles) 133 / 81 against 125 / 48;  2816 x 4352 (187) 153 / 82 against 141 / 55;
+//   8192 x 1536 (192) 120 / 51 against 135 / 57;  3840 x 4096 (240) 122 / 48 against 148 / 55;  4096 x 4096 (256) 126 / 51 against 147 / 57
 MxProductPlan mx_product_plan(int64_t m, int64_t n, int64_t kt, int npairs) {
   MxProductPlan p{};
   const int64_t big = ((m + 255) / 256) * ((n + 255) / 256), small = ((m + 127) / 128) * ((n + 127) / 128);

@@ -7,12 +7,12 @@
 // wave holds all of gw in its accumulators (up to 128 x 128: 256 of a lane's 512 registers, one wave a SIMD) and takes 16 rows a
 // step, the next step's rows already on their way.  The waves of a workgroup add up in LDS, the workgroups in a second kernel, in a
 // fixed order.  Bound by reading g and the checkpoint once: 262144 x 128 x 128 fp32 under tanh in 116 us, 1.5 TB/s (the 6 products of
-// a term and the tanh come on top of the bytes), bf16 84 us.
+// a term and the tanh come on top of the bytes), bf16 92 us, the sums' kernel included.
 //
 // gradient_tile_kernel, for few rows and any width.  A workgroup makes one 32 x 32 tile of gw from a slice of the rows; its eight
 // waves take 16 rows each in turn.  g and the checkpoint are read once for every tile beside or below, from the caches, but a
 // few rows spread over many workgroups, and a workgroup has 16 sums a lane to bring together instead of 256.  Bound by latency while
-// the rows are few (269 x 128 x 128 fp32: 5.8 us), by those reads later.
+// the rows are few (269 x 128 x 128 fp32: 5.7 us), by those reads later.
 #include <type_traits>
 
 #include "fmd_mx_host.h"
@@ -333,14 +333,14 @@ int slices_for(int dtype, int64_t m, int64_t k) {
 
 // Which kernel: a tile at a time while the rows are few; it reads a narrow layer's rows once for each 32 columns of the other side,
 // the parts' kernel once for each 128, and general products write both operands anew.  Tiles against the other, us, tanh, with sums:
-//   narrow: 1000 x 128 x 128 fp32 8.0 / 50, 65536 fp32 49 / 70, 98304 66 / 77 (bf16 54 / 64), 131072 85 / 85 (bf16 70 / 68), 262144
-//           158 / 116; 98304 x 256 x 200 264 / 305, x 64 x 256 64 / 60
-//   wide:   500 x 1000 x 1000 fp32 24 / 41 (bf16 16 / 29), 1000 42 / 48 (28 / 35), 2000 78 / 62 (52 / 40); 64 x 1024 x 4096 bf16 15 / 16,
-//           128 19 / 17, 300 34 / 21; 5000 x 300 x 300 31 / 59
+//   narrow: 1000 x 128 x 128 fp32 8.1 / 50, 65536 fp32 46 / 70, 98304 71 / 77 (bf16 55 / 67), 131072 85 / 85 (bf16 70 / 72), 262144
+//           160 / 117 (bf16 135 / 92); 98304 x 256 x 200 264 / 306, x 64 x 256 64 / 60
+//   wide:   500 x 1000 x 1000 fp32 23 / 41 (bf16 17 / 29), 1000 40 / 48 (30 / 34), 2000 75 / 63 (56 / 39); 64 x 1024 x 4096 bf16 15 / 16,
+//           128 21 / 18, 300 36 / 21; 5000 x 300 x 300 32 / 58
 constexpr int64_t FEW = 98304, FEW_PRODUCTS = (int64_t)1 << 29;
 bool by_tiles(int64_t m, int64_t n, int64_t k) { return k <= 256 && n <= 256 ? m <= FEW : m * n <= FEW_PRODUCTS / k; }
 // Rows in parts: two steps of 16 for each wave at least, and none up to 512 rows, where the sum over parts is a launch too many (400 x
-// 128 x 128 fp32: 7.1 in one, 7.9 in two; 1000: 13.6 in one, 8.0 in four)
+// 128 x 128 fp32: 7.1 in one, 8.0 in two; 1000: 13.6 in one, 8.0 in four)
 int tile_slices(int64_t m, int64_t n, int64_t k) {
   const int64_t tiles = ((k + 31) / 32) * ((n + 31) / 32), s = (m + 32 * TILE_WAVES - 1) / (32 * TILE_WAVES), most = (512 + tiles - 1) / tiles;
   return (int)(m <= 512 ? 1 : s < most ? s : most);

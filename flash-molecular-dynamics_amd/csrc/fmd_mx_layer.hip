@@ -12,11 +12,11 @@
 // chunk takes columns 8s..8s+7 of either half.  Output column NT*lane + tile: a lane's NT results are neighbours, and a
 // store of one register per tile writes two whole rows.
 //
-// Measured: 1882048 x 50 -> 128 fp32 under tanh, 4-bit weights 263 us (5.1 TB/s; a large copy runs at 5.0), with an 8-bit checkpoint of
-// x 279, the gradient back through tanh' and the bias's sums 504 (4.6 TB/s).  Against the general product, us a call: 256 x 128 x 128 bf16
-// 3.6 / 8.9 (fp32 5.1 / 12), 34432 rows 9 / 15 (12 / 25), 193688 rows 22 / 40 (34 / 96); 256 x 256: 4096 rows 9.5 / 12 (14 / 27), 193688
-// rows 53 / 80 (106 / 205); both operands in 4 bits at 256 x 256: 4096 rows 6.9 / 8.8, 193688 52 / 50, and 34432 24 / 18, the one shape
-// where the product is ahead.
+// Measured: 1882048 x 50 -> 128 fp32 under tanh, 4-bit weights 271 us (4.9 TB/s; a large copy runs at 5.0), with an 8-bit checkpoint of
+// x 278, the gradient back through tanh' and the bias's sums 501 (4.6 TB/s); 1000000 x 128 -> 128 bf16 150 and 171 (5.1 and 4.5 TB/s).
+// Against the general product, us a call in a graph: 256 x 128 x 128 bf16 3.6 / 9.0 (fp32 5.1 / 12), 34432 rows 9 / 15 (12 / 25), 193688
+// rows 20 / 58 (34 / 154); 256 x 256: 4096 rows 9.3 / 12 (14 / 27), 193688 rows 53 / 78 (107 / 231); both operands in 4 bits at
+// 256 x 256: 4096 rows 6.8 / 8.7, 193688 51 / 50, and 34432 24 / 18, the one shape where the product is ahead.
 #include <type_traits>
 
 #include "fmd_mx_host.h"

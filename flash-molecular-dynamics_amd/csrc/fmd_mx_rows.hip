@@ -7,9 +7,10 @@
 // weight's exact bf16 values.  Rows of x that do not exist cost matrix time that is free here.  The waves' sums meet in LDS and
 // are added in a fixed order: one launch, no workspace.
 //
-// Bound by the latency of two rounds of loads: 4096 x 4096 for one row in 5.6 us (1.6 TB/s of weights).  Against the general product, us a
-// call, bf16 x / x in 4 bits: 1 row of 1000 x 1000 4.0 / 4.0 and 17.5 / 14.9, of 4096 x 4096 5.6 / 5.9 and 42 / 18; 64 rows of
-// 1000 x 1000 7.9 / 8.4 and 20 / 17, of 4096 x 4096 19 / 20 and 37 / 23: more rows are the product's.
+// Bound by the latency of two rounds of loads: 4096 x 4096 for one row in 5.8 us (1.5 TB/s of weights) repeated in a graph, 7 to 8.5 by
+// itself between other work.  Against the general product, us a call in a graph, bf16 x / x in 4 bits: 1 row of 1000 x 1000 4.1 / 4.1 and
+// 13.5 / 10.6, of 4096 x 4096 5.8 / 6.0 and 38 / 14.5; 64 rows of 1000 x 1000 7.9 / 8.4 and 16.4 / 13.3, of 4096 x 4096 19.1 / 19.6 and
+// 34.7 / 18.5: more rows are the product's.
 #include "fmd_mx_host.h"
 
 namespace {

@@ -5,6 +5,9 @@ mode.  By default only the weights are narrow: activations stay in the model's t
 the energy the swapped model computes.  ``quantize_activations=True`` also takes every layer's input in its 4-bit blocks; the
 energy is then a step function of the positions and the forces are those of the straight-through gradient, which no longer
 conserve it: for measuring a model, not for running dynamics.  As in W16A16 there is no CPU path.
+
+A swapped model runs on the operator path, not on the fused engine, which holds 32- or 16-bit networks only: energies and forces of 128
+molecules of 269 beads in 10.2 ms, against 14.4 ms on that path in fp32 and 1.75 ms on the engine.
 """
 from __future__ import annotations
 
