@@ -156,22 +156,33 @@ class _NotTwice(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, anchor, grad_output, *gradients):
-        return gradients
+        ctx.set_materialize_grads(False)
+        return tuple(g.new_empty(0).set_(g) for g in gradients)  # the same memory, but no views, which could not be changed in place
 
     @staticmethod
-    def backward(ctx, *_):
+    def backward(ctx, *again):
+        if all(g is None for g in again):  # reached, but with nothing to pass on
+            return (None,) * (2 + len(again))
         raise RuntimeError("flashmd_amd: the gradients of block-scaled layers cannot be differentiated again, so a loss on forces "
                            "cannot be trained through them; use a loss on energies, or the layers they stand for "
                            "(set_activation_checkpoints(model, bits=None))")
 
 
+def _anchored(ctx, y, need: bool) -> tuple:
+    ctx.y_shape = y.shape
+    ctx.set_materialize_grads(False)  # the anchor's would be made each time
+    return y, y.new_empty(0) if need else None
+
+
 def _once(backward):
-    """For a layer whose forward returns (y, anchor) and saves the anchor, an empty output, last.  Under ``create_graph`` the kernels'
+    """For a layer whose forward returns what ``_anchored`` does and saves the anchor, an empty output, last.  Under ``create_graph`` the kernels'
     results would be constants to autograd, and whatever is derived from them would lack their part without a word.  The anchor
     leads to the layer's inputs without keeping them."""
 
     @functools.wraps(backward)
     def wrapper(ctx, grad_output, _):
+        if grad_output is None:  # what comes behind y passed it no gradient
+            grad_output = ctx.saved_tensors[-1].new_zeros(ctx.y_shape)
         if not torch.is_grad_enabled():
             return backward(ctx, grad_output)
         with torch.no_grad():
@@ -233,8 +244,7 @@ class MXFP4LinearFunction(torch.autograd.Function):
         y, dact = _linear(x, codes, scales, bias, DTYPES[x.dtype], tanh, quantize_input, tanh and need and not wide)
         ctx.aux_kind = AUX_NONE if not tanh else AUX_Y if wide else AUX_DACT
         ctx.k = x.shape[1]
-        ctx.set_materialize_grads(False)
-        anchor = x.new_empty(0) if need else None
+        y, anchor = _anchored(ctx, y, need)
         ctx.save_for_backward(codes, scales, y if ctx.aux_kind == AUX_Y else dact, anchor)
         return y, anchor
 
@@ -288,8 +298,7 @@ class LinearCkpt8Function(torch.autograd.Function):
             ws = _workspace(x, "fmd_linear_ckpt8_workspace_bytes", kind, m, n, k)
             _launch(x.device, "fmd_linear_ckpt8", _at(x), kind, _at(w), _at(bias), _at(y), _at(codes), _at(scales), m, n, k, tanh,
                     _at(ws))
-        ctx.set_materialize_grads(False)
-        anchor = x.new_empty(0) if any(ctx.needs_input_grad) else None
+        y, anchor = _anchored(ctx, y, any(ctx.needs_input_grad))
         ctx.save_for_backward(codes, scales, weight, anchor)
         ctx.tanh = tanh
         return y, anchor

@@ -208,6 +208,8 @@ def test_gradients_are_not_differentiated_again(op, monkeypatch):
                 torch.autograd.grad((forces * forces).sum(), leaf, retain_graph=True)
         with pytest.raises(RuntimeError, match="differentiated again"):
             ((forces * forces).sum() + y.sum()).backward(retain_graph=True)
+        for g in torch.autograd.grad(y.sum(), leaves, create_graph=True):
+            g.mul_(2.0)                                       # theirs to change
         # a loss of the outputs beside them is no second derivative
         assert all(g.shape == t.shape for g, t in zip(torch.autograd.grad(y.sum(), leaves), leaves))
 
@@ -246,6 +248,36 @@ print("refused", n)
     env = dict(os.environ, PYTHONPATH=os.path.join(here, "flash-molecular-dynamics_amd"))
     p = subprocess.run([sys.executable, "-O", "-c", code], env=env, capture_output=True, text=True, timeout=110)
     assert p.stdout.strip() == "refused 18", (p.stdout, p.stderr[-500:])
+
+
+class _Unmoved(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x):
+        return x.sum().detach()
+
+    @staticmethod
+    def backward(ctx, g):
+        return None
+
+
+@pytest.mark.parametrize("create_graph", [False, True])
+def test_an_undefined_gradient_counts_as_zeros(create_graph, monkeypatch):
+    """What comes behind a layer may pass it no gradient at all: its own are then those of zeros, in shape and presence."""
+    import flashmd_amd.kernels as K
+    from flashmd_amd import _ffi, mx
+
+    seen = []
+    monkeypatch.setattr(_ffi, "require_gpu", lambda *t: None)
+    monkeypatch.setattr(mx, "_launch", lambda device, name, *a: seen.append(name))
+    x, w, b = (torch.randn(*s, requires_grad=True) for s in ((5, 40), (40, 6), (6,)))
+    codes, scales = torch.zeros(6, 32, dtype=FP4), torch.zeros(6, 2, dtype=torch.uint8)
+    for y, leaves, name in ((K.fused_tanh_linear_ckpt8_autograd(x, w, b), (x, w, b), "fmd_linear_ckpt8_bwd"),
+                            (K.mxfp4_linear_autograd(x, codes, scales, b, "tanh"), (x, b), "fmd_mxfp4_linear_bwd")):
+        got = torch.autograd.grad(_Unmoved.apply(y), leaves, create_graph=create_graph)
+        assert seen[-1] == name and all(g.shape == t.shape for g, t in zip(got, leaves))
+    y = K.linear_ckpt8_autograd(x, w, b)                      # nor the gradient one of its own
+    gx = torch.autograd.grad(y.sum(), x, create_graph=True)[0]
+    assert torch.autograd.grad(_Unmoved.apply(gx) + (w * 0.0).sum(), w)[0].shape == w.shape
 
 
 def _model(activation=None):
