@@ -3,7 +3,7 @@
 // reference's Triton path drops).  Replaces K6/K7 + K10/K2 (kernels/cfconv_kernels.py:973-1035,
 // 1174-1208,178-258; csr_kernels.py:302-396) and the autograd chain through them on the whole-path route.
 // Compiled twice, as the forward kernel's file: as itself the fp32-grade kernels with scalar pair arithmetic;
-// included by fmd_engine_edge_bwd_half.hip with FMD_HALF_TU set, the W16A16 kernels with the packed pair type.
+// included by fmd_engine_edge_bwd_half.hip with FMD_HALF_TU set, the W16A16 kernels with pairs as vectors.
 #ifndef FMD_HALF_TU
 #define FMD_SCALAR_PAIRS 1
 #endif

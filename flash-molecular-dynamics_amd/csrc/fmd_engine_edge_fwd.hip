@@ -5,8 +5,9 @@
 // This file is compiled twice: as itself it holds the fp32-grade kernels, whose pair arithmetic is SCALAR
 // (FMD_SCALAR_PAIRS, fmd_engine.h: packed fp32 cannot issue beside the partner wave's MFMAs, and these kernels are three
 // MFMAs per product); fmd_engine_edge_fwd_half.hip includes it with FMD_HALF_TU set and holds the W16A16 kernels, one
-// MFMA per product, with pairs as vectors of two floats (faster as long as packed instructions were allowed: same-box A/B,
-// profiles/r05_ab_packed_half.txt; the library is built without them, see the Makefile).
+// MFMA per product, with pairs as vectors of two floats (the library is built without packed fp32 instructions, see the Makefile;
+// with them this type gained 2.0-2.6 %, profiles/r05_ab_packed_half.txt; without, it is level with the scalar one or ahead: timestep
+// of 128 molecules 118.8k and 118.1k against 117.9k and 116.2k).
 #ifndef FMD_HALF_TU
 #define FMD_SCALAR_PAIRS 1
 #endif
